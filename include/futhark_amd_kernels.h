@@ -323,6 +323,123 @@ int fa_matmul_ws(fa_stream_t stream, fa_dtype in_t,
                  int64_t batch, int64_t M, int64_t N, int64_t K,
                  void *workspace, size_t workspace_bytes);
 
+/* --------------------------------------------- attention over packed sequences
+ * No counterpart in the reference: these launchers stand beside fa_matmul (the
+ * products) and fa_segred_irregular (the segments) for a program that runs the
+ * attention of a language model.
+ *
+ * Arrays of rows of heads: component d of head h of row r is element
+ * r * row_stride + h * head_stride + d of `data` (strides count elements), so
+ * that queries, keys and values may be parts of one wider row, and heads may
+ * come before rows.  data is 16-byte aligned and strides are multiples of 8
+ * (FA_EALIGN); strides are not negative, and in an array that is written no two
+ * elements share a place (FA_EINVAL).  A read array may repeat rows or heads
+ * with a stride of 0; the gradient then has one entry per row and head and is
+ * the caller's to sum.
+ *
+ * Element types: FA_F16 and FA_BF16.  head_dim is a multiple of 8, 8 to 128;
+ * heads is a multiple of kv_heads, and query head h reads key and value head
+ * h / (heads / kv_heads), at most 128 query heads to one.  Other types, sizes
+ * and groups return FA_ENOTSUP.  Products are summed and softmax statistics
+ * kept in f32.
+ *
+ * Sequences are segments of the rows, offsets[i] and lens[i] for i < m, on the
+ * device, under the rules of fa_segred_irregular (in order, disjoint, inside
+ * the n rows; n and m below 2^31).  Rows in no segment are neither read nor
+ * written.  A segment that breaks the rules (or has a length or page number out
+ * of range, below) is detected on the device: `code` is stored into *failure
+ * (device-visible memory; NULL: not reported), the segment is left out, and
+ * nothing outside the arrays is touched.
+ *
+ * Nothing is allocated and no state is kept between calls: launches may be
+ * captured into a graph, and calls on several streams may overlap as long as
+ * they do not share outputs or workspace.
+ * Results do not depend on timing (no floating-point atomics). */
+typedef struct fa_heads {
+  void *data;
+  int64_t row_stride, head_stride;
+} fa_heads;
+
+/* Segment i of q attends to segment i of k and v:
+ *   out_i = sum_j p_ij v_j,  p_ij = exp(scale q_i.k_j - lse_i),
+ *   lse_i = log sum_j exp(scale q_i.k_j)
+ * over all j of the segment, or, if causal, over j <= i + (k length - q length)
+ * (i, j counted from the start of their segments: the last query sees every
+ * key).  A row that sees no key, or only keys of score -inf, gives out = 0 and
+ * lse = -inf.  Keys that a row does not see have no effect on it, whatever
+ * values they hold.  scale is positive and finite.  lse: [q_rows][heads] f32,
+ * or NULL.  A pair of q and k segments where either is invalid is left out. */
+int fa_attention(fa_stream_t stream, fa_dtype t, const fa_heads *q, int64_t q_rows,
+                 const fa_heads *k, const fa_heads *v, int64_t k_rows,
+                 int64_t heads, int64_t kv_heads, int64_t head_dim,
+                 const int64_t *q_offsets, const int64_t *q_lens,
+                 const int64_t *k_offsets, const int64_t *k_lens, int64_t m,
+                 float scale, int causal, const fa_heads *out, float *lse,
+                 int32_t *failure, int32_t code);
+
+/* Gradients of fa_attention's out with respect to q, k and v, given dout and
+ * what fa_attention returned for the same arguments (out and lse):
+ *   D_i = dout_i.out_i,  ds_ij = p_ij (dout_i.v_j - D_i),
+ *   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij dout_i,
+ * dk and dv summed over the query heads of a key head as well.  Rows in no
+ * segment keep what they held.  Unlike in fa_attention, non-finite values in a
+ * segment may spread to other rows of that segment.  workspace:
+ * fa_attention_grad_workspace_bytes() bytes, 16-byte aligned, contents
+ * irrelevant. */
+size_t fa_attention_grad_workspace_bytes(int64_t q_rows, int64_t k_rows, int64_t heads, int64_t kv_heads,
+                                         int64_t head_dim, int64_t m);
+int fa_attention_grad(fa_stream_t stream, fa_dtype t, const fa_heads *q, int64_t q_rows,
+                      const fa_heads *k, const fa_heads *v, int64_t k_rows,
+                      int64_t heads, int64_t kv_heads, int64_t head_dim,
+                      const int64_t *q_offsets, const int64_t *q_lens,
+                      const int64_t *k_offsets, const int64_t *k_lens, int64_t m,
+                      float scale, int causal, const fa_heads *out, const float *lse,
+                      const fa_heads *dout, const fa_heads *dq, const fa_heads *dk, const fa_heads *dv,
+                      void *workspace, size_t workspace_bytes, int32_t *failure, int32_t code);
+
+/* A paged cache of keys and values: k_pages and v_pages are
+ * [n_pages][kv_heads][page_size][head_dim], page_size a power of two
+ * (FA_ENOTSUP otherwise), 16-byte aligned; page_table is [m][table_cols] i32,
+ * and position p of sequence i lives in slot p % page_size of page
+ * page_table[i][p / page_size].  table_cols * page_size is below 2^31.
+ * Sequence i holds past_lens[i] tokens before the new ones, lens[i] tokens at
+ * rows offsets[i]...; past + new must fit its table row.
+ *
+ * fa_kv_append writes the new tokens' keys and values into the cache at
+ * positions past_lens[i], past_lens[i] + 1, ...; the first rot_dim components
+ * of every key (and of every query, into q_out, if q is not NULL) are rotated
+ * in pairs (a, b) -> (a cos x - b sin x, b cos x + a sin x) by
+ * x = position * freqs[c], c < rot_dim / 2 (f32, device; the product is taken
+ * in f64).  Pair c is components (2c, 2c+1) if interleaved, else
+ * (c, c + rot_dim/2).  rot_dim is even, 0 to head_dim; components beyond it
+ * are copied.  q_out may be q itself.  A token whose page number is not in
+ * [0, n_pages) is not stored (its query is still rotated).  Two tokens of one
+ * call that share a slot race. */
+int fa_kv_append(fa_stream_t stream, fa_dtype t, const fa_heads *q, const fa_heads *q_out,
+                 const fa_heads *k, const fa_heads *v, int64_t n,
+                 int64_t heads, int64_t kv_heads, int64_t head_dim,
+                 const int64_t *offsets, const int64_t *lens, int64_t m, const int64_t *past_lens,
+                 const float *freqs, int64_t rot_dim, int interleaved,
+                 void *k_pages, void *v_pages, int64_t n_pages, int64_t page_size,
+                 const int32_t *page_table, int64_t table_cols, int32_t *failure, int32_t code);
+
+/* Attention of the new tokens over the cache that already holds them: new
+ * token t of sequence i sees positions 0 .. past_lens[i] + t (fa_attention's
+ * formulas, causal).  Slots past the end of a sequence are never used; a page
+ * number out of range stands for a page of zeros.  lse: [n][heads] f32 or NULL.
+ * workspace: fa_attention_paged_workspace_bytes() bytes for the same sizes,
+ * 16-byte aligned, contents irrelevant (NULL if that is 0). */
+size_t fa_attention_paged_workspace_bytes(int64_t n, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                          int64_t m, int64_t page_size, int64_t table_cols);
+int fa_attention_paged(fa_stream_t stream, fa_dtype t, const fa_heads *q, int64_t n,
+                       int64_t heads, int64_t kv_heads, int64_t head_dim,
+                       const int64_t *offsets, const int64_t *lens, int64_t m,
+                       const int64_t *past_lens, float scale,
+                       const void *k_pages, const void *v_pages, int64_t n_pages, int64_t page_size,
+                       const int32_t *page_table, int64_t table_cols,
+                       const fa_heads *out, float *lse, void *workspace, size_t workspace_bytes,
+                       int32_t *failure, int32_t code);
+
 /* Scan with a vector operator: out[i][j] = xss[0][j] op ... op xss[i][j] for
  * xss, out : [n][k], without a transposed copy.  Replaces: the SegScan of
  * `scan (map2 op) (replicate k ne) xss`, which the reference compiles with its

@@ -1,0 +1,655 @@
+"""GPU parity of the attention operators with their formulas in 64 bits (attention_reference.py
+derives the bounds): packed prompts forward and backward, the paged cache and attention over it."""
+import math
+
+import numpy as np
+import pytest
+
+from futhark_amd import Kernels, heads
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+import attention_reference as ref  # noqa: E402
+
+DEV = "cuda"
+MARK = 7.0  # what outputs hold before a call
+
+
+@pytest.fixture(scope="module")
+def K():
+    return Kernels()
+
+
+def view(x):
+    return heads(x.data_ptr(), x.stride(0), x.stride(1))
+
+
+def randn(gen, t, *shape, scale=1.0):
+    return (torch.randn(*shape, generator=gen, device=DEV) * scale).to(ref.DTYPE[t])
+
+
+def generator(seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    return g
+
+
+def segments(lens, gaps):
+    """(first, length) pairs with gaps[i] rows before segment i, and the rows in all (some behind
+    the last)."""
+    segs, at = [], 0
+    for i, n in enumerate(lens):
+        at += gaps[i % len(gaps)]
+        segs.append((at, n))
+        at += n
+    return segs, at + gaps[0] + 3
+
+
+def device_segments(segs):
+    return (torch.tensor([s[0] for s in segs], dtype=torch.int64, device=DEV),
+            torch.tensor([s[1] for s in segs], dtype=torch.int64, device=DEV))
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+class Problem:
+    """One packed batch; layout "rows" is [rows][heads][dim], "heads" is [heads][rows][dim],
+    "fused" has q, k and v as parts of one row."""
+
+    def __init__(self, t, h, hk, dim, q_lens, k_lens=None, causal=True, layout="rows", gaps=(0,), seed=0,
+                 spread=1.0):
+        gen = generator(seed)
+        self.t, self.h, self.hk, self.dim, self.causal = t, h, hk, dim, causal
+        self.segs_q, self.nq = segments(q_lens, gaps)
+        self.segs_k, self.nk = segments(q_lens if k_lens is None else k_lens, gaps)
+        self.scale = 1 / math.sqrt(dim)
+
+        def make(rows, n, scale=1.0):
+            if layout == "heads":
+                return randn(gen, t, n, rows, dim, scale=scale).transpose(0, 1)
+            return randn(gen, t, rows, n, dim, scale=scale)
+
+        if layout == "fused":
+            x = randn(gen, t, self.nq, h + 2 * hk, dim, scale=spread)
+            self.q, self.k, self.v = x[:, :h], x[:, h:h + hk], x[:, h + hk:]
+        else:
+            self.q, self.k, self.v = make(self.nq, h, spread), make(self.nk, hk, spread), make(self.nk, hk)
+        self.dout = make(self.nq, h)
+        self.out, self.dq, self.dk, self.dv = (torch.full_like(x, MARK) for x in (self.q, self.q, self.k, self.v))
+        self.lse = torch.full((self.nq, h), MARK, dtype=torch.float32, device=DEV)
+        self.qo, self.ql = device_segments(self.segs_q)
+        self.ko, self.kl = device_segments(self.segs_k)
+        self.failure = torch.zeros(1, dtype=torch.int32, device=DEV)
+
+    def args(self):
+        return (self.t, view(self.q), self.nq, view(self.k), view(self.v), self.nk, self.h, self.hk, self.dim,
+                self.qo.data_ptr(), self.ql.data_ptr(), self.ko.data_ptr(), self.kl.data_ptr(), len(self.segs_q),
+                self.scale, int(self.causal), view(self.out))
+
+    def forward(self, K, lse=True):
+        K.attention(stream(), *self.args(), self.lse.data_ptr() if lse else None, self.failure.data_ptr(), 5)
+
+    def backward(self, K):
+        size = K.attention_grad_workspace_bytes(self.nq, self.nk, self.h, self.hk, self.dim, len(self.segs_q))
+        self.workspace = torch.full((max(size, 1),), 0xff, dtype=torch.uint8, device=DEV)
+        K.attention_grad(stream(), *self.args(), self.lse.data_ptr(), view(self.dout), view(self.dq), view(self.dk),
+                         view(self.dv), self.workspace.data_ptr(), size, self.failure.data_ptr(), 5)
+
+    def check_forward(self, lse=True):
+        out, l, tol_o, tol_l = ref.forward(self.t, self.q, self.k, self.v, self.segs_q, self.segs_k, self.scale,
+                                           self.causal)
+        outside = out.isnan()
+        assert bool((self.out[outside] == MARK).all()), "rows in no segment were written"
+        ref.within(self.out, out, tol_o)
+        if lse:
+            assert bool((self.lse[l.isnan()] == MARK).all())
+            ref.within(self.lse, l, tol_l)
+        assert self.failure.item() == 0
+
+    def check_backward(self):
+        grads, tols = ref.gradient(self.t, self.q, self.k, self.v, self.dout, self.segs_q, self.segs_k, self.scale,
+                                   self.causal)
+        for got, want, tol in zip((self.dq, self.dk, self.dv), grads, tols):
+            assert bool((got[want.isnan()] == MARK).all()), "rows in no segment were written"
+            ref.within(got, want, tol)
+        assert self.failure.item() == 0
+
+
+RAGGED = [1, 0, 2, 63, 64, 65, 31, 33, 127, 128, 129, 200, 0]
+PROMPTS = [
+    # type, heads, kv_heads, dim, q lengths, k lengths (None: the same), causal, layout, gaps
+    ("bf16", 2, 1, 128, RAGGED, None, True, "rows", (0,)),
+    ("f16", 2, 2, 64, RAGGED, None, True, "rows", (3, 0, 1)),
+    ("f16", 3, 1, 128, RAGGED, None, False, "fused", (0, 2)),
+    ("bf16", 4, 2, 64, RAGGED, None, False, "heads", (1,)),
+    ("bf16", 1, 1, 8, [1], None, True, "rows", (0,)),
+    ("f16", 1, 1, 8, [5, 70], None, False, "rows", (0,)),
+    ("bf16", 5, 1, 72, [130, 17], None, True, "fused", (0,)),
+    ("f16", 6, 2, 96, [257], None, True, "heads", (0,)),
+    ("bf16", 16, 1, 120, [90, 3], None, True, "rows", (5,)),
+    ("f16", 128, 1, 64, [7, 40], None, True, "rows", (0,)),
+    ("bf16", 127, 1, 16, [70], None, True, "rows", (0,)),
+    ("bf16", 8, 8, 128, [513, 1030], None, True, "rows", (0,)),
+    ("f16", 8, 2, 64, [1537], None, True, "rows", (0,)),
+    # rows with nothing to see, queries behind cached keys, keys nobody asks
+    ("bf16", 2, 1, 128, [100, 70, 5, 9, 0, 130], [40, 0, 1, 200, 30, 129], True, "rows", (0,)),
+    ("f16", 4, 1, 64, [100, 70, 5, 9, 0, 300], [40, 0, 1, 200, 30, 131], True, "rows", (2,)),
+    ("bf16", 2, 2, 40, [3, 260], [700, 0], False, "rows", (0,)),
+    ("f16", 6, 3, 128, [1, 1, 1], [1, 900, 64], True, "rows", (0,)),
+]
+
+
+@pytest.mark.parametrize("i", range(len(PROMPTS)))
+def test_prompts_forward(K, i):
+    p = Problem(*PROMPTS[i], seed=i)
+    p.forward(K)
+    p.check_forward()
+    lse = p.lse.clone()
+    p.out.fill_(MARK)
+    p.lse.fill_(MARK)
+    p.forward(K, lse=False)
+    p.check_forward(lse=False)
+    assert bool((p.lse == MARK).all()) and lse.shape == p.lse.shape
+
+
+@pytest.mark.parametrize("i", range(len(PROMPTS)))
+def test_prompts_backward(K, i):
+    p = Problem(*PROMPTS[i], seed=100 + i)
+    p.forward(K)
+    p.backward(K)
+    p.check_backward()
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_wide_scores(K, t, dim):
+    """Scores spread over hundreds: weights of one, weights that vanish, maxima that move late."""
+    p = Problem(t, 4, 2, dim, [300, 129], spread=6.0, seed=3)
+    order = torch.arange(p.nk, device=DEV, dtype=torch.float32) / 100
+    p.k.copy_((p.k.float() * order[:, None, None]).to(p.k.dtype))  # later keys have larger scores
+    p.forward(K)
+    p.check_forward()
+    p.backward(K)
+    p.check_backward()
+
+
+def test_gradient_against_differences(K):
+    """The derivative of sum(out * dout) along a direction, by central differences in 64 bits."""
+    p = Problem("f16", 4, 2, 64, [70, 33], [90, 20], seed=9)
+    p.forward(K)
+    p.backward(K)
+    gen = generator(10)
+    grads, tols = ref.gradient(p.t, p.q, p.k, p.v, p.dout, p.segs_q, p.segs_k, p.scale, p.causal)
+    for i, name in enumerate("qkv"):
+        d = torch.randn(getattr(p, name).shape, generator=gen, device=DEV, dtype=torch.float64)
+
+        def loss(step):
+            x = {n: getattr(p, n).double() for n in "qkv"}
+            x[name] = x[name] + step * d
+            out = ref.forward(p.t, x["q"], x["k"], x["v"], p.segs_q, p.segs_k, p.scale, p.causal)[0]
+            return float(torch.nansum(out * p.dout.double()))
+
+        h = 1e-4  # third derivatives times h^2 stay below 1e-6 of the sum's terms
+        slope = (loss(h) - loss(-h)) / (2 * h)
+        got = (p.dq, p.dk, p.dv)[i].double()
+        inside = ~grads[i].isnan()
+        along = float((got * d)[inside].sum())
+        tol = float((tols[i] * d.abs())[inside].sum()) * 0.2 + 1e-4
+        # 0.2: errors of thousands of elements with random signs add like their root; a wrong
+        # factor or sign moves the sum by far more
+        assert abs(along - slope) <= tol, (name, along, slope, tol)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf"), 65504.0])
+def test_keys_that_are_not_seen_have_no_effect(K, causal, bad):
+    """NaN and infinities in rows behind a sequence, between sequences and, under a causal mask, in
+    the future of a row change nothing for that row."""
+    lens = [37, 100, 129, 64]
+    clean = Problem("f16", 4, 2, 64, lens, causal=causal, gaps=(2, 5), seed=21)
+    dirty = Problem("f16", 4, 2, 64, lens, causal=causal, gaps=(2, 5), seed=21)
+    inside = torch.zeros(clean.nk, dtype=torch.bool, device=DEV)
+    for f, n in clean.segs_k:
+        inside[f:f + n] = True
+    dirty.k[~inside] = bad
+    dirty.v[~inside] = bad
+    clean.forward(K)
+    dirty.forward(K)
+    clean.check_forward()
+    assert torch.equal(clean.out, dirty.out) and torch.equal(clean.lse, dirty.lse)
+    if not causal:
+        return
+    for hole in (20, 36):  # token `hole` of every sequence long enough: rows before it are untouched
+        for x in ("k", "v"):
+            d = Problem("f16", 4, 2, 64, lens, causal=True, gaps=(2, 5), seed=21)
+            for f, n in d.segs_k:
+                getattr(d, x)[f + hole, :, 3] = bad
+            d.forward(K)
+            for f, n in d.segs_k:
+                assert torch.equal(clean.out[f:f + hole], d.out[f:f + hole]), (hole, x)
+                if bad != 65504.0 and x == "v":  # and rows from it on see it
+                    assert not bool(d.out[f + hole:f + n, :, 3].isfinite().any())
+                    rest = [c for c in range(64) if c != 3]
+                    assert torch.equal(d.out[f + hole:f + n][..., rest], clean.out[f + hole:f + n][..., rest])
+
+
+def test_broken_segments_are_reported_and_left_out(K):
+    for which, seg, what in [("ql", 1, -1), ("ql", 2, 1 << 40), ("qo", 1, -5), ("qo", 2, 3), ("kl", 1, -7),
+                             ("ko", 0, 1 << 62), ("kl", 2, 1 << 62), ("ko", 1, -(1 << 63)), ("ql", 0, (1 << 63) - 1)]:
+        p = Problem("bf16", 2, 1, 64, [40, 50, 60], gaps=(1,), seed=30)
+        getattr(p, which)[seg] = what
+        p.forward(K)
+        assert p.failure.item() == 5, (which, seg, what)
+        f, n = p.segs_q[seg]
+        assert bool((p.out[f:f + n] == MARK).all())
+        p.failure.zero_()
+        p.backward(K)
+        assert p.failure.item() == 5, (which, seg, what)
+        if seg > 0:  # the segment before the broken one has its values
+            q = Problem("bf16", 2, 1, 64, [40, 50, 60], gaps=(1,), seed=30)
+            q.forward(K)
+            a, b = q.segs_q[0]
+            assert torch.equal(q.out[a:a + b], p.out[a:a + b])
+
+
+def test_without_a_failure_word_and_without_segments(K):
+    p = Problem("bf16", 2, 1, 64, [40], seed=31)
+    p.ql[0] = -1
+    K.attention(stream(), *p.args(), None, None, 0)
+    torch.cuda.synchronize()
+    assert bool((p.out == MARK).all())
+    p = Problem("bf16", 2, 1, 64, [0, 0], seed=31)
+    p.forward(K)
+    p.backward(K)
+    p.check_forward()
+    p.check_backward()
+
+
+def test_repeated_rows_of_keys(K):
+    """Strides of 0 in what is read: every head shares one key head's memory."""
+    p = Problem("f16", 4, 4, 64, [50], seed=32)
+    k1, v1 = randn(generator(1), "f16", p.nk, 64), randn(generator(2), "f16", p.nk, 64)
+    p.k, p.v = k1[:, None].expand(-1, 4, -1), v1[:, None].expand(-1, 4, -1)
+    p.forward(K)
+    p.check_forward()
+    p.backward(K)
+    p.check_backward()
+
+
+def test_many_segments(K):
+    lens = [(7 * i) % 5 for i in range(1000)]
+    p = Problem("bf16", 2, 2, 64, lens, gaps=(0, 1), seed=33)
+    p.forward(K)
+    p.check_forward()
+    p.backward(K)
+    p.check_backward()
+
+
+def test_another_stream_and_the_same_bits_again(K):
+    p = Problem("bf16", 8, 2, 128, [400, 77], seed=34)
+    p.forward(K)
+    p.backward(K)
+    first = [x.clone() for x in (p.out, p.lse, p.dq, p.dk, p.dv)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for x in (p.out, p.dq, p.dk, p.dv, p.lse):
+            x.fill_(MARK)
+        p.forward(K)
+        p.backward(K)
+    torch.cuda.current_stream().wait_stream(side)
+    for a, b in zip(first, (p.out, p.lse, p.dq, p.dk, p.dv)):
+        assert torch.equal(a, b)
+
+
+def test_captured_and_replayed(K):
+    p = Problem("f16", 4, 2, 64, [150, 30], seed=35)
+    size = K.attention_grad_workspace_bytes(p.nq, p.nk, p.h, p.hk, p.dim, 2)
+    ws = torch.empty(max(size, 1), dtype=torch.uint8, device=DEV)
+
+    def step():
+        K.attention(stream(), *p.args(), p.lse.data_ptr(), p.failure.data_ptr(), 5)
+        K.attention_grad(stream(), *p.args(), p.lse.data_ptr(), view(p.dout), view(p.dq), view(p.dk), view(p.dv),
+                         ws.data_ptr(), size, p.failure.data_ptr(), 5)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for seed in (1, 2, 3):
+        for i, x in enumerate((p.q, p.k, p.v, p.dout)):
+            x.copy_(randn(generator(10 * seed + i), "f16", *x.shape))
+        p.ql[0], p.kl[0] = 150 - 10 * seed, 150 - 10 * seed  # lengths may change between replays
+        p.segs_q[0] = p.segs_k[0] = (0, 150 - 10 * seed)
+        for x in (p.out, p.dq, p.dk, p.dv, p.lse):
+            x.fill_(MARK)
+        graph.replay()
+        torch.cuda.synchronize()
+        p.check_forward()
+        p.check_backward()
+
+
+# ------------------------------------------------------------------------ the paged cache
+class Cache:
+    def __init__(self, t, h, hk, dim, page, new, past, gaps=(0,), seed=0, extra_cols=0):
+        gen = generator(seed)
+        self.t, self.h, self.hk, self.dim, self.page, self.past = t, h, hk, dim, page, past
+        self.segs, self.n = segments(new, gaps)
+        need = [-(-(n + p) // page) for n, p in zip(new, past)]
+        self.cols, self.pages = max(need) + extra_cols, sum(need) + 2
+        order = torch.randperm(self.pages, generator=gen, device=DEV).cpu().numpy()
+        table = np.full((len(new), self.cols), -1, np.int32)  # places no sequence needs are out of range
+        at = 0
+        for s, c in enumerate(need):
+            table[s, :c] = order[at:at + c]
+            at += c
+        self.table = torch.from_numpy(table).to(DEV)
+        self.kp, self.vp = (randn(gen, t, self.pages, hk, page, dim) for _ in range(2))
+        self.q, self.k, self.v = (randn(gen, t, self.n, x, dim) for x in (h, hk, hk))
+        self.out = torch.full_like(self.q, MARK)
+        self.lse = torch.full((self.n, h), MARK, dtype=torch.float32, device=DEV)
+        self.offsets, self.lens = device_segments(self.segs)
+        self.past_lens = torch.tensor(past, dtype=torch.int64, device=DEV)
+        self.failure = torch.zeros(1, dtype=torch.int32, device=DEV)
+        self.scale = 1 / math.sqrt(dim)
+        size = Kernels().attention_paged_workspace_bytes(self.n, h, hk, dim, len(new), page, self.cols)
+        self.size, self.workspace = size, torch.full((max(size, 1),), 0xff, dtype=torch.uint8, device=DEV)
+
+    def cache(self):
+        return (self.kp.data_ptr(), self.vp.data_ptr(), self.pages, self.page, self.table.data_ptr(), self.cols)
+
+    def append(self, K, freqs, rot, interleaved, q=True, q_out=None):
+        q_out = self.out if q_out is None else q_out
+        K.kv_append(stream(), self.t, view(self.q) if q else None, view(q_out) if q else None, view(self.k),
+                    view(self.v), self.n, self.h, self.hk, self.dim, self.offsets.data_ptr(), self.lens.data_ptr(),
+                    len(self.segs), self.past_lens.data_ptr(), freqs.data_ptr() if rot else None, rot,
+                    int(interleaved), *self.cache(), self.failure.data_ptr(), 6)
+
+    def attend(self, K, q=None, lse=True):
+        q = self.q if q is None else q
+        K.attention_paged(stream(), self.t, view(q), self.n, self.h, self.hk, self.dim, self.offsets.data_ptr(),
+                          self.lens.data_ptr(), len(self.segs), self.past_lens.data_ptr(), self.scale, *self.cache(),
+                          view(self.out), self.lse.data_ptr() if lse else None, self.workspace.data_ptr(), self.size,
+                          self.failure.data_ptr(), 6)
+
+    def gathered(self):
+        """Keys and values of all sequences, packed, and their segments."""
+        ks, vs, segs, at = [], [], [], 0
+        for s, ((_, n), p) in enumerate(zip(self.segs, self.past)):
+            ids = self.table[s, :-(-(n + p) // self.page)].long()
+            for pages, out in ((self.kp, ks), (self.vp, vs)):
+                x = pages[ids].transpose(1, 2).reshape(-1, self.hk, self.dim)[:n + p]
+                out.append(x)
+            segs.append((at, n + p))
+            at += n + p
+        return torch.cat(ks), torch.cat(vs), segs
+
+    def check(self, q=None):
+        k, v, segs = self.gathered()
+        out, lse, tol_o, tol_l = ref.forward(self.t, self.q if q is None else q, k, v, self.segs, segs, self.scale, True)
+        assert bool((self.out[out.isnan()] == MARK).all()) and bool((self.lse[lse.isnan()] == MARK).all())
+        ref.within(self.out, out, tol_o)
+        ref.within(self.lse, lse, tol_l)
+        assert self.failure.item() == 0
+
+    def positions(self):
+        pos = torch.full((self.n,), -1, dtype=torch.int64, device=DEV)
+        for (f, n), p in zip(self.segs, self.past):
+            pos[f:f + n] = torch.arange(p, p + n, device=DEV)
+        return pos
+
+
+PAGED = [
+    # type, heads, kv_heads, dim, page, new tokens, cached tokens, gaps, extra columns
+    ("bf16", 4, 1, 128, 16, [1, 1, 1, 1], [0, 1, 15, 700], (0,), 0),
+    ("f16", 8, 8, 64, 16, [1, 1, 1], [31, 32, 33], (0,), 5),
+    ("bf16", 6, 2, 96, 32, [1, 0, 1, 1], [1000, 7, 63, 64], (1, 0), 0),
+    ("f16", 3, 1, 72, 1, [1, 2], [40, 129], (0,), 1),
+    ("bf16", 32, 1, 128, 64, [1, 1], [257, 2000], (0,), 0),
+    ("f16", 40, 1, 64, 8, [1, 1, 3], [5, 300, 90], (0,), 0),
+    ("bf16", 128, 1, 64, 16, [1, 4], [200, 77], (0,), 0),
+    ("f16", 8, 2, 64, 4, [5, 9, 0, 2], [100, 0, 50, 1027], (2,), 0),
+    ("bf16", 4, 4, 128, 128, [70, 1, 200], [300, 90, 0], (0, 3), 2),
+    ("f16", 6, 2, 128, 2, [129, 64], [63, 128], (0,), 0),
+    ("bf16", 5, 1, 8, 16, [33], [0], (0,), 0),
+    ("f16", 8, 1, 64, 256, [300, 30], [5000, 1], (0,), 40),
+    ("bf16", 8, 2, 128, 16, [1], [20000], (0,), 0),       # a long axis and few rows
+    ("f16", 4, 1, 64, 32, [3], [9001], (0,), 300),
+    ("bf16", 2, 1, 64, 16, [1] * 300, [(37 * i) % 90 for i in range(300)], (0,), 0),
+]
+
+
+@pytest.mark.parametrize("i", range(len(PAGED)))
+def test_paged(K, i):
+    *p, gaps, extra = PAGED[i]
+    c = Cache(*p, gaps=gaps, seed=200 + i, extra_cols=extra)
+    c.attend(K)
+    c.check()
+    c.out.fill_(MARK)
+    before = c.lse.clone()
+    c.lse.fill_(MARK)
+    c.attend(K, lse=False)
+    assert bool((c.lse == MARK).all())
+    c.lse.copy_(before)
+    c.check()
+
+
+@pytest.mark.parametrize("i", [0, 2, 3, 8, 11, 12])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_slots_past_the_end_have_no_effect(K, i, bad):
+    *p, gaps, extra = PAGED[i]
+    a, b = (Cache(*p, gaps=gaps, seed=300 + i, extra_cols=extra) for _ in range(2))
+    used = torch.zeros(b.pages, b.page, dtype=torch.bool, device=DEV)
+    for s, ((_, n), past) in enumerate(zip(b.segs, b.past)):
+        pos = torch.arange(n + past, device=DEV)
+        used[b.table[s].long()[pos // b.page], pos % b.page] = True
+    for x in (b.kp, b.vp):
+        x.masked_fill_(~used[:, None, :, None], bad)
+    a.attend(K)
+    b.attend(K)
+    assert torch.equal(a.out, b.out) and torch.equal(a.lse, b.lse)
+    b.check()
+
+
+@pytest.mark.parametrize("i", range(len(PAGED)))
+@pytest.mark.parametrize("rot,interleaved", [(1.0, False), (0.5, True), (0.0, False)])
+def test_append(K, i, rot, interleaved):
+    *p, gaps, extra = PAGED[i]
+    c = Cache(*p, gaps=gaps, seed=400 + i, extra_cols=extra)
+    rot = 2 * int(rot * c.dim / 2)
+    freqs = torch.tensor([10000.0 ** (-2 * j / max(rot, 1)) for j in range(rot // 2)], dtype=torch.float32, device=DEV)
+    kp, vp = c.kp.clone(), c.vp.clone()
+    c.append(K, freqs, rot, interleaved)
+    check_append(c, kp, vp, freqs, rot, interleaved)
+    # without queries, and with queries rotated where they are
+    c.kp.copy_(kp)
+    c.vp.copy_(vp)
+    c.out.fill_(MARK)
+    c.append(K, freqs, rot, interleaved, q=False)
+    assert bool((c.out == MARK).all())
+    q = c.q.clone()
+    c.append(K, freqs, rot, interleaved, q_out=c.q)
+    c.out, c.q = c.q, q
+    pos = c.positions()
+    assert torch.equal(c.out[pos < 0], q[pos < 0])
+    c.out[pos < 0] = MARK
+    check_append(c, kp, vp, freqs, rot, interleaved)
+
+
+def check_append(c, kp, vp, freqs, rot, interleaved):
+    pos = c.positions()
+    assert bool((c.out[pos < 0] == MARK).all())
+    want_q = torch.where((pos < 0)[:, None, None], MARK, ref.rotate(c.q, pos.clamp(min=0), freqs, rot, interleaved))
+    want_k, want_v, k = kp.double(), vp.double(), ref.rotate(c.k, pos.clamp(min=0), freqs, rot, interleaved)
+    for s, ((f, n), past) in enumerate(zip(c.segs, c.past)):
+        at = torch.arange(past, past + n, device=DEV)
+        ids = c.table[s].long()[at // c.page]
+        want_k[ids, :, at % c.page] = k[f:f + n]
+        want_v[ids, :, at % c.page] = c.v[f:f + n].double()
+    # one rounding of the result; sine, cosine, two products and a sum in f32 stay within
+    # 4 * 2^-24 * (|a| + |b|), components here being below 8; f16 subnormals: half a step
+    for got, want in ((c.out, want_q), (c.kp, want_k)):
+        ref.within(got, want, ref.U[c.t] * want.abs() + 4 * 2.0 ** -24 * 16 + ref.tiny(c.t))
+    assert torch.equal(c.vp.double(), want_v)
+    assert c.failure.item() == 0
+
+
+@pytest.mark.parametrize("past", [1 << 20, (1 << 24) + 1, (1 << 30) + 12345])
+def test_angles_of_far_positions(K, past):
+    """Positions whose product with a frequency keeps few bits of the angle in 32 bits.  The table
+    names pages only where the new tokens go."""
+    page = 1 << 22
+    t, n = "f16", 5
+    cols = (past + n) // page + 1
+    q, k, v = (randn(generator(s), t, n, 1, 64) for s in range(3))
+    out = torch.zeros_like(q)
+    kp, vp = (torch.zeros(2, 1, page, 64, dtype=torch.float16, device=DEV) for _ in range(2))
+    table = torch.full((1, cols), -1, dtype=torch.int32, device=DEV)
+    table[0, past // page] = 1
+    table[0, (past + n - 1) // page] = 1
+    off, lens = device_segments([(0, n)])
+    pl = torch.tensor([past], dtype=torch.int64, device=DEV)
+    fail = torch.zeros(1, dtype=torch.int32, device=DEV)
+    freqs = torch.tensor([10000.0 ** (-j / 32) for j in range(32)], dtype=torch.float32, device=DEV)
+    K.kv_append(stream(), t, view(q), view(out), view(k), view(v), n, 1, 1, 64, off.data_ptr(), lens.data_ptr(), 1,
+                pl.data_ptr(), freqs.data_ptr(), 64, 0, kp.data_ptr(), vp.data_ptr(), 2, page, table.data_ptr(), cols,
+                fail.data_ptr(), 1)
+    pos = torch.arange(past, past + n, device=DEV)
+    for got, want in ((out, ref.rotate(q, pos, freqs, 64, False)),
+                      (kp[1, 0, pos % page].unsqueeze(1), ref.rotate(k, pos, freqs, 64, False))):
+        ref.within(got, want, ref.U[t] * want.abs() + 4 * 2.0 ** -24 * 16 + ref.tiny(t))
+    assert fail.item() == 0
+
+
+def test_bad_pages_and_lengths_are_reported(K):
+    freqs = torch.ones(32, dtype=torch.float32, device=DEV)
+    for what in ("page high", "page low", "past negative", "past high", "past huge", "len"):
+        c = Cache("f16", 2, 1, 64, 16, [4, 5, 3], [30, 20, 40], seed=50)
+        if what == "page high":
+            c.table[1, 1] = c.pages
+        elif what == "page low":
+            c.table[1, 1] = -3
+        elif what == "len":
+            c.lens[1] = -5
+        else:
+            c.past_lens[1] = {"past negative": -1, "past high": c.cols * 16 - 4, "past huge": (1 << 63) - 1}[what]
+        kp, vp = c.kp.clone(), c.vp.clone()
+        c.append(K, freqs, 64, False)
+        assert c.failure.item() == 6, what
+        if what == "page high" or what == "page low":  # tokens 20..24 go to page 1: none is stored
+            mine = c.table[1].clone()
+            mine = mine[(mine >= 0) & (mine < c.pages)].long()
+            assert torch.equal(kp[mine], c.kp[mine]) and torch.equal(vp[mine], c.vp[mine])
+        c.failure.zero_()
+        c.out.fill_(MARK)
+        c.attend(K)
+        assert c.failure.item() == 6, what
+        f, n = c.segs[1]
+        if "page" not in what:
+            assert bool((c.out[f:f + n] == MARK).all()), what
+        good = Cache("f16", 2, 1, 64, 16, [4, 5, 3], [30, 20, 40], seed=50)
+        good.append(K, freqs, 64, False)
+        good.attend(K)
+        f, n = c.segs[0]
+        assert torch.equal(good.out[f:f + n], c.out[f:f + n]), what
+
+
+def test_a_table_without_columns(K):
+    c = Cache("f16", 2, 1, 64, 16, [1], [3], seed=51)
+    c.cols = 0
+    c.attend(K)
+    assert c.failure.item() == 6
+    assert bool((c.out == MARK).all())
+
+
+def test_prompt_then_tokens_as_a_server_runs_them(K):
+    """The prompt's keys go into the cache, attention over the packed prompt and attention over the
+    cache agree with the formulas; then tokens one at a time, captured once and replayed."""
+    t, h, hk, dim, page, rot = "bf16", 8, 2, 128, 16, 128
+    new, steps = [50, 1, 129], 4
+    freqs = torch.tensor([10000.0 ** (-j / 64) for j in range(64)], dtype=torch.float32, device=DEV)
+    c = Cache(t, h, hk, dim, page, new, [0, 0, 0], seed=60, extra_cols=1)
+    table = torch.arange(c.pages, device=DEV, dtype=torch.int32)
+    spare = [i for i in table.tolist() if i not in c.table.flatten().tolist()]
+    for s in range(3):  # one more page for each sequence, from a cache that is made larger
+        c.table[s, -(-new[s] // page)] = c.pages + s
+    assert len(spare) == 2
+    c.kp, c.vp = (torch.cat([x, torch.zeros(3, *x.shape[1:], dtype=x.dtype, device=DEV)]) for x in (c.kp, c.vp))
+    c.pages += 3
+    q_rot = torch.full_like(c.q, MARK)
+    c.append(K, freqs, rot, False, q_out=q_rot)
+    c.attend(K, q=q_rot)
+    c.check(q=q_rot)
+    paged = c.out.clone()
+    k, v, segs = c.gathered()
+    p = Problem(t, h, hk, dim, new, seed=61)
+    p.q, p.k, p.v = q_rot[:sum(new)].contiguous(), k, v
+    p.nq = p.nk = sum(new)
+    p.out = torch.full_like(p.q, MARK)
+    p.lse = torch.full((p.nq, h), MARK, dtype=torch.float32, device=DEV)
+    p.forward(K)
+    p.check_forward()
+    assert paged[:sum(new)].shape == p.out.shape
+    # one token of each sequence at a time
+    d = Cache(t, h, hk, dim, page, [1, 1, 1], new, seed=62)
+    d.kp, d.vp, d.pages, d.table, d.cols = c.kp, c.vp, c.pages, c.table, c.cols
+    d.size = K.attention_paged_workspace_bytes(d.n, h, hk, dim, 3, page, d.cols)
+    d.workspace = torch.empty(max(d.size, 1), dtype=torch.uint8, device=DEV)
+    q_rot = torch.full_like(d.q, MARK)
+
+    def step():
+        d.append(K, freqs, rot, False, q_out=q_rot)
+        d.attend(K, q=q_rot)
+
+    before = d.kp.clone(), d.vp.clone()
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    d.kp.copy_(before[0])
+    d.vp.copy_(before[1])
+    for i in range(steps):
+        for j, x in enumerate((d.q, d.k, d.v)):
+            x.copy_(randn(generator(70 + 10 * i + j), t, *x.shape))
+        d.out.fill_(MARK)
+        d.lse.fill_(MARK)
+        q_rot.fill_(MARK)
+        graph.replay()
+        torch.cuda.synchronize()
+        pos = d.positions()
+        live = pos >= 0
+        want = ref.rotate(d.q, pos.clamp(min=0), freqs, rot, False)
+        ref.within(q_rot[live], want[live], ref.U[t] * want[live].abs() + 4 * 2.0 ** -24 * 16)
+        d.check(q=q_rot)
+        d.past = [n + 1 for n in d.past]
+        d.past_lens += 1
+
+
+def test_with_the_arrays_of_a_context(ctx, K):
+    """The same operators on a Futhark context's arrays and stream, next to its own entry points."""
+    from futhark_amd import datagen as dg
+    n, h, dim = 96, 4, 64
+    x = dg.normal_f32(80, 3 * n * h * dim).reshape(3, n, h * dim)
+    bits = dg.to_f16_bits(x)
+    q, k, v = (ctx.new("f16_3d", bits[i][None]) for i in range(3))
+    out = ctx.new("f16_3d", np.zeros((1, n, h * dim), np.uint16))
+    offsets, lens = ctx.new("i64_1d", np.array([0, 40], np.int64)), ctx.new("i64_1d", np.array([40, n - 40], np.int64))
+    arr = [heads(a.device_ptr, h * dim, dim) for a in (q, k, v, out)]
+    K.attention(ctx.stream, "f16", arr[0], n, arr[1], arr[2], n, h, h, dim, offsets.device_ptr, lens.device_ptr,
+                offsets.device_ptr, lens.device_ptr, 2, 1 / math.sqrt(dim), 1, arr[3], None, None, 0)
+    got = torch.from_numpy(out.values().view(np.float16).reshape(n, h, dim).copy())
+    tq, tk, tv = (torch.from_numpy(bits[i].view(np.float16).reshape(n, h, dim).copy()) for i in range(3))
+    want, _, tol, _ = ref.forward("f16", tq, tk, tv, [(0, 40), (40, n - 40)], [(0, 40), (40, n - 40)],
+                                  1 / math.sqrt(dim), True)
+    ref.within(got, want, tol)
+    # scores of a product of the same arrays: the context's own matmul after the attention
+    prod = ctx.call("bmm_f16", ["f32_3d"], out, ctx.new("f16_3d", np.ascontiguousarray(bits[1].T)[None])).values()[0]
+    a, b = got.reshape(n, -1).double().numpy(), tk.reshape(n, -1).double().numpy()
+    assert np.all(np.abs(prod - a @ b.T) <= 1e-5 * (np.abs(a) @ np.abs(b).T))
+    for y in (q, k, v, out, offsets, lens):
+        y.free()
