@@ -1,108 +1,376 @@
 // Attention over packed sequences and over a paged cache: forward.
+//
+// A block takes 128 query rows of one key head: the query heads of the group
+// side by side for each of 128 / group tokens, so that keys and values are
+// fetched once for the group.  A wave owns 32 of the rows and walks the keys 64
+// at a time with the running maximum and sum of the softmax:
+//   S^T = K Q^T      keys are rows, query rows are columns: a lane holds 32 of the
+//                    64 scores of ONE query row, its partner in the other half of
+//                    the wave the rest, and maximum, sum and weights need no
+//                    exchange but one with that partner;
+//   O^T += V^T P^T   the weights are the right operand as they stand in their
+//                    registers (tile_columns reads V in the matching key order),
+//                    and a lane's column of O^T is its query row again, so that
+//                    rescaling is a multiplication by the lane's own factor.
+// Keys and values go from memory straight into LDS, double buffered, one
+// barrier per 64 keys.  Weights are rounded to the element type for the second
+// product (the matrix units take nothing wider at this rate); sums stay f32.
 #include "attention.hip.h"
 
 namespace fa {
 
-static __device__ uint4 g_zero_row[16];  // a key or value of zeros: 128 components
+constexpr int AT_WAVES = 4, AT_THREADS = AT_WAVES * WAVE;
+constexpr int AT_ROWS = 32 * AT_WAVES;  // query rows a block
+constexpr int AT_KEYS = 64;             // keys a step
+// A wave rescales its output only when a maximum has grown by 2^8 since it last
+// did: until then weights are at most 2^8, which f16 and bf16 hold as well as 1.
+constexpr float AT_RESCALE = 8.0f;
 
-// A wave per query row and head: lane l holds components l and l + 64, walks
-// the visible keys one by one and keeps the running maximum and sum of the
-// softmax in f32.
-struct Row {
-  float q[2], o[2] = {0.0f, 0.0f};
-  float top = -INFINITY, sum = 0.0f;
+struct AttentionArgs {
+  Heads q, k, v, out;
+  float *lse;
+  int64_t q_rows, k_rows;
+  int heads, kv_heads, group, dim;
+  const int64_t *q_offsets, *q_lens, *k_offsets, *k_lens;
+  int64_t m;
+  float scale_log2;  // scale * log2(e)
+  int causal;
+  int32_t *failure, code;
+  // paged only: the cache; keys of a unit that one block takes, and where parts go
+  Pages pages;
+  int chunk, splits;
+  float *part_o, *part_ml;
 };
-template <class E>
-__device__ __forceinline__ void row_see(Row &r, const uint16_t *k, const uint16_t *v, int dim, float scale) {
-  const int lane = lane_id();
-  float s = 0.0f, vv[2];
-#pragma unroll
-  for (int c = 0; c < 2; c++) {
-    const int d = lane + 64 * c;
-    s += d < dim ? r.q[c] * E::load(k[d]) : 0.0f;
-    vv[c] = d < dim ? E::load(v[d]) : 0.0f;
+
+// Keys, values and query rows a block works on.
+struct Unit {
+  int64_t seg, q_first, k_first;
+  int tokens, t0, q_len, k_len;  // tokens of the tile, its first one, lengths
+  int kv_head;
+};
+
+template <bool PAGED>
+__device__ __forceinline__ bool find_unit(const AttentionArgs &a, int64_t number, int per_tile, Unit &u) {
+  SegTile t;
+  if (!find_tile(a.q_offsets, a.q_lens, a.q_rows, PAGED ? nullptr : a.k_offsets, a.k_lens, a.k_rows, a.m, per_tile,
+                 number / a.kv_heads, t))
+    return false;
+  u.kv_head = (int)(number % a.kv_heads);
+  u.seg = t.seg;
+  u.q_first = t.first;
+  u.q_len = (int)t.len;
+  u.k_first = t.first2;
+  u.k_len = (int)t.len2;
+  if constexpr (PAGED) {
+    const int64_t past = a.pages.past_lens[t.seg], room = a.pages.capacity();
+    if (past < 0 || past > room || t.len > room - past) {
+      if (a.failure != nullptr) *a.failure = a.code;
+      return false;
+    }
+    u.k_len = (int)(past + t.len);
   }
-  for (int step = 1; step < WAVE; step *= 2) s += __shfl_xor(s, step);
-  s *= scale;
-  const float top = fmaxf(r.top, s);
-  if (top == -INFINITY) return;
-  const float old = __expf(r.top - top), p = __expf(s - top);
-  r.sum = r.sum * old + p;
-#pragma unroll
-  for (int c = 0; c < 2; c++) r.o[c] = r.o[c] * old + p * vv[c];
-  r.top = top;
-}
-template <class E> __device__ __forceinline__ void row_load(Row &r, const uint16_t *q, int dim) {
-#pragma unroll
-  for (int c = 0; c < 2; c++) {
-    const int d = lane_id() + 64 * c;
-    r.q[c] = d < dim ? E::load(q[d]) : 0.0f;
-  }
-}
-template <class E> __device__ __forceinline__ void row_store(const Row &r, uint16_t *out, float *lse, int dim) {
-#pragma unroll
-  for (int c = 0; c < 2; c++) {
-    const int d = lane_id() + 64 * c;
-    if (d < dim) out[d] = E::store(r.top == -INFINITY ? 0.0f : r.o[c] / r.sum);
-  }
-  if (lse != nullptr && lane_id() == 0) *lse = r.top == -INFINITY ? -INFINITY : r.top + __logf(r.sum);
+  u.t0 = (int)(t.tiles - 1 - t.tile) * per_tile;  // the last tokens see most: they start first
+  u.tokens = u.q_len - u.t0 < per_tile ? u.q_len - u.t0 : per_tile;
+  return true;
 }
 
-template <class E>
-__global__ __launch_bounds__(256) void attention_kernel(
-    Heads q, Heads k, Heads v, Heads out, float *lse, int64_t q_rows, int64_t k_rows, int heads, int group,
-    int dim, const int64_t *q_offsets, const int64_t *q_lens, const int64_t *k_offsets,
-    const int64_t *k_lens, int64_t m, float scale, int causal, int32_t *failure, int32_t code) {
+// What splits of a unit leave for the kernel that joins them.
+__device__ __forceinline__ int64_t part_row(const AttentionArgs &a, int64_t unit, int split, int row) {
+  return (unit * a.splits + split) * AT_ROWS + row;
+}
+
+template <class E, int D, bool PAGED>
+__global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs a) {
+  constexpr int TILE = AT_KEYS * D * 2;               // bytes of 64 keys (or values)
+  constexpr int LOADS = TILE / (AT_THREADS * 16);     // 16-byte loads a thread and tile
+  constexpr int LOAD_ROWS = AT_KEYS / LOADS;          // rows one of them covers
+  constexpr int UNITS = D / 8;                        // 16-byte units of a row
+  extern __shared__ __align__(16) unsigned char lds[];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int half = lane >> 5;
   if (blockIdx.x == 0 && blockIdx.y == 0) {
-    report_segments(q_offsets, q_lens, m, q_rows, failure, code);
-    report_segments(k_offsets, k_lens, m, k_rows, failure, code);
+    report_segments(a.q_offsets, a.q_lens, a.m, a.q_rows, a.failure, a.code);
+    if constexpr (!PAGED) report_segments(a.k_offsets, a.k_lens, a.m, a.k_rows, a.failure, a.code);
   }
-  const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / WAVE;
-  const int h = blockIdx.y;
-  if (row >= q_rows) return;
-  int64_t q_first, q_len, k_first, k_len;
-  const int64_t seg = segment_of_row(q_offsets, q_lens, m, q_rows, row, q_first, q_len);
-  if (seg < 0 || !segment_ok(k_offsets, k_lens, seg, k_rows, k_first, k_len)) return;
-  int64_t keys = causal ? row - q_first + (k_len - q_len) + 1 : k_len;
-  Row r;
-  row_load<E>(r, q.at(row, h), dim);
-  for (int64_t j = 0; j < keys; j++)
-    row_see<E>(r, k.at(k_first + j, h / group), v.at(k_first + j, h / group), dim, scale);
-  row_store<E>(r, out.at(row, h), lse == nullptr ? nullptr : lse + row * heads + h, dim);
-}
+  const int per_tile = AT_ROWS / a.group;
+  Unit u;
+  if (!find_unit<PAGED>(a, blockIdx.x, per_tile, u)) return;
 
-template <class E>
-__global__ __launch_bounds__(256) void attention_paged_kernel(
-    Heads q, Heads out, float *lse, int64_t n, int heads, int group, int dim, const int64_t *offsets,
-    const int64_t *lens, int64_t m, float scale, Pages pages, int32_t *failure, int32_t code) {
-  if (blockIdx.x == 0 && blockIdx.y == 0) report_segments(offsets, lens, m, n, failure, code);
-  const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / WAVE;
-  const int h = blockIdx.y;
-  if (row >= n) return;
-  int64_t first, len;
-  const int64_t seg = segment_of_row(offsets, lens, m, n, row, first, len);
-  if (seg < 0) return;
-  const int64_t past = pages.past_lens[seg];
-  if (past < 0 || past > pages.capacity() || len > pages.capacity() - past) {
-    if (failure != nullptr) *failure = code;
+  // This lane's query row, and the last key it, its wave and its block see.
+  const int behind = a.causal ? u.k_len - u.q_len : 0;
+  const auto last_key = [&](int token) { return a.causal ? u.t0 + token + behind : u.k_len - 1; };
+  const int rows = u.tokens * a.group;
+  const int row = wave * 32 + (lane & 31);
+  const int my_row = row < rows ? row : rows - 1;
+  const int token = my_row / a.group, head = u.kv_head * a.group + my_row % a.group;
+  const int limit = last_key(token);
+  const bool wave_works = wave * 32 < rows;
+  const int wave_last = __builtin_amdgcn_readfirstlane(
+      last_key(((wave + 1) * 32 < rows ? (wave + 1) * 32 - 1 : rows - 1) / a.group));
+  const int wave_first = __builtin_amdgcn_readfirstlane(last_key(wave_works ? wave * 32 / a.group : 0));
+  const int block_first = last_key(0), block_last = last_key(u.tokens - 1);
+  const int keys = block_last + 1;  // all the block's rows see together
+  int from = 0, to = keys;
+  if constexpr (PAGED) {
+    from = blockIdx.y * a.chunk;
+    to = keys - from < a.chunk ? keys : from + a.chunk;
+    if (from >= keys && blockIdx.y > 0) return;
+  }
+
+  // Loads: load i of this thread brings unit `unit` of row load_row + i LOAD_ROWS.
+  const int slot = threadIdx.x % UNITS, load_row = threadIdx.x / UNITS;
+  const int unit = slot ^ tile_swizzle<D>(load_row);  // the same for all its rows
+  const bool unit_live = unit * 8 < a.dim;
+  const uint32_t lds_base = lds_address(lds) + wave * 1024;
+  int32_t page[LOADS];
+  const auto fetch_pages = [&](int key0) __attribute__((always_inline)) {
+    if constexpr (PAGED) {
+#pragma unroll
+      for (int i = 0; i < LOADS; i++) {
+        const int key = key0 + load_row + i * LOAD_ROWS;
+        page[i] = key < to ? a.pages.table[u.seg * a.pages.cols + (key >> a.pages.page_shift)] : 0;
+      }
+    }
+  };
+  const auto fetch = [&](int key0, int stage) __attribute__((always_inline)) {
+    const uint32_t dst = lds_base + stage * (2 * TILE);
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) {
+      const int key = key0 + load_row + i * LOAD_ROWS;
+      const uint16_t *ks = (const uint16_t *)&g_zeros, *vs = ks;
+      bool live = unit_live && key < to;
+      if constexpr (PAGED) {
+        if (key < to && (page[i] < 0 || page[i] >= a.pages.n_pages)) {
+          live = false;
+          if (a.failure != nullptr) *a.failure = a.code;
+        }
+        if (live) {
+          const int64_t at = (a.pages.row_of(page[i], u.kv_head, a.kv_heads) +
+                              (key & ((1 << a.pages.page_shift) - 1))) * a.dim + unit * 8;
+          ks = a.pages.k + at;
+          vs = a.pages.v + at;
+        }
+      } else if (live) {
+        ks = a.k.at(u.k_first + key, u.kv_head) + unit * 8;
+        vs = a.v.at(u.k_first + key, u.kv_head) + unit * 8;
+      }
+      load_to_lds(ks, dst + i * (AT_THREADS * 16));
+      load_to_lds(vs, dst + TILE + i * (AT_THREADS * 16));
+    }
+  };
+
+  uint4 q[D / 16];
+  {
+    const uint16_t *src = a.q.at(u.q_first + u.t0 + token, head);
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ks++) {
+      const int c = ks * 16 + half * 8;
+      q[ks] = c < a.dim ? *reinterpret_cast<const uint4 *>(src + c) : uint4{0, 0, 0, 0};
+    }
+  }
+  f32x16 o[D / 32];
+#pragma unroll
+  for (int dt = 0; dt < D / 32; dt++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) o[dt][i] = 0.0f;
+  float top = -INFINITY, sum = 0.0f;  // top: of scores times log2(e); sum: this lane's half
+
+  fetch_pages(from);
+  if (from < to) fetch(from, 0);
+  fetch_pages(from + AT_KEYS);
+  int stage = 0;
+  for (int key0 = from; key0 < to; key0 += AT_KEYS, stage ^= 1) {
+    wait_loads();
+    __syncthreads();
+    if (key0 + AT_KEYS < to) {
+      fetch(key0 + AT_KEYS, stage ^ 1);
+      fetch_pages(key0 + 2 * AT_KEYS);
+    }
+    unsigned char *kt = lds + stage * (2 * TILE), *vt = kt + TILE;
+    const int last = key0 + AT_KEYS - 1;
+    // Rows of the block see different keys of this tile: a value that a row does
+    // not see must not reach it, and 0 * NaN would.
+    bool unsafe = false;
+    if (last > block_first && block_first < block_last) {
+      bool found = false;
+#pragma unroll
+      for (int i = 0; i < LOADS; i++) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(vt + (i * AT_THREADS + threadIdx.x) * 16);
+        for (uint32_t w : {x.x, x.y, x.z, x.w})
+          found = found || (w & E::exponent) == E::exponent || (w >> 16 & E::exponent) == E::exponent;
+      }
+      unsafe = __syncthreads_or(found);
+    }
+    const bool active = wave_works && key0 <= wave_last;
+    uint4 p[4];
+    if (active) {
+      f32x16 s[2];
+#pragma unroll
+      for (int b = 0; b < 2; b++) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) s[b][i] = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < D / 16; ks++) s[b] = E::mfma(tile_rows<D>(kt, b * 32 + (lane & 31), ks), q[ks], s[b]);
+      }
+      if (last > wave_first) {
+#pragma unroll
+        for (int b = 0; b < 2; b++)
+#pragma unroll
+          for (int i = 0; i < 16; i++)
+            if (key0 + b * 32 + 8 * (i >> 2) + 4 * half + (i & 3) > limit) s[b][i] = -INFINITY;
+      }
+      float high = s[0][0];
+#pragma unroll
+      for (int i = 1; i < 32; i++) high = fmaxf(high, s[i >> 4][i & 15]);
+      high = fmaxf(high, other_half(high)) * a.scale_log2;
+      if (__any(high > top + AT_RESCALE)) {
+        const float now = fmaxf(top, high);
+        const float factor = now == -INFINITY ? 1.0f : exp2f(top - now);
+        top = now;
+        sum *= factor;
+#pragma unroll
+        for (int dt = 0; dt < D / 32; dt++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) o[dt][i] *= factor;
+      }
+      const float shift = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+      for (int c = 0; c < 4; c++) {
+        f32x8 w;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          w[i] = __builtin_amdgcn_exp2f(fmaf(s[c >> 1][(c & 1) * 8 + i], a.scale_log2, -shift));
+          sum += w[i];
+        }
+        p[c] = E::pack(w);
+      }
+    }
+    if (unsafe) {
+      // Add what the rows see of the values that are not finite, one by one, and
+      // take them out of the tile.
+      if (active) {
+        for (int j = 0; j < AT_KEYS && key0 + j < to; j++) {
+#pragma unroll
+          for (int dt = 0; dt < D / 32; dt++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+              const int d = dt * 32 + 8 * (i >> 2) + 4 * half + (i & 3);
+              const uint16_t bits = *reinterpret_cast<const uint16_t *>(vt + tile_offset<D>(j, d >> 3) + (d & 7) * 2);
+              if ((bits & E::exponent) == E::exponent && key0 + j <= limit) o[dt][i] += E::load(bits);
+            }
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < LOADS * 8; i++) {
+        uint16_t *x = reinterpret_cast<uint16_t *>(vt) + (i / 8 * AT_THREADS + threadIdx.x) * 8 + i % 8;
+        if ((*x & E::exponent) == E::exponent) *x = 0;
+      }
+      __syncthreads();
+    }
+    if (active) {
+#pragma unroll
+      for (int c = 0; c < 4; c++)
+#pragma unroll
+        for (int dt = 0; dt < D / 32; dt++) o[dt] = E::mfma(tile_columns<D>(vt, c * 16, dt * 32), p[c], o[dt]);
+    }
+  }
+
+  sum += other_half(sum);
+  if (row >= rows) return;
+  if (PAGED && keys > a.chunk) {
+    const int64_t at = part_row(a, blockIdx.x, blockIdx.y, row);
+#pragma unroll
+    for (int dt = 0; dt < D / 32; dt++)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4)
+        *reinterpret_cast<f32x4 *>(a.part_o + at * D + dt * 32 + 2 * i + 4 * half) =
+            f32x4{o[dt][i], o[dt][i + 1], o[dt][i + 2], o[dt][i + 3]};
+    if (half == 0) {
+      a.part_ml[2 * at] = top;
+      a.part_ml[2 * at + 1] = sum;
+    }
     return;
   }
-  Row r;
-  row_load<E>(r, q.at(row, h), dim);
-  for (int64_t j = 0; j <= past + (row - first); j++) {
-    const int64_t page = pages.table[seg * pages.cols + (j >> pages.page_shift)];
-    const int64_t slot = j & (((int64_t)1 << pages.page_shift) - 1);
-    const uint16_t *kp = (const uint16_t *)g_zero_row, *vp = kp;
-    if (page >= 0 && page < pages.n_pages) {
-      const int64_t at = (pages.row_of(page, h / group, heads / group) + slot) * dim;
-      kp = pages.k + at;
-      vp = pages.v + at;
-    } else if (failure != nullptr) {
-      *failure = code;
+  const int64_t out_row = u.q_first + u.t0 + token;
+  const bool empty = top == -INFINITY;  // saw nothing, or only scores of -inf
+  const float inverse = empty ? 0.0f : 1.0f / sum;
+  uint16_t *dst = a.out.at(out_row, head);
+#pragma unroll
+  for (int dt = 0; dt < D / 32; dt++)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int d = dt * 32 + 2 * i + 4 * half;
+      uint16_t x[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) x[j] = E::store(empty ? 0.0f : o[dt][i + j] * inverse);
+      if (d < a.dim) *reinterpret_cast<uint2 *>(dst + d) = uint2{x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16};
     }
-    row_see<E>(r, kp, vp, dim, scale);
+  if (a.lse != nullptr && half == 0)
+    a.lse[out_row * a.heads + head] = empty ? -INFINITY : (top + log2f(sum)) * 0.693147180559945309f;
+}
+
+// Joins the parts of the units whose keys were split: a wave per query row.
+template <class E, int D> __global__ __launch_bounds__(AT_THREADS) void attention_join_kernel(AttentionArgs a) {
+  const int per_tile = AT_ROWS / a.group;
+  Unit u;
+  if (!find_unit<true>(a, blockIdx.x, per_tile, u)) return;
+  const int row = blockIdx.y * AT_WAVES + threadIdx.x / WAVE, rows = u.tokens * a.group;
+  const int keys = u.t0 + u.tokens + u.k_len - u.q_len;
+  if (row >= rows || keys <= a.chunk) return;
+  const int splits = (keys + a.chunk - 1) / a.chunk;
+  float top = -INFINITY;
+  for (int s = 0; s < splits; s++) top = fmaxf(top, a.part_ml[2 * part_row(a, blockIdx.x, s, row)]);
+  float sum = 0.0f, o[D / WAVE] = {};
+  if (top != -INFINITY) {
+    for (int s = 0; s < splits; s++) {
+      const int64_t at = part_row(a, blockIdx.x, s, row);
+      const float f = exp2f(a.part_ml[2 * at] - top);
+      sum += f * a.part_ml[2 * at + 1];
+#pragma unroll
+      for (int c = 0; c < D / WAVE; c++) o[c] += f * a.part_o[at * D + c * WAVE + lane_id()];
+    }
   }
-  row_store<E>(r, out.at(row, h), lse == nullptr ? nullptr : lse + row * heads + h, dim);
+  const int head = u.kv_head * a.group + row % a.group;
+  const int64_t out_row = u.q_first + u.t0 + row / a.group;
+#pragma unroll
+  for (int c = 0; c < D / WAVE; c++) {
+    const int d = c * WAVE + lane_id();
+    if (d < a.dim) a.out.at(out_row, head)[d] = E::store(top == -INFINITY ? 0.0f : o[c] / sum);
+  }
+  if (a.lse != nullptr && lane_id() == 0)
+    a.lse[out_row * a.heads + head] = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * 0.693147180559945309f;
+}
+
+// How a cache's keys are split over blocks: enough blocks to fill the chip if
+// all sequences are as long as the table allows, at least 256 keys to a block.
+struct SplitPlan {
+  int64_t units;
+  int chunk, splits;
+};
+static SplitPlan split_plan(int64_t n, int64_t heads, int64_t kv_heads, int64_t m, int64_t capacity) {
+  SplitPlan p;
+  p.units = most_tiles(n, m, AT_ROWS / (heads / kv_heads)) * kv_heads;
+  const int64_t even = ceil_div(capacity * p.units, 8 * NUM_CUS_HINT);
+  const int64_t chunk = ceil_div(even < 256 ? 256 : even, AT_KEYS) * AT_KEYS;
+  p.chunk = (int)(chunk < capacity ? chunk : (capacity > 0 ? capacity : 1));
+  p.splits = (int)(capacity > 0 ? ceil_div(capacity, p.chunk) : 1);
+  return p;
+}
+
+template <bool PAGED> static int launch_attention(hipStream_t stream, fa_dtype t, const AttentionArgs &a, int64_t units) {
+  if (units > INT32_MAX) return FA_ENOTSUP;
+  const dim3 grid((unsigned)units, (unsigned)a.splits);
+  const bool narrow = a.dim <= 64;
+  const size_t lds = 4 * AT_KEYS * (narrow ? 64 : 128) * 2;
+  if (t == FA_F16) {
+    if (narrow) attention_kernel<ElemF16, 64, PAGED><<<grid, AT_THREADS, lds, stream>>>(a);
+    else attention_kernel<ElemF16, 128, PAGED><<<grid, AT_THREADS, lds, stream>>>(a);
+  } else {
+    if (narrow) attention_kernel<ElemBF16, 64, PAGED><<<grid, AT_THREADS, lds, stream>>>(a);
+    else attention_kernel<ElemBF16, 128, PAGED><<<grid, AT_THREADS, lds, stream>>>(a);
+  }
+  return launch_status();
 }
 
 }  // namespace fa
@@ -125,17 +393,28 @@ extern "C" int fa_attention(fa_stream_t stream, fa_dtype t, const fa_heads *q, i
   if (rc == 0) rc = check_heads(out, q_rows, heads, head_dim, true);
   if (rc == 0 && !is_aligned(lse, 4)) rc = FA_EALIGN;
   if (rc != 0) return rc;
-  const auto kernel = t == FA_F16 ? attention_kernel<ElemF16> : attention_kernel<ElemBF16>;
-  kernel<<<dim3((unsigned)ceil_div(q_rows, 4), (unsigned)heads), dim3(256), 0, (hipStream_t)stream>>>(
-      to_heads(q), to_heads(k), to_heads(v), to_heads(out), lse, q_rows, k_rows, (int)heads,
-      (int)(heads / kv_heads), (int)head_dim, q_offsets, q_lens, k_offsets, k_lens, m, scale, causal, failure,
-      code);
-  return launch_status();
+  AttentionArgs a = {};
+  a.q = to_heads(q), a.k = to_heads(k), a.v = to_heads(v), a.out = to_heads(out);
+  a.lse = lse;
+  a.q_rows = q_rows, a.k_rows = k_rows;
+  a.heads = (int)heads, a.kv_heads = (int)kv_heads, a.group = (int)(heads / kv_heads), a.dim = (int)head_dim;
+  a.q_offsets = q_offsets, a.q_lens = q_lens, a.k_offsets = k_offsets, a.k_lens = k_lens;
+  a.m = m;
+  a.scale_log2 = scale * 1.44269504088896341f;
+  a.causal = causal != 0;
+  a.failure = failure, a.code = code;
+  a.splits = 1;
+  return launch_attention<false>((hipStream_t)stream, t, a, most_tiles(q_rows, m, AT_ROWS / a.group) * kv_heads);
 }
 
-extern "C" size_t fa_attention_paged_workspace_bytes(int64_t, int64_t, int64_t, int64_t, int64_t, int64_t,
-                                                     int64_t) {
-  return 0;
+extern "C" size_t fa_attention_paged_workspace_bytes(int64_t n, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                                     int64_t m, int64_t page_size, int64_t table_cols) {
+  if (n <= 0 || m <= 0 || n > AT_MOST_ROWS || m > AT_MOST_ROWS || page_size <= 0 || table_cols <= 0 ||
+      (__int128)page_size * table_cols > AT_MOST_ROWS || check_shape(FA_F16, heads, kv_heads, head_dim) != 0)
+    return 0;
+  const SplitPlan p = split_plan(n, heads, kv_heads, m, page_size * table_cols);
+  if (p.splits == 1) return 0;
+  return (size_t)p.units * p.splits * AT_ROWS * ((head_dim <= 64 ? 64 : 128) + 2) * sizeof(float);
 }
 
 extern "C" int fa_attention_paged(fa_stream_t stream, fa_dtype t, const fa_heads *q, int64_t n,
@@ -157,11 +436,37 @@ extern "C" int fa_attention_paged(fa_stream_t stream, fa_dtype t, const fa_heads
   if (rc == 0 && !is_aligned(lse, 4)) rc = FA_EALIGN;
   if (rc != 0) return rc;
   const size_t need = fa_attention_paged_workspace_bytes(n, heads, kv_heads, head_dim, m, page_size, table_cols);
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return FA_ESCRATCH;
-  const Pages pages = to_pages(k_pages, v_pages, n_pages, page_size, page_table, table_cols, past_lens);
-  const auto kernel = t == FA_F16 ? attention_paged_kernel<ElemF16> : attention_paged_kernel<ElemBF16>;
-  kernel<<<dim3((unsigned)ceil_div(n, 4), (unsigned)heads), dim3(256), 0, (hipStream_t)stream>>>(
-      to_heads(q), to_heads(out), lse, n, (int)heads, (int)(heads / kv_heads), (int)head_dim, offsets, lens, m,
-      scale, pages, failure, code);
+  if (need > 0) {
+    if (workspace == nullptr || workspace_bytes < need) return FA_ESCRATCH;
+    if (!is_aligned(workspace, 16)) return FA_EALIGN;
+  }
+  const SplitPlan p = split_plan(n, heads, kv_heads, m, page_size * table_cols);
+  AttentionArgs a = {};
+  a.q = to_heads(q), a.out = to_heads(out);
+  a.lse = lse;
+  a.q_rows = n;
+  a.heads = (int)heads, a.kv_heads = (int)kv_heads, a.group = (int)(heads / kv_heads), a.dim = (int)head_dim;
+  a.q_offsets = offsets, a.q_lens = lens;
+  a.m = m;
+  a.scale_log2 = scale * 1.44269504088896341f;
+  a.causal = 1;
+  a.failure = failure, a.code = code;
+  a.pages = to_pages(k_pages, v_pages, n_pages, page_size, page_table, table_cols, past_lens);
+  a.chunk = p.chunk, a.splits = p.splits;
+  if (p.splits > 1) {
+    const int64_t parts = p.units * p.splits * AT_ROWS;
+    a.part_o = (float *)workspace;
+    a.part_ml = a.part_o + parts * (head_dim <= 64 ? 64 : 128);
+  }
+  rc = launch_attention<true>((hipStream_t)stream, t, a, p.units);
+  if (rc != 0 || p.splits == 1) return rc;
+  const dim3 grid((unsigned)p.units, (unsigned)ceil_div(AT_ROWS, AT_WAVES));
+  if (t == FA_F16) {
+    if (head_dim <= 64) attention_join_kernel<ElemF16, 64><<<grid, AT_THREADS, 0, (hipStream_t)stream>>>(a);
+    else attention_join_kernel<ElemF16, 128><<<grid, AT_THREADS, 0, (hipStream_t)stream>>>(a);
+  } else {
+    if (head_dim <= 64) attention_join_kernel<ElemBF16, 64><<<grid, AT_THREADS, 0, (hipStream_t)stream>>>(a);
+    else attention_join_kernel<ElemBF16, 128><<<grid, AT_THREADS, 0, (hipStream_t)stream>>>(a);
+  }
   return launch_status();
 }

@@ -12,14 +12,33 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
-// 16-bit element types.  `store` rounds to nearest even.
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+// 16-bit element types.  `store` and `pack` round to nearest even; `mfma` is
+// C += A B with A 32 x 16, B 16 x 32: lane l holds row (column) l % 32 of A (B)
+// and the eight k from 8 (l / 32), and of C column l % 32, rows
+// 8 (i / 4) + 4 (l / 32) + i % 4 for i < 16.
 struct ElemF16 {
+  static constexpr uint32_t exponent = 0x7c00;  // all ones: infinity or NaN
   static __device__ __forceinline__ float load(uint16_t b) { return (float)bit_cast<_Float16>(b); }
   static __device__ __forceinline__ uint16_t store(float f) { return bit_cast<uint16_t>((_Float16)f); }
+  static __device__ __forceinline__ uint4 pack(f32x8 x) {
+    return bit_cast<uint4>(__builtin_convertvector(x, f16x8));
+  }
+  static __device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(bit_cast<f16x8>(a), bit_cast<f16x8>(b), c, 0, 0, 0);
+  }
 };
 struct ElemBF16 {
+  static constexpr uint32_t exponent = 0x7f80;
   static __device__ __forceinline__ float load(uint16_t b) { return bit_cast<float>((uint32_t)b << 16); }
   static __device__ __forceinline__ uint16_t store(float f) { return bit_cast<uint16_t>((__bf16)f); }
+  static __device__ __forceinline__ uint4 pack(f32x8 x) {
+    return bit_cast<uint4>(__builtin_convertvector(x, bf16x8));
+  }
+  static __device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(bit_cast<bf16x8>(a), bit_cast<bf16x8>(b), c, 0, 0, 0);
+  }
 };
 
 // fa_heads as the kernels take it.
@@ -80,6 +99,106 @@ __device__ __forceinline__ int64_t segment_of_row(const int64_t *offsets, const 
   return -1;
 }
 
+// Work on a segment comes in tiles of `per_tile` rows, numbered through the
+// segments in order; the tile of number `number`, or false if there are fewer.
+// The same for the whole wave, which looks at 64 segments at a time.  A broken
+// segment (also one whose partner in `offsets2` is broken) has no tiles.
+struct SegTile {
+  int64_t seg, tile, tiles;  // segment, tile in it, tiles it has
+  int64_t first, len;
+  int64_t first2, len2;  // the partner segment's
+};
+__device__ __forceinline__ bool find_tile(const int64_t *offsets, const int64_t *lens, int64_t n,
+                                          const int64_t *offsets2, const int64_t *lens2, int64_t n2, int64_t m,
+                                          int per_tile, int64_t number, SegTile &t) {
+  int64_t before = 0;
+  for (int64_t base = 0; base < m; base += WAVE) {
+    const int64_t i = base + lane_id();
+    int64_t f = 0, l = 0, f2 = 0, l2 = 0;
+    bool ok = i < m && segment_ok(offsets, lens, i, n, f, l);
+    if (offsets2 != nullptr) ok = ok && segment_ok(offsets2, lens2, i, n2, f2, l2);
+    // lengths are below 2^31
+    const int64_t tiles = ok ? ((uint32_t)l + (uint32_t)per_tile - 1) / (uint32_t)per_tile : 0;
+    const int64_t upto = before + wave_incl_scan<int64_t, OpAdd<int64_t>>(tiles);
+    const uint64_t past = __ballot(upto > number);
+    if (past != 0) {
+      const int at = __builtin_ctzll(past);
+      t.seg = base + at;
+      t.tiles = read_lane(tiles, at);
+      t.tile = number - (read_lane(upto, at) - t.tiles);
+      t.first = read_lane(f, at);
+      t.len = read_lane(l, at);
+      t.first2 = read_lane(f2, at);
+      t.len2 = read_lane(l2, at);
+      return true;
+    }
+    before = read_lane(upto, WAVE - 1);
+  }
+  return false;
+}
+
+// Tiles that n rows in m segments make at most (empty segments make none).
+inline int64_t most_tiles(int64_t n, int64_t m, int64_t per_tile) {
+  const int64_t by_parts = (n + m * (per_tile - 1)) / per_tile;
+  return by_parts < n ? by_parts : n;
+}
+
+// ------------------------------------------------------------- tiles in LDS
+// Rows of D 16-bit components (D 64 or 128) in 16-byte units; unit u of row r
+// sits in slot u ^ f(r).  f makes both ways of reading a tile free of bank
+// conflicts: 16 consecutive rows, one unit each (128-bit operand reads; f
+// differs for all rows that share a bank), and four rows (4-aligned) of 64
+// consecutive bytes (the transposing reads; f differs in the bits above the
+// lowest two, which move 64-byte groups).
+template <int D> __device__ __forceinline__ int tile_swizzle(int r) {
+  static_assert(D == 64 || D == 128, "rows of 128 or 256 bytes");
+  if constexpr (D == 128) return ((r & 3) << 2) | ((r >> 2) & 3);
+  else return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+}
+template <int D> __device__ __forceinline__ int tile_offset(int r, int unit) {
+  return r * (D * 2) + ((unit ^ tile_swizzle<D>(r)) << 4);
+}
+
+// Sixteen bytes a lane from global memory into LDS at `lds` (wave uniform) +
+// 16 * lane.  The compiler does not see this load: wait_loads() and a barrier
+// come before what it brings is read.
+__device__ __forceinline__ void load_to_lds(const void *src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(
+                   __builtin_amdgcn_readfirstlane(lds)),
+               "v"(src)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t lds_address(const void *p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char *)p;
+}
+
+// Operand of a product over components: row `r`, components 16 step + 8 (lane / 32) ...
+template <int D> __device__ __forceinline__ uint4 tile_rows(const unsigned char *tile, int r, int step) {
+  return *reinterpret_cast<const uint4 *>(tile + tile_offset<D>(r, 2 * step + (lane_id() >> 5)));
+}
+// Operand of a product over rows: for lane l component c0 + l % 32 of the rows
+// r0 + 4 (l / 32) + {0..3, 8..11}: the rows whose products a lane holds in
+// registers 0..7 of an MFMA result, so that a result is the other operand as it
+// stands.  r0 is a multiple of 16, c0 of 32.
+template <int D> __device__ __forceinline__ uint4 tile_columns(const unsigned char *tile, int r0, int c0) {
+  const int l = lane_id(), r = l & 15;
+  const int row = r0 + 4 * (l >> 5) + (r >> 2), c = c0 + ((l >> 4) & 1) * 16 + 4 * (r & 3);
+  const auto read = [&](int at) __attribute__((always_inline)) {
+    const unsigned char *p = tile + tile_offset<D>(at, c >> 3) + (c & 7) * 2;
+    return bit_cast<uint2>(
+        __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 __attribute__((address_space(3))) *)(p)));
+  };
+  const uint2 lo = read(row), hi = read(row + 8);
+  return uint4{lo.x, lo.y, hi.x, hi.y};
+}
+
+// The value a lane's partner in the other half of the wave holds.
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+
+static __device__ uint4 g_zeros;  // what loads past the end of a tile read
+
 // Reports broken segments; every thread of the calling block takes part.
 __device__ __forceinline__ void report_segments(const int64_t *offsets, const int64_t *lens, int64_t m,
                                                 int64_t n, int32_t *failure, int32_t code) {
@@ -119,9 +238,12 @@ inline int check_shape(fa_dtype t, int64_t heads, int64_t kv_heads, int64_t head
   return 0;
 }
 
+// Most rows and positions: 32-bit numbers that may run a few tiles past them.
+constexpr int64_t AT_MOST_ROWS = INT32_MAX - 4095;
+
 inline int check_segments(const int64_t *offsets, const int64_t *lens, int64_t m, int64_t n) {
   if (m < 0 || n < 0) return FA_EINVAL;
-  if (m > INT32_MAX || n > INT32_MAX) return FA_ENOTSUP;
+  if (m > AT_MOST_ROWS || n > AT_MOST_ROWS) return FA_ENOTSUP;
   if (m > 0 && (offsets == nullptr || lens == nullptr)) return FA_EINVAL;
   if (!is_aligned(offsets, 8) || !is_aligned(lens, 8)) return FA_EALIGN;
   return 0;
@@ -132,7 +254,7 @@ inline int check_pages(const void *k_pages, const void *v_pages, int64_t n_pages
                        int64_t head_dim) {
   if (n_pages < 0 || page_size <= 0 || cols < 0) return FA_EINVAL;
   if ((page_size & (page_size - 1)) != 0 || n_pages > INT32_MAX) return FA_ENOTSUP;
-  if ((__int128)cols * page_size > INT32_MAX) return FA_ENOTSUP;
+  if ((__int128)cols * page_size > AT_MOST_ROWS) return FA_ENOTSUP;
   if ((__int128)n_pages * page_size * kv_heads * head_dim >= ((__int128)1 << 61)) return FA_EINVAL;
   if (past_lens == nullptr || (table == nullptr && cols > 0)) return FA_EINVAL;
   if ((k_pages == nullptr || v_pages == nullptr) && n_pages > 0) return FA_EINVAL;

@@ -345,7 +345,7 @@ int fa_matmul_ws(fa_stream_t stream, fa_dtype in_t,
  *
  * Sequences are segments of the rows, offsets[i] and lens[i] for i < m, on the
  * device, under the rules of fa_segred_irregular (in order, disjoint, inside
- * the n rows; n and m below 2^31).  Rows in no segment are neither read nor
+ * the n rows; n and m at most 2^31 - 4096).  Rows in no segment are neither read nor
  * written.  A segment that breaks the rules (or has a length or page number out
  * of range, below) is detected on the device: `code` is stored into *failure
  * (device-visible memory; NULL: not reported), the segment is left out, and
@@ -401,7 +401,7 @@ int fa_attention_grad(fa_stream_t stream, fa_dtype t, const fa_heads *q, int64_t
  * [n_pages][kv_heads][page_size][head_dim], page_size a power of two
  * (FA_ENOTSUP otherwise), 16-byte aligned; page_table is [m][table_cols] i32,
  * and position p of sequence i lives in slot p % page_size of page
- * page_table[i][p / page_size].  table_cols * page_size is below 2^31.
+ * page_table[i][p / page_size].  table_cols * page_size is at most 2^31 - 4096.
  * Sequence i holds past_lens[i] tokens before the new ones, lens[i] tokens at
  * rows offsets[i]...; past + new must fit its table row.
  *
