@@ -81,10 +81,8 @@ __device__ __forceinline__ int64_t part_row(const AttentionArgs &a, int64_t unit
 
 template <class E, int D, bool PAGED>
 __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs a) {
-  constexpr int TILE = AT_KEYS * D * 2;               // bytes of 64 keys (or values)
-  constexpr int LOADS = TILE / (AT_THREADS * 16);     // 16-byte loads a thread and tile
-  constexpr int LOAD_ROWS = AT_KEYS / LOADS;          // rows one of them covers
-  constexpr int UNITS = D / 8;                        // 16-byte units of a row
+  constexpr int TILE = TileLoads<D, AT_THREADS>::BYTES;   // 64 keys (or values)
+  constexpr int LOADS = TileLoads<D, AT_THREADS>::COUNT;  // 16-byte loads a thread and tile
   extern __shared__ __align__(16) unsigned char lds[];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   const int half = lane >> 5;
@@ -117,17 +115,14 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
     if (from >= keys && blockIdx.y > 0) return;
   }
 
-  // Loads: load i of this thread brings unit `unit` of row load_row + i LOAD_ROWS.
-  const int slot = threadIdx.x % UNITS, load_row = threadIdx.x / UNITS;
-  const int unit = slot ^ tile_swizzle<D>(load_row);  // the same for all its rows
-  const bool unit_live = unit * 8 < a.dim;
-  const uint32_t lds_base = lds_address(lds) + wave * 1024;
+  const TileLoads<D, AT_THREADS> loads(a.dim);
+  const uint32_t lds_base = lds_address(lds);
   int32_t page[LOADS];
   const auto fetch_pages = [&](int key0) __attribute__((always_inline)) {
     if constexpr (PAGED) {
 #pragma unroll
       for (int i = 0; i < LOADS; i++) {
-        const int key = key0 + load_row + i * LOAD_ROWS;
+        const int key = key0 + loads.row + i * loads.STEP;
         page[i] = key < to ? a.pages.table[u.seg * a.pages.cols + (key >> a.pages.page_shift)] : 0;
       }
     }
@@ -136,26 +131,24 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
     const uint32_t dst = lds_base + stage * (2 * TILE);
 #pragma unroll
     for (int i = 0; i < LOADS; i++) {
-      const int key = key0 + load_row + i * LOAD_ROWS;
-      const uint16_t *ks = (const uint16_t *)&g_zeros, *vs = ks;
-      bool live = unit_live && key < to;
+      const int key = key0 + loads.row + i * loads.STEP;
+      bool there = key < to;
+      const uint16_t *ks, *vs;
       if constexpr (PAGED) {
-        if (key < to && (page[i] < 0 || page[i] >= a.pages.n_pages)) {
-          live = false;
+        if (there && (page[i] < 0 || page[i] >= a.pages.n_pages)) {
+          there = false;
           if (a.failure != nullptr) *a.failure = a.code;
         }
-        if (live) {
-          const int64_t at = (a.pages.row_of(page[i], u.kv_head, a.kv_heads) +
-                              (key & ((1 << a.pages.page_shift) - 1))) * a.dim + unit * 8;
-          ks = a.pages.k + at;
-          vs = a.pages.v + at;
-        }
-      } else if (live) {
-        ks = a.k.at(u.k_first + key, u.kv_head) + unit * 8;
-        vs = a.v.at(u.k_first + key, u.kv_head) + unit * 8;
+        const int64_t at = (a.pages.row_of(page[i], u.kv_head, a.kv_heads) +
+                            (key & ((1 << a.pages.page_shift) - 1))) * a.dim;
+        ks = a.pages.k + at;
+        vs = a.pages.v + at;
+      } else {
+        ks = a.k.at(u.k_first + key, u.kv_head);
+        vs = a.v.at(u.k_first + key, u.kv_head);
       }
-      load_to_lds(ks, dst + i * (AT_THREADS * 16));
-      load_to_lds(vs, dst + TILE + i * (AT_THREADS * 16));
+      loads.load(ks, there, dst, i);
+      loads.load(vs, there, dst + TILE, i);
     }
   };
 

@@ -194,10 +194,31 @@ template <int D> __device__ __forceinline__ uint4 tile_columns(const unsigned ch
   return uint4{lo.x, lo.y, hi.x, hi.y};
 }
 
+static __device__ uint4 g_zeros;  // what is loaded in place of rows and units that are not there
+
+// A block's loads of a tile of 64 rows: load i of a thread brings 16-byte unit
+// `unit` of row `row` + i * STEP to its place (a thread's slot and, with it, its
+// unit are the same in all its rows).
+template <int D, int THREADS> struct TileLoads {
+  static constexpr int BYTES = 64 * D * 2, COUNT = BYTES / (THREADS * 16), STEP = 64 / COUNT;
+  static_assert(COUNT > 0 && STEP % 16 == 0, "the swizzle repeats every 16 rows");
+  int row, unit;
+  bool live;  // the unit has components below dim; the others are zeros
+  uint32_t lds;  // where the wave's first load goes in the tile at LDS address 0
+  __device__ __forceinline__ explicit TileLoads(int dim) {
+    row = threadIdx.x / (D / 8);
+    unit = (threadIdx.x % (D / 8)) ^ tile_swizzle<D>(row);
+    live = unit * 8 < dim;
+    lds = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE) * 1024;
+  }
+  __device__ __forceinline__ void load(const uint16_t *row_data, bool there, uint32_t tile, int i) const {
+    const void *src = there && live ? (const void *)(row_data + unit * 8) : (const void *)&g_zeros;
+    load_to_lds(src, tile + lds + i * (THREADS * 16));
+  }
+};
+
 // The value a lane's partner in the other half of the wave holds.
 __device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
-
-static __device__ uint4 g_zeros;  // what loads past the end of a tile read
 
 // Reports broken segments; every thread of the calling block takes part.
 __device__ __forceinline__ void report_segments(const int64_t *offsets, const int64_t *lens, int64_t m,

@@ -3,109 +3,457 @@
 
 namespace fa {
 
+constexpr int AG_WAVES = 4, AG_THREADS = AG_WAVES * WAVE;
+constexpr int AG_ROWS = 32 * AG_WAVES;  // query rows (keys) a block of the first (second) kernel owns
+constexpr int AG_STEP = 64;             // keys (query rows) a step
+// A row of few keys has an output as large as its values, and D taken from the
+// rounded output is then off by as much as a rounding of the scores' derivative;
+// rows with fewer keys than this take D from the weights instead.
+constexpr int AG_EXACT_KEYS = 64;
+// Steps that are worth a part of their own when the rows of a key tile are split.
+constexpr int AG_PART_STEPS = 16;
+constexpr float LOG2E = 1.44269504088896341f;
+
 struct GradArgs {
   Heads q, k, v, out, dout, dq, dk, dv;
   const float *lse;
-  float *delta;  // [q_rows][heads]: dout . out
+  float *delta;  // [q_rows][heads]: D
+  float *part;   // sums of the parts of split key tiles
   int64_t q_rows, k_rows;
   int heads, kv_heads, group, dim;
   const int64_t *q_offsets, *q_lens, *k_offsets, *k_lens;
   int64_t m;
   float scale;
-  int causal;
+  int causal, parts;
   int32_t *failure, code;
 };
 
-// Two components a lane, as in the forward kernel.
-template <class E> __device__ __forceinline__ void load2(float (&x)[2], const uint16_t *p, int dim) {
+template <int D> __device__ __forceinline__ void load_operand(uint4 (&x)[D / 16], const uint16_t *src, int dim) {
 #pragma unroll
-  for (int c = 0; c < 2; c++) {
-    const int d = lane_id() + 64 * c;
-    x[c] = d < dim ? E::load(p[d]) : 0.0f;
+  for (int s = 0; s < D / 16; s++) {
+    const int c = s * 16 + (lane_id() >> 5) * 8;
+    x[s] = c < dim ? *reinterpret_cast<const uint4 *>(src + c) : uint4{0, 0, 0, 0};
   }
 }
-template <class E> __device__ __forceinline__ void store2(const float (&x)[2], uint16_t *p, int dim) {
+template <int D> __device__ __forceinline__ void clear(f32x16 (&x)[D / 32]) {
 #pragma unroll
-  for (int c = 0; c < 2; c++) {
-    const int d = lane_id() + 64 * c;
-    if (d < dim) p[d] = E::store(x[c]);
-  }
+  for (int t = 0; t < D / 32; t++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) x[t][i] = 0.0f;
 }
-__device__ __forceinline__ float dot2(const float (&a)[2], const float (&b)[2]) {
-  float s = a[0] * b[0] + a[1] * b[1];
-  for (int step = 1; step < WAVE; step *= 2) s += __shfl_xor(s, step);
-  return s;
+// A lane's column of a transposed result, as a row of the output.
+template <class E, int D>
+__device__ __forceinline__ void store_column(const f32x16 (&x)[D / 32], float factor, uint16_t *dst, int dim) {
+#pragma unroll
+  for (int t = 0; t < D / 32; t++)
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) {
+      const int d = t * 32 + 2 * i + 4 * (lane_id() >> 5);
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) w[j] = E::store(x[t][i + j] * factor);
+      if (d < dim) *reinterpret_cast<uint2 *>(dst + d) = uint2{w[0] | w[1] << 16, w[2] | w[3] << 16};
+    }
 }
-
-// A wave per query row and head: delta, then dq over the keys the row sees.
-template <class E> __global__ __launch_bounds__(256) void attention_dq_kernel(GradArgs a) {
-  if (blockIdx.x == 0 && blockIdx.y == 0) {
+// dq and D.  Laid out as the forward kernel: 128 query rows of a key head, a wave
+// owns 32 of them, 64 keys a step;
+//   S^T = K Q^T, dP^T = V dO^T, dS^T = P^T (dP^T - D), dQ^T += K^T dS^T,
+// where K is read from one tile both by rows and by columns.
+template <class E, int D> __global__ __launch_bounds__(AG_THREADS, 2) void attention_dq_kernel(GradArgs a) {
+  constexpr int TILE = TileLoads<D, AG_THREADS>::BYTES;
+  extern __shared__ __align__(16) unsigned char lds[];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), half = lane >> 5;
+  if (blockIdx.x == 0) {
     report_segments(a.q_offsets, a.q_lens, a.m, a.q_rows, a.failure, a.code);
     report_segments(a.k_offsets, a.k_lens, a.m, a.k_rows, a.failure, a.code);
   }
-  const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / WAVE;
-  const int h = blockIdx.y;
-  if (row >= a.q_rows) return;
-  int64_t q_first, q_len, k_first, k_len;
-  const int64_t seg = segment_of_row(a.q_offsets, a.q_lens, a.m, a.q_rows, row, q_first, q_len);
-  if (seg < 0 || !segment_ok(a.k_offsets, a.k_lens, seg, a.k_rows, k_first, k_len)) return;
-  float q[2], o[2], g[2], dq[2] = {0.0f, 0.0f};
-  load2<E>(q, a.q.at(row, h), a.dim);
-  load2<E>(o, a.out.at(row, h), a.dim);
-  load2<E>(g, a.dout.at(row, h), a.dim);
-  const float delta = dot2(o, g), lse = a.lse[row * a.heads + h];
-  if (lane_id() == 0) a.delta[row * a.heads + h] = delta;
-  const int64_t keys = a.causal ? row - q_first + (k_len - q_len) + 1 : k_len;
-  for (int64_t j = 0; j < keys; j++) {
-    float k[2], v[2];
-    load2<E>(k, a.k.at(k_first + j, h / a.group), a.dim);
-    load2<E>(v, a.v.at(k_first + j, h / a.group), a.dim);
-    const float p = lse == -INFINITY ? 0.0f : __expf(dot2(q, k) * a.scale - lse);
-    const float ds = p * (dot2(g, v) - delta) * a.scale;
-    dq[0] += ds * k[0];
-    dq[1] += ds * k[1];
-  }
-  store2<E>(dq, a.dq.at(row, h), a.dim);
-}
+  const int per_tile = AG_ROWS / a.group, kv_head = blockIdx.x % a.kv_heads;
+  SegTile t;
+  if (!find_tile(a.q_offsets, a.q_lens, a.q_rows, a.k_offsets, a.k_lens, a.k_rows, a.m, per_tile,
+                 blockIdx.x / a.kv_heads, t))
+    return;
+  const int q_len = (int)t.len, k_len = (int)t.len2;
+  const int t0 = (int)(t.tiles - 1 - t.tile) * per_tile;  // the last tokens see most: they start first
+  const int tokens = q_len - t0 < per_tile ? q_len - t0 : per_tile;
+  const int behind = k_len - q_len;
+  const auto last_key = [&](int token) { return a.causal ? t0 + token + behind : k_len - 1; };
+  const int rows = tokens * a.group, row = wave * 32 + (lane & 31);
+  const int my_row = row < rows ? row : rows - 1;
+  const int token = my_row / a.group, head = kv_head * a.group + my_row % a.group;
+  const int limit = last_key(token);
+  const bool wave_works = wave * 32 < rows;
+  const int wave_last = __builtin_amdgcn_readfirstlane(
+      last_key(((wave + 1) * 32 < rows ? (wave + 1) * 32 - 1 : rows - 1) / a.group));
+  const int wave_first = __builtin_amdgcn_readfirstlane(last_key(wave_works ? wave * 32 / a.group : 0));
+  const int keys = last_key(tokens - 1) + 1;
 
-// A wave per key row and key head: dk and dv over the query rows that see it,
-// of all the query heads of the group.
-template <class E> __global__ __launch_bounds__(256) void attention_dkv_kernel(GradArgs a) {
-  const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / WAVE;
-  const int h = blockIdx.y;
-  if (row >= a.k_rows) return;
-  int64_t q_first, q_len, k_first, k_len;
-  const int64_t seg = segment_of_row(a.k_offsets, a.k_lens, a.m, a.k_rows, row, k_first, k_len);
-  if (seg < 0 || !segment_ok(a.q_offsets, a.q_lens, seg, a.q_rows, q_first, q_len)) return;
-  float k[2], v[2], dk[2] = {0.0f, 0.0f}, dv[2] = {0.0f, 0.0f};
-  load2<E>(k, a.k.at(row, h), a.dim);
-  load2<E>(v, a.v.at(row, h), a.dim);
-  int64_t from = a.causal ? row - k_first - (k_len - q_len) : 0;
-  if (from < 0) from = 0;
-  for (int qh = h * a.group; qh < (h + 1) * a.group; qh++)
-    for (int64_t i = from; i < q_len; i++) {
-      float q[2], g[2];
-      load2<E>(q, a.q.at(q_first + i, qh), a.dim);
-      load2<E>(g, a.dout.at(q_first + i, qh), a.dim);
-      const float lse = a.lse[(q_first + i) * a.heads + qh], delta = a.delta[(q_first + i) * a.heads + qh];
-      const float p = lse == -INFINITY ? 0.0f : __expf(dot2(q, k) * a.scale - lse);
-      const float ds = p * (dot2(g, v) - delta) * a.scale;
+  const TileLoads<D, AG_THREADS> loads(a.dim);
+  const uint32_t lds_base = lds_address(lds);
+  const auto fetch = [&](int key0, int stage) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < loads.COUNT; i++) {
+      const int key = key0 + loads.row + i * loads.STEP;
+      loads.load(a.k.at(t.first2 + key, kv_head), key < keys, lds_base + stage * (2 * TILE), i);
+      loads.load(a.v.at(t.first2 + key, kv_head), key < keys, lds_base + stage * (2 * TILE) + TILE, i);
+    }
+  };
+
+  const int64_t at = t.first + t0 + token;
+  uint4 q[D / 16], g[D / 16];
+  load_operand<D>(q, a.q.at(at, head), a.dim);
+  load_operand<D>(g, a.dout.at(at, head), a.dim);
+  float delta = 0.0f;
+  {
+    uint4 o[D / 16];
+    load_operand<D>(o, a.out.at(at, head), a.dim);
+#pragma unroll
+    for (int s = 0; s < D / 16; s++)
+      for (int w = 0; w < 4; w++) {
+        const uint32_t x = (&o[s].x)[w], y = (&g[s].x)[w];
+        delta += E::load((uint16_t)x) * E::load((uint16_t)y) + E::load((uint16_t)(x >> 16)) * E::load((uint16_t)(y >> 16));
+      }
+    delta += other_half(delta);
+  }
+  // A row that sees nothing has lse = -inf; its weights must come out as zero.
+  const float lse = a.lse[at * a.heads + head];
+  const float shift = lse == -INFINITY ? INFINITY : lse * LOG2E, scale_log2 = a.scale * LOG2E;
+  f32x16 dq[D / 32];
+  clear<D>(dq);
+
+  // Weights and derivatives of their scores' products for keys b .. b+31 of the tile.
+  const auto weights = [&](const unsigned char *kt, int key0, int b, f32x16 &p, f32x16 &dp) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 16; i++) p[i] = dp[i] = 0.0f;
+#pragma unroll
+    for (int s = 0; s < D / 16; s++) {
+      p = E::mfma(tile_rows<D>(kt, b + (lane & 31), s), q[s], p);
+      dp = E::mfma(tile_rows<D>(kt + TILE, b + (lane & 31), s), g[s], dp);
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], scale_log2, -shift));
+    if (key0 + b + 31 > wave_first) {
+#pragma unroll
+      for (int i = 0; i < 16; i++)
+        if (key0 + b + 8 * (i >> 2) + 4 * half + (i & 3) > limit) p[i] = 0.0f;
+    }
+  };
+  // All keys, `step` for each 64 of them.
+  const auto walk = [&](auto step) __attribute__((always_inline)) {
+    if (keys > 0) fetch(0, 0);
+    int stage = 0;
+    for (int key0 = 0; key0 < keys; key0 += AG_STEP, stage ^= 1) {
+      wait_loads();
+      __syncthreads();
+      if (key0 + AG_STEP < keys) fetch(key0 + AG_STEP, stage ^ 1);
+      if (wave_works && key0 <= wave_last) step(lds + stage * (2 * TILE), key0);
+    }
+  };
+  if (last_key(0) < AG_EXACT_KEYS) {
+    float d = 0.0f;
+    walk([&](const unsigned char *kt, int key0) __attribute__((always_inline)) {
+      for (int b = 0; b < AG_STEP; b += 32) {
+        f32x16 p, dp;
+        weights(kt, key0, b, p, dp);
+#pragma unroll
+        for (int i = 0; i < 16; i++) d += p[i] * dp[i];
+      }
+    });
+    delta = d + other_half(d);
+    __syncthreads();  // the tiles are read again from the start
+  }
+  if (row < rows && half == 0) a.delta[at * a.heads + head] = delta;
+  walk([&](const unsigned char *kt, int key0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < AG_STEP; b += 32) {
+      f32x16 p, dp;
+      weights(kt, key0, b, p, dp);
 #pragma unroll
       for (int c = 0; c < 2; c++) {
-        dk[c] += ds * q[c];
-        dv[c] += p * g[c];
+        f32x8 w;
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i] = p[c * 8 + i] * (dp[c * 8 + i] - delta);
+        const uint4 ds = E::pack(w);
+#pragma unroll
+        for (int dt = 0; dt < D / 32; dt++)
+          dq[dt] = E::mfma(tile_columns<D>(kt, b + c * 16, dt * 32), ds, dq[dt]);
       }
     }
-  store2<E>(dk, a.dk.at(row, h), a.dim);
-  store2<E>(dv, a.dv.at(row, h), a.dim);
+  });
+  if (row < rows) store_column<E, D>(dq, a.scale, a.dq.at(at, head), a.dim);
+}
+
+// The query rows of a key tile, in steps of AG_STEP: `heads` query heads side by
+// side (all of the group up to 64 of them, else in `chunks` rounds) for `tokens`
+// tokens.
+struct RowSteps {
+  int heads, chunks, tokens, first, per_chunk;  // first token, steps of a chunk
+  __device__ __forceinline__ RowSteps(int group, int q_len, int from) {
+    heads = group < AG_STEP ? group : AG_STEP;
+    chunks = (group + heads - 1) / heads;
+    tokens = AG_STEP / heads;
+    first = from;
+    per_chunk = from < q_len ? (q_len - from + tokens - 1) / tokens : 0;
+  }
+  __device__ __forceinline__ int64_t count() const { return (int64_t)chunks * per_chunk; }
+};
+__device__ __forceinline__ int parts_of(int64_t steps, int most) {
+  const int64_t worth = (steps + AG_PART_STEPS - 1) / AG_PART_STEPS;
+  return worth < 1 ? 1 : (worth < most ? (int)worth : most);
+}
+// First token that sees a key of the tile from key0 on.
+__device__ __forceinline__ int first_token(const GradArgs &a, int key0, int q_len, int k_len) {
+  const int from = a.causal ? key0 - (k_len - q_len) : 0;
+  return from > 0 ? from : 0;
+}
+// Where part `part` of a key tile leaves its sums: dk then dv, [128][D] each.
+template <int D> __device__ __forceinline__ float *part_sums(const GradArgs &a, int64_t tile, int part) {
+  return a.part + (tile * a.parts + part) * (2 * AG_ROWS * D);
+}
+
+// dk and dv.  A block owns 128 keys of a key head, a wave 32 of them with K and V
+// as right operands in registers, and walks the query rows that see them, all
+// heads of the group, 64 a step:
+//   S = Q K^T, dP = dO V^T, dS = P (dP - D), dV^T += dO^T P, dK^T += Q^T dS,
+// with Q and dO read from one tile each by rows and by columns.  The keys at the
+// start of a long sequence are seen by all its rows: their rows are split over
+// `parts` blocks, whose sums a second kernel adds in order.
+template <class E, int D> __global__ __launch_bounds__(AG_THREADS, 2) void attention_dkv_kernel(GradArgs a) {
+  constexpr int TILE = TileLoads<D, AG_THREADS>::BYTES, STAGE = 2 * TILE + 3 * AG_STEP * 4;
+  extern __shared__ __align__(16) unsigned char lds[];
+  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), half = lane >> 5;
+  const int kv_head = blockIdx.x % a.kv_heads, part = blockIdx.y;
+  SegTile t;
+  if (!find_tile(a.k_offsets, a.k_lens, a.k_rows, a.q_offsets, a.q_lens, a.q_rows, a.m, AG_ROWS,
+                 blockIdx.x / a.kv_heads, t))
+    return;
+  const int k_len = (int)t.len, q_len = (int)t.len2, key0 = (int)t.tile * AG_ROWS, behind = k_len - q_len;
+  const RowSteps steps(a.group, q_len, first_token(a, key0, q_len, k_len));
+  const int parts = parts_of(steps.count(), a.parts);
+  if (part >= parts) return;
+  const int64_t from = steps.count() * part / parts, to = steps.count() * (part + 1) / parts;
+
+  const int key = key0 + wave * 32 + (lane & 31);
+  const int wave_last = key0 + wave * 32 + 31;
+  uint4 k[D / 16], v[D / 16];
+  {
+    const int64_t at = t.first + (key < k_len ? key : k_len - 1);
+    load_operand<D>(k, a.k.at(at, kv_head), a.dim);
+    load_operand<D>(v, a.v.at(at, kv_head), a.dim);
+  }
+  f32x16 dk[D / 32], dv[D / 32];
+  clear<D>(dk);
+  clear<D>(dv);
+
+  const TileLoads<D, AG_THREADS> loads(a.dim);
+  const uint32_t lds_base = lds_address(lds);
+  // Row r of a step is token r / heads, head r % heads of the step's tokens and chunk.
+  const auto place = [&](int r, int64_t step, int &token, int &head) __attribute__((always_inline)) {
+    const int chunk = (int)(step / steps.per_chunk);
+    token = steps.first + (int)(step - (int64_t)chunk * steps.per_chunk) * steps.tokens + r / steps.heads;
+    const int h = chunk * steps.heads + r % steps.heads;
+    head = kv_head * a.group + h;
+    return r < steps.tokens * steps.heads && h < a.group && token < q_len;
+  };
+  const auto fetch = [&](int64_t step, int stage) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < loads.COUNT; i++) {
+      int token, head;
+      const bool there = place(loads.row + i * loads.STEP, step, token, head);
+      loads.load(a.q.at(t.first2 + token, head), there, lds_base + stage * STAGE, i);
+      loads.load(a.dout.at(t.first2 + token, head), there, lds_base + stage * STAGE + TILE, i);
+    }
+  };
+  // Of every row: log2 of the sum (infinite where there is no row or it sees
+  // nothing: weights become zero), D, and the last key it sees.
+  float row_shift = 0.0f, row_delta = 0.0f;
+  int row_last = 0;
+  const auto fetch_row = [&](int64_t step) __attribute__((always_inline)) {
+    if (threadIdx.x < AG_STEP) {
+      int token, head;
+      const bool there = place(threadIdx.x, step, token, head);
+      const int64_t at = there ? (t.first2 + token) * a.heads + head : 0;
+      const float lse = there ? a.lse[at] : -INFINITY;
+      row_shift = lse == -INFINITY ? INFINITY : lse * LOG2E;
+      row_delta = there ? a.delta[at] : 0.0f;
+      row_last = a.causal ? token + behind : INT32_MAX;
+    }
+  };
+  const auto put_row = [&](int stage) __attribute__((always_inline)) {
+    if (threadIdx.x < AG_STEP) {
+      float *x = reinterpret_cast<float *>(lds + stage * STAGE + 2 * TILE);
+      x[threadIdx.x] = row_shift;
+      x[AG_STEP + threadIdx.x] = row_delta;
+      reinterpret_cast<int *>(x)[2 * AG_STEP + threadIdx.x] = row_last;
+    }
+  };
+  const float scale_log2 = a.scale * LOG2E;
+  if (from < to) {
+    fetch_row(from);
+    fetch(from, 0);
+    put_row(0);
+  }
+  int stage = 0;
+  for (int64_t step = from; step < to; step++, stage ^= 1) {
+    wait_loads();
+    __syncthreads();
+    if (step + 1 < to) {
+      fetch_row(step + 1);
+      fetch(step + 1, stage ^ 1);
+    }
+    const unsigned char *qt = lds + stage * STAGE, *gt = qt + TILE;
+    const float *shifts = reinterpret_cast<const float *>(qt + 2 * TILE), *deltas = shifts + AG_STEP;
+    const int *lasts = reinterpret_cast<const int *>(deltas + AG_STEP);
+    // the step's first row sees least
+    const bool masked = a.causal && lasts[0] < wave_last;
+#pragma unroll
+    for (int b = 0; b < AG_STEP; b += 32) {
+      f32x16 p, dp;
+#pragma unroll
+      for (int i = 0; i < 16; i++) p[i] = dp[i] = 0.0f;
+#pragma unroll
+      for (int s = 0; s < D / 16; s++) {
+        p = E::mfma(tile_rows<D>(qt, b + (lane & 31), s), k[s], p);
+        dp = E::mfma(tile_rows<D>(gt, b + (lane & 31), s), v[s], dp);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const f32x4 shift = *reinterpret_cast<const f32x4 *>(shifts + b + 8 * j + 4 * half);
+#pragma unroll
+        for (int i = 0; i < 4; i++) p[4 * j + i] = __builtin_amdgcn_exp2f(fmaf(p[4 * j + i], scale_log2, -shift[i]));
+      }
+      if (masked) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int4 last = *reinterpret_cast<const int4 *>(lasts + b + 8 * j + 4 * half);
+          if (key > last.x) p[4 * j] = 0.0f;
+          if (key > last.y) p[4 * j + 1] = 0.0f;
+          if (key > last.z) p[4 * j + 2] = 0.0f;
+          if (key > last.w) p[4 * j + 3] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; c++) {
+        f32x8 w, ds;
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const f32x4 delta = *reinterpret_cast<const f32x4 *>(deltas + b + 16 * c + 8 * j + 4 * half);
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            w[4 * j + i] = p[8 * c + 4 * j + i];
+            ds[4 * j + i] = w[4 * j + i] * (dp[8 * c + 4 * j + i] - delta[i]);
+          }
+        }
+        const uint4 pw = E::pack(w), pds = E::pack(ds);
+#pragma unroll
+        for (int dt = 0; dt < D / 32; dt++) {
+          dv[dt] = E::mfma(tile_columns<D>(gt, b + 16 * c, dt * 32), pw, dv[dt]);
+          dk[dt] = E::mfma(tile_columns<D>(qt, b + 16 * c, dt * 32), pds, dk[dt]);
+        }
+      }
+    }
+    if (step + 1 < to) put_row(stage ^ 1);
+  }
+  if (parts > 1) {
+    float *dst = part_sums<D>(a, blockIdx.x, part) + (wave * 32 + (lane & 31)) * D;
+#pragma unroll
+    for (int dt = 0; dt < D / 32; dt++)
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) {
+        const int d = dt * 32 + 2 * i + 4 * half;
+        *reinterpret_cast<f32x4 *>(dst + d) = f32x4{dk[dt][i], dk[dt][i + 1], dk[dt][i + 2], dk[dt][i + 3]};
+        *reinterpret_cast<f32x4 *>(dst + AG_ROWS * D + d) =
+            f32x4{dv[dt][i], dv[dt][i + 1], dv[dt][i + 2], dv[dt][i + 3]};
+      }
+  } else if (key < k_len) {
+    store_column<E, D>(dk, a.scale, a.dk.at(t.first + key, kv_head), a.dim);
+    store_column<E, D>(dv, 1.0f, a.dv.at(t.first + key, kv_head), a.dim);
+  }
+}
+
+// Adds the parts of the split key tiles: a block an eighth of a tile, four components a thread.
+template <class E, int D> __global__ __launch_bounds__(AG_THREADS) void attention_dkv_join_kernel(GradArgs a) {
+  const int kv_head = blockIdx.x % a.kv_heads;
+  SegTile t;
+  if (!find_tile(a.k_offsets, a.k_lens, a.k_rows, a.q_offsets, a.q_lens, a.q_rows, a.m, AG_ROWS,
+                 blockIdx.x / a.kv_heads, t))
+    return;
+  const int k_len = (int)t.len, q_len = (int)t.len2, key0 = (int)t.tile * AG_ROWS;
+  const int parts = parts_of(RowSteps(a.group, q_len, first_token(a, key0, q_len, k_len)).count(), a.parts);
+  if (parts == 1) return;
+  constexpr int ROWS = AG_ROWS / 8, FOURS = D / 4;
+  for (int i = threadIdx.x; i < ROWS * FOURS; i += AG_THREADS) {
+    const int row = blockIdx.y * ROWS + i / FOURS, d = i % FOURS * 4;
+    if (key0 + row >= k_len || d >= a.dim) continue;
+    f32x4 dk = {0.0f, 0.0f, 0.0f, 0.0f}, dv = dk;
+    for (int p = 0; p < parts; p++) {
+      const float *src = part_sums<D>(a, blockIdx.x, p) + row * D + d;
+      dk += *reinterpret_cast<const f32x4 *>(src);
+      dv += *reinterpret_cast<const f32x4 *>(src + AG_ROWS * D);
+    }
+    uint32_t x[4], y[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      x[j] = E::store(dk[j] * a.scale);
+      y[j] = E::store(dv[j]);
+    }
+    const int64_t at = t.first + key0 + row;
+    *reinterpret_cast<uint2 *>(a.dk.at(at, kv_head) + d) = uint2{x[0] | x[1] << 16, x[2] | x[3] << 16};
+    *reinterpret_cast<uint2 *>(a.dv.at(at, kv_head) + d) = uint2{y[0] | y[1] << 16, y[2] | y[3] << 16};
+  }
+}
+
+// Workspace: D of every row and head, then the parts.  Key tiles are split so
+// that there are about four blocks for every place on the chip (two a CU).
+struct GradPlan {
+  int64_t tiles;
+  int parts;
+  size_t delta_bytes, part_bytes;
+};
+static GradPlan grad_plan(int64_t q_rows, int64_t k_rows, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t m) {
+  GradPlan p;
+  p.tiles = most_tiles(k_rows, m, AG_ROWS) * kv_heads;
+  const int64_t wanted = p.tiles > 0 ? ceil_div(8 * NUM_CUS_HINT, p.tiles) : 1;
+  p.parts = (int)(wanted < 8 ? wanted : 8);
+  // no tile has more steps than the rows of one head group make
+  const int64_t group = heads / kv_heads, lanes = group < AG_STEP ? group : AG_STEP;
+  const int64_t steps = ceil_div(group, lanes) * ceil_div(q_rows, AG_STEP / lanes);
+  if (p.parts > ceil_div(steps, AG_PART_STEPS)) p.parts = (int)ceil_div(steps, AG_PART_STEPS);
+  if (p.parts < 1) p.parts = 1;
+  p.delta_bytes = (size_t)ceil_div(q_rows * heads, 4) * 16;
+  p.part_bytes = p.parts > 1 ? (size_t)p.tiles * p.parts * 2 * AG_ROWS * (head_dim <= 64 ? 64 : 128) * sizeof(float) : 0;
+  return p;
+}
+
+template <class E, int D> static int launch_grad(hipStream_t stream, const GradArgs &a, const GradPlan &p) {
+  constexpr int TILE = TileLoads<D, AG_THREADS>::BYTES, STAGE = 2 * TILE + 3 * AG_STEP * 4;
+  const auto dkv = attention_dkv_kernel<E, D>;
+  static const hipError_t raised =
+      hipFuncSetAttribute((const void *)dkv, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * STAGE);
+  if (raised != hipSuccess) return (int)raised;
+  const int64_t units = most_tiles(a.q_rows, a.m, AG_ROWS / a.group) * a.kv_heads;
+  if (units > INT32_MAX || p.tiles > INT32_MAX) return FA_ENOTSUP;
+  if (units > 0) {
+    attention_dq_kernel<E, D><<<dim3((unsigned)units), AG_THREADS, 4 * TILE, stream>>>(a);
+    const int rc = launch_status();
+    if (rc != 0) return rc;
+  }
+  if (p.tiles == 0) return 0;
+  dkv<<<dim3((unsigned)p.tiles, (unsigned)p.parts), AG_THREADS, 2 * STAGE, stream>>>(a);
+  const int rc = launch_status();
+  if (rc != 0 || p.parts == 1) return rc;
+  attention_dkv_join_kernel<E, D><<<dim3((unsigned)p.tiles, 8), AG_THREADS, 0, stream>>>(a);
+  return launch_status();
 }
 
 }  // namespace fa
 
 extern "C" size_t fa_attention_grad_workspace_bytes(int64_t q_rows, int64_t k_rows, int64_t heads,
                                                     int64_t kv_heads, int64_t head_dim, int64_t m) {
-  (void)k_rows, (void)kv_heads, (void)head_dim, (void)m;
-  return q_rows > 0 && heads > 0 ? (size_t)q_rows * heads * sizeof(float) : 0;
+  if (q_rows < 0 || k_rows < 0 || m <= 0 || q_rows > AT_MOST_ROWS || k_rows > AT_MOST_ROWS || m > AT_MOST_ROWS ||
+      check_shape(FA_F16, heads, kv_heads, head_dim) != 0)
+    return 0;
+  const GradPlan p = grad_plan(q_rows, k_rows, heads, kv_heads, head_dim, m);
+  return p.delta_bytes + p.part_bytes;
 }
 
 extern "C" int fa_attention_grad(fa_stream_t stream, fa_dtype t, const fa_heads *q, int64_t q_rows,
@@ -136,20 +484,13 @@ extern "C" int fa_attention_grad(fa_stream_t stream, fa_dtype t, const fa_heads 
   const size_t need = fa_attention_grad_workspace_bytes(q_rows, k_rows, heads, kv_heads, head_dim, m);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need)) return FA_ESCRATCH;
   if (!is_aligned(workspace, 16)) return FA_EALIGN;
+  const GradPlan p = grad_plan(q_rows, k_rows, heads, kv_heads, head_dim, m);
   const GradArgs a = {to_heads(q), to_heads(k), to_heads(v), to_heads(out), to_heads(dout), to_heads(dq),
-                      to_heads(dk), to_heads(dv), lse, (float *)workspace, q_rows, k_rows, (int)heads,
-                      (int)kv_heads, (int)(heads / kv_heads), (int)head_dim, q_offsets, q_lens, k_offsets,
-                      k_lens, m, scale, causal, failure, code};
-  if (q_rows > 0) {
-    const auto kernel = t == FA_F16 ? attention_dq_kernel<ElemF16> : attention_dq_kernel<ElemBF16>;
-    kernel<<<dim3((unsigned)ceil_div(q_rows, 4), (unsigned)heads), dim3(256), 0, (hipStream_t)stream>>>(a);
-    rc = launch_status();
-    if (rc != 0) return rc;
-  }
-  if (k_rows > 0) {
-    const auto kernel = t == FA_F16 ? attention_dkv_kernel<ElemF16> : attention_dkv_kernel<ElemBF16>;
-    kernel<<<dim3((unsigned)ceil_div(k_rows, 4), (unsigned)kv_heads), dim3(256), 0, (hipStream_t)stream>>>(a);
-    rc = launch_status();
-  }
-  return rc;
+                      to_heads(dk), to_heads(dv), lse, (float *)workspace,
+                      (float *)((char *)workspace + p.delta_bytes), q_rows, k_rows, (int)heads, (int)kv_heads,
+                      (int)(heads / kv_heads), (int)head_dim, q_offsets, q_lens, k_offsets, k_lens, m, scale,
+                      causal != 0, p.parts, failure, code};
+  const hipStream_t s = (hipStream_t)stream;
+  if (t == FA_F16) return head_dim <= 64 ? launch_grad<ElemF16, 64>(s, a, p) : launch_grad<ElemF16, 128>(s, a, p);
+  return head_dim <= 64 ? launch_grad<ElemBF16, 64>(s, a, p) : launch_grad<ElemBF16, 128>(s, a, p);
 }
