@@ -22,26 +22,6 @@ namespace fa {
 constexpr int AT_WAVES = 4, AT_THREADS = AT_WAVES * WAVE;
 constexpr int AT_ROWS = 32 * AT_WAVES;  // query rows a block
 constexpr int AT_KEYS = 64;             // keys a step
-// A wave rescales its output only when a maximum has grown by 2^8 since it last
-// did: until then weights are at most 2^8, which f16 and bf16 hold as well as 1.
-constexpr float AT_RESCALE = 8.0f;
-
-struct AttentionArgs {
-  Heads q, k, v, out;
-  float *lse;
-  int64_t q_rows, k_rows;
-  int heads, kv_heads, group, dim;
-  const int64_t *q_offsets, *q_lens, *k_offsets, *k_lens;
-  int64_t m;
-  float scale_log2;  // scale * log2(e)
-  int causal;
-  int32_t *failure, code;
-  // paged only: the cache; keys of a unit that one block takes, and where parts go
-  Pages pages;
-  int chunk, splits;
-  float *part_o, *part_ml;
-};
-
 // Keys, values and query rows a block works on.
 struct Unit {
   int64_t seg, q_first, k_first;
@@ -215,7 +195,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
       float high = s[0][0];
 #pragma unroll
       for (int i = 1; i < 32; i++) high = fmaxf(high, s[i >> 4][i & 15]);
-      high = fmaxf(high, other_half(high)) * a.scale_log2;
+      high = fold_halves(high, FMax()) * a.scale_log2;
       if (__any(high > top + AT_RESCALE)) {
         const float now = fmaxf(top, high);
         const float factor = now == -INFINITY ? 1.0f : exp2f(top - now);
@@ -269,7 +249,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
     }
   }
 
-  sum += other_half(sum);
+  sum = fold_halves(sum, FAdd());
   if (row >= rows) return;
   if (PAGED && keys > a.chunk) {
     const int64_t at = part_row(a, blockIdx.x, blockIdx.y, row);
@@ -300,7 +280,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
       if (d < a.dim) *reinterpret_cast<uint2 *>(dst + d) = uint2{x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16};
     }
   if (a.lse != nullptr && half == 0)
-    a.lse[out_row * a.heads + head] = empty ? -INFINITY : (top + log2f(sum)) * 0.693147180559945309f;
+    a.lse[out_row * a.heads + head] = empty ? -INFINITY : (top + log2f(sum)) * LN2;
 }
 
 // Joins the parts of the units whose keys were split: a wave per query row.
@@ -332,7 +312,7 @@ template <class E, int D> __global__ __launch_bounds__(AT_THREADS) void attentio
     if (d < a.dim) a.out.at(out_row, head)[d] = E::store(top == -INFINITY ? 0.0f : o[c] / sum);
   }
   if (a.lse != nullptr && lane_id() == 0)
-    a.lse[out_row * a.heads + head] = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * 0.693147180559945309f;
+    a.lse[out_row * a.heads + head] = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * LN2;
 }
 
 // How a cache's keys are split over blocks: enough blocks to fill the chip if
@@ -393,7 +373,7 @@ extern "C" int fa_attention(fa_stream_t stream, fa_dtype t, const fa_heads *q, i
   a.heads = (int)heads, a.kv_heads = (int)kv_heads, a.group = (int)(heads / kv_heads), a.dim = (int)head_dim;
   a.q_offsets = q_offsets, a.q_lens = q_lens, a.k_offsets = k_offsets, a.k_lens = k_lens;
   a.m = m;
-  a.scale_log2 = scale * 1.44269504088896341f;
+  a.scale_log2 = scale * LOG2E;
   a.causal = causal != 0;
   a.failure = failure, a.code = code;
   a.splits = 1;
@@ -405,6 +385,8 @@ extern "C" size_t fa_attention_paged_workspace_bytes(int64_t n, int64_t heads, i
   if (n <= 0 || m <= 0 || n > AT_MOST_ROWS || m > AT_MOST_ROWS || page_size <= 0 || table_cols <= 0 ||
       (__int128)page_size * table_cols > AT_MOST_ROWS || check_shape(FA_F16, heads, kv_heads, head_dim) != 0)
     return 0;
+  const int few = few_rows(n, heads, kv_heads, m);
+  if (few > 0) return few_workspace(few, head_dim);
   const SplitPlan p = split_plan(n, heads, kv_heads, m, page_size * table_cols);
   if (p.splits == 1) return 0;
   return (size_t)p.units * p.splits * AT_ROWS * ((head_dim <= 64 ? 64 : 128) + 2) * sizeof(float);
@@ -433,7 +415,7 @@ extern "C" int fa_attention_paged(fa_stream_t stream, fa_dtype t, const fa_heads
     if (workspace == nullptr || workspace_bytes < need) return FA_ESCRATCH;
     if (!is_aligned(workspace, 16)) return FA_EALIGN;
   }
-  const SplitPlan p = split_plan(n, heads, kv_heads, m, page_size * table_cols);
+  const int few = few_rows(n, heads, kv_heads, m);
   AttentionArgs a = {};
   a.q = to_heads(q), a.out = to_heads(out);
   a.lse = lse;
@@ -441,10 +423,12 @@ extern "C" int fa_attention_paged(fa_stream_t stream, fa_dtype t, const fa_heads
   a.heads = (int)heads, a.kv_heads = (int)kv_heads, a.group = (int)(heads / kv_heads), a.dim = (int)head_dim;
   a.q_offsets = offsets, a.q_lens = lens;
   a.m = m;
-  a.scale_log2 = scale * 1.44269504088896341f;
+  a.scale_log2 = scale * LOG2E;
   a.causal = 1;
   a.failure = failure, a.code = code;
   a.pages = to_pages(k_pages, v_pages, n_pages, page_size, page_table, table_cols, past_lens);
+  if (few > 0) return launch_few((hipStream_t)stream, t, few, a, workspace);
+  const SplitPlan p = split_plan(n, heads, kv_heads, m, page_size * table_cols);
   a.chunk = p.chunk, a.splits = p.splits;
   if (p.splits > 1) {
     const int64_t parts = p.units * p.splits * AT_ROWS;

@@ -28,6 +28,10 @@ struct ElemF16 {
   static __device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(bit_cast<f16x8>(a), bit_cast<f16x8>(b), c, 0, 0, 0);
   }
+  // 16 x 32 times 32 x 16: row (column) l % 16, k from 8 (l / 16); C rows 4 (l / 16) + i.
+  static __device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(bit_cast<f16x8>(a), bit_cast<f16x8>(b), c, 0, 0, 0);
+  }
 };
 struct ElemBF16 {
   static constexpr uint32_t exponent = 0x7f80;
@@ -38,6 +42,9 @@ struct ElemBF16 {
   }
   static __device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(bit_cast<bf16x8>(a), bit_cast<bf16x8>(b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 mfma16(uint4 a, uint4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(bit_cast<bf16x8>(a), bit_cast<bf16x8>(b), c, 0, 0, 0);
   }
 };
 
@@ -64,6 +71,34 @@ struct Pages {
     return (page * kv_heads + head) << page_shift;
   }
 };
+
+// What the forward kernels take.
+struct AttentionArgs {
+  Heads q, k, v, out;
+  float *lse;
+  int64_t q_rows, k_rows;
+  int heads, kv_heads, group, dim;
+  const int64_t *q_offsets, *q_lens, *k_offsets, *k_lens;
+  int64_t m;
+  float scale_log2;  // scale * log2(e)
+  int causal;
+  int32_t *failure, code;
+  // paged only: the cache; keys of a unit that one block takes, and where parts go
+  Pages pages;
+  int chunk, splits;
+  float *part_o, *part_ml;
+};
+
+// A wave rescales its output only when a maximum has grown by 2^8 since it last
+// did: until then weights are at most 2^8, which f16 and bf16 hold as well as 1.
+constexpr float AT_RESCALE = 8.0f;
+constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
+
+// attention_few.hip: attention over the cache for few query rows a sequence.
+// Rows a unit of work holds for such a call, or 0 if the other kernel should take it.
+int few_rows(int64_t n, int64_t heads, int64_t kv_heads, int64_t m);
+size_t few_workspace(int rows, int64_t head_dim);
+int launch_few(hipStream_t stream, fa_dtype t, int rows, const AttentionArgs &a, void *workspace);
 
 // ------------------------------------------------------------------ segments
 // Segment i as the rules of fa_segred_irregular read it: inside [0, n), not
@@ -217,8 +252,23 @@ template <int D, int THREADS> struct TileLoads {
   }
 };
 
-// The value a lane's partner in the other half of the wave holds.
-__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32); }
+// Maximum (sum) over the lanes 16 and 32 apart, and over lanes 32 apart alone.
+// A swap of a register with itself leaves the even rows (the lower half) in one
+// result and the odd rows (the upper half) in the other, for all lanes.
+template <class F> __device__ __forceinline__ float fold_halves(float x, F f) {
+  const auto r = __builtin_amdgcn_permlane32_swap(bit_cast<uint32_t>(x), bit_cast<uint32_t>(x), false, false);
+  return f(bit_cast<float>((uint32_t)r[0]), bit_cast<float>((uint32_t)r[1]));
+}
+template <class F> __device__ __forceinline__ float fold_quarters(float x, F f) {
+  const auto r = __builtin_amdgcn_permlane16_swap(bit_cast<uint32_t>(x), bit_cast<uint32_t>(x), false, false);
+  return fold_halves(f(bit_cast<float>((uint32_t)r[0]), bit_cast<float>((uint32_t)r[1])), f);
+}
+struct FMax {
+  __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+struct FAdd {
+  __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
 
 // Reports broken segments; every thread of the calling block takes part.
 __device__ __forceinline__ void report_segments(const int64_t *offsets, const int64_t *lens, int64_t m,

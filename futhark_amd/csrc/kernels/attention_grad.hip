@@ -4,7 +4,7 @@
 namespace fa {
 
 constexpr int AG_WAVES = 4, AG_THREADS = AG_WAVES * WAVE;
-constexpr int AG_ROWS = 32 * AG_WAVES;  // query rows (keys) a block of the first (second) kernel owns
+constexpr int AG_ROWS = 32 * AG_WAVES;  // query rows a block of the first kernel owns
 constexpr int AG_STEP = 64;             // keys (query rows) a step
 // A row of few keys has an output as large as its values, and D taken from the
 // rounded output is then off by as much as a rounding of the scores' derivative;
@@ -12,7 +12,6 @@ constexpr int AG_STEP = 64;             // keys (query rows) a step
 constexpr int AG_EXACT_KEYS = 64;
 // Steps that are worth a part of their own when the rows of a key tile are split.
 constexpr int AG_PART_STEPS = 16;
-constexpr float LOG2E = 1.44269504088896341f;
 
 struct GradArgs {
   Heads q, k, v, out, dout, dq, dk, dv;
@@ -112,7 +111,7 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, 2) void atten
         const uint32_t x = (&o[s].x)[w], y = (&g[s].x)[w];
         delta += E::load((uint16_t)x) * E::load((uint16_t)y) + E::load((uint16_t)(x >> 16)) * E::load((uint16_t)(y >> 16));
       }
-    delta += other_half(delta);
+    delta = fold_halves(delta, FAdd());
   }
   // A row that sees nothing has lse = -inf; its weights must come out as zero.
   const float lse = a.lse[at * a.heads + head];
@@ -158,7 +157,7 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, 2) void atten
         for (int i = 0; i < 16; i++) d += p[i] * dp[i];
       }
     });
-    delta = d + other_half(d);
+    delta = fold_halves(d, FAdd());
     __syncthreads();  // the tiles are read again from the start
   }
   if (row < rows && half == 0) a.delta[at * a.heads + head] = delta;
@@ -205,9 +204,14 @@ __device__ __forceinline__ int first_token(const GradArgs &a, int key0, int q_le
   const int from = a.causal ? key0 - (k_len - q_len) : 0;
   return from > 0 ? from : 0;
 }
-// Where part `part` of a key tile leaves its sums: dk then dv, [128][D] each.
+// Keys a block of the second kernel owns, PER_WAVE times 32 a wave (twice 32 for
+// D = 128 does not fit the registers: 1.6 ms instead of 0.66 ms on 7201 rows).
+template <int D> struct KeyTile {
+  static constexpr int PER_WAVE = 1, KEYS = 32 * PER_WAVE * AG_WAVES;
+};
+// Where part `part` of a key tile leaves its sums: dk then dv, [KEYS][D] each.
 template <int D> __device__ __forceinline__ float *part_sums(const GradArgs &a, int64_t tile, int part) {
-  return a.part + (tile * a.parts + part) * (2 * AG_ROWS * D);
+  return a.part + (tile * a.parts + part) * (2 * KeyTile<D>::KEYS * D);
 }
 
 // dk and dv.  A block owns 128 keys of a key head, a wave 32 of them with K and V
@@ -217,32 +221,34 @@ template <int D> __device__ __forceinline__ float *part_sums(const GradArgs &a, 
 // with Q and dO read from one tile each by rows and by columns.  The keys at the
 // start of a long sequence are seen by all its rows: their rows are split over
 // `parts` blocks, whose sums a second kernel adds in order.
-template <class E, int D> __global__ __launch_bounds__(AG_THREADS, 2) void attention_dkv_kernel(GradArgs a) {
+template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 : 2) void attention_dkv_kernel(GradArgs a) {
   constexpr int TILE = TileLoads<D, AG_THREADS>::BYTES, STAGE = 2 * TILE + 3 * AG_STEP * 4;
+  constexpr int KT = KeyTile<D>::PER_WAVE, KEYS = KeyTile<D>::KEYS;
   extern __shared__ __align__(16) unsigned char lds[];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), half = lane >> 5;
   const int kv_head = blockIdx.x % a.kv_heads, part = blockIdx.y;
   SegTile t;
-  if (!find_tile(a.k_offsets, a.k_lens, a.k_rows, a.q_offsets, a.q_lens, a.q_rows, a.m, AG_ROWS,
+  if (!find_tile(a.k_offsets, a.k_lens, a.k_rows, a.q_offsets, a.q_lens, a.q_rows, a.m, KEYS,
                  blockIdx.x / a.kv_heads, t))
     return;
-  const int k_len = (int)t.len, q_len = (int)t.len2, key0 = (int)t.tile * AG_ROWS, behind = k_len - q_len;
+  const int k_len = (int)t.len, q_len = (int)t.len2, key0 = (int)t.tile * KEYS, behind = k_len - q_len;
   const RowSteps steps(a.group, q_len, first_token(a, key0, q_len, k_len));
   const int parts = parts_of(steps.count(), a.parts);
   if (part >= parts) return;
   const int64_t from = steps.count() * part / parts, to = steps.count() * (part + 1) / parts;
 
-  const int key = key0 + wave * 32 + (lane & 31);
-  const int wave_last = key0 + wave * 32 + 31;
-  uint4 k[D / 16], v[D / 16];
-  {
-    const int64_t at = t.first + (key < k_len ? key : k_len - 1);
-    load_operand<D>(k, a.k.at(at, kv_head), a.dim);
-    load_operand<D>(v, a.v.at(at, kv_head), a.dim);
+  const int key = key0 + wave * (32 * KT) + (lane & 31);  // and 32 further on
+  const int wave_last = key0 + (wave + 1) * (32 * KT) - 1;
+  uint4 k[KT][D / 16], v[KT][D / 16];
+  f32x16 dk[KT][D / 32], dv[KT][D / 32];
+#pragma unroll
+  for (int x = 0; x < KT; x++) {
+    const int64_t at = t.first + (key + 32 * x < k_len ? key + 32 * x : k_len - 1);
+    load_operand<D>(k[x], a.k.at(at, kv_head), a.dim);
+    load_operand<D>(v[x], a.v.at(at, kv_head), a.dim);
+    clear<D>(dk[x]);
+    clear<D>(dv[x]);
   }
-  f32x16 dk[D / 32], dv[D / 32];
-  clear<D>(dk);
-  clear<D>(dv);
 
   const TileLoads<D, AG_THREADS> loads(a.dim);
   const uint32_t lds_base = lds_address(lds);
@@ -307,80 +313,103 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, 2) void atten
     const bool masked = a.causal && lasts[0] < wave_last;
 #pragma unroll
     for (int b = 0; b < AG_STEP; b += 32) {
-      f32x16 p, dp;
+      f32x16 p[KT], dp[KT];
 #pragma unroll
-      for (int i = 0; i < 16; i++) p[i] = dp[i] = 0.0f;
+      for (int x = 0; x < KT; x++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) p[x][i] = dp[x][i] = 0.0f;
 #pragma unroll
       for (int s = 0; s < D / 16; s++) {
-        p = E::mfma(tile_rows<D>(qt, b + (lane & 31), s), k[s], p);
-        dp = E::mfma(tile_rows<D>(gt, b + (lane & 31), s), v[s], dp);
+        const uint4 qr = tile_rows<D>(qt, b + (lane & 31), s), gr = tile_rows<D>(gt, b + (lane & 31), s);
+#pragma unroll
+        for (int x = 0; x < KT; x++) p[x] = E::mfma(qr, k[x][s], p[x]);
+#pragma unroll
+        for (int x = 0; x < KT; x++) dp[x] = E::mfma(gr, v[x][s], dp[x]);
       }
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         const f32x4 shift = *reinterpret_cast<const f32x4 *>(shifts + b + 8 * j + 4 * half);
 #pragma unroll
-        for (int i = 0; i < 4; i++) p[4 * j + i] = __builtin_amdgcn_exp2f(fmaf(p[4 * j + i], scale_log2, -shift[i]));
+        for (int x = 0; x < KT; x++)
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            p[x][4 * j + i] = __builtin_amdgcn_exp2f(fmaf(p[x][4 * j + i], scale_log2, -shift[i]));
       }
       if (masked) {
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           const int4 last = *reinterpret_cast<const int4 *>(lasts + b + 8 * j + 4 * half);
-          if (key > last.x) p[4 * j] = 0.0f;
-          if (key > last.y) p[4 * j + 1] = 0.0f;
-          if (key > last.z) p[4 * j + 2] = 0.0f;
-          if (key > last.w) p[4 * j + 3] = 0.0f;
+#pragma unroll
+          for (int x = 0; x < KT; x++) {
+            if (key + 32 * x > last.x) p[x][4 * j] = 0.0f;
+            if (key + 32 * x > last.y) p[x][4 * j + 1] = 0.0f;
+            if (key + 32 * x > last.z) p[x][4 * j + 2] = 0.0f;
+            if (key + 32 * x > last.w) p[x][4 * j + 3] = 0.0f;
+          }
         }
       }
 #pragma unroll
       for (int c = 0; c < 2; c++) {
-        f32x8 w, ds;
+        uint4 pw[KT], pds[KT];
+        f32x4 delta[2];
 #pragma unroll
-        for (int j = 0; j < 2; j++) {
-          const f32x4 delta = *reinterpret_cast<const f32x4 *>(deltas + b + 16 * c + 8 * j + 4 * half);
+        for (int j = 0; j < 2; j++)
+          delta[j] = *reinterpret_cast<const f32x4 *>(deltas + b + 16 * c + 8 * j + 4 * half);
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            w[4 * j + i] = p[8 * c + 4 * j + i];
-            ds[4 * j + i] = w[4 * j + i] * (dp[8 * c + 4 * j + i] - delta[i]);
+        for (int x = 0; x < KT; x++) {
+          f32x8 w, ds;
+#pragma unroll
+          for (int i = 0; i < 8; i++) {
+            w[i] = p[x][8 * c + i];
+            ds[i] = w[i] * (dp[x][8 * c + i] - delta[i >> 2][i & 3]);
           }
+          pw[x] = E::pack(w);
+          pds[x] = E::pack(ds);
         }
-        const uint4 pw = E::pack(w), pds = E::pack(ds);
 #pragma unroll
         for (int dt = 0; dt < D / 32; dt++) {
-          dv[dt] = E::mfma(tile_columns<D>(gt, b + 16 * c, dt * 32), pw, dv[dt]);
-          dk[dt] = E::mfma(tile_columns<D>(qt, b + 16 * c, dt * 32), pds, dk[dt]);
+          const uint4 gc = tile_columns<D>(gt, b + 16 * c, dt * 32), qc = tile_columns<D>(qt, b + 16 * c, dt * 32);
+#pragma unroll
+          for (int x = 0; x < KT; x++) dv[x][dt] = E::mfma(gc, pw[x], dv[x][dt]);
+#pragma unroll
+          for (int x = 0; x < KT; x++) dk[x][dt] = E::mfma(qc, pds[x], dk[x][dt]);
         }
       }
     }
     if (step + 1 < to) put_row(stage ^ 1);
   }
-  if (parts > 1) {
-    float *dst = part_sums<D>(a, blockIdx.x, part) + (wave * 32 + (lane & 31)) * D;
 #pragma unroll
-    for (int dt = 0; dt < D / 32; dt++)
+  for (int x = 0; x < KT; x++) {
+    if (parts > 1) {
+      float *dst = part_sums<D>(a, blockIdx.x, part) + (key - key0 + 32 * x) * D;
 #pragma unroll
-      for (int i = 0; i < 16; i += 4) {
-        const int d = dt * 32 + 2 * i + 4 * half;
-        *reinterpret_cast<f32x4 *>(dst + d) = f32x4{dk[dt][i], dk[dt][i + 1], dk[dt][i + 2], dk[dt][i + 3]};
-        *reinterpret_cast<f32x4 *>(dst + AG_ROWS * D + d) =
-            f32x4{dv[dt][i], dv[dt][i + 1], dv[dt][i + 2], dv[dt][i + 3]};
-      }
-  } else if (key < k_len) {
-    store_column<E, D>(dk, a.scale, a.dk.at(t.first + key, kv_head), a.dim);
-    store_column<E, D>(dv, 1.0f, a.dv.at(t.first + key, kv_head), a.dim);
+      for (int dt = 0; dt < D / 32; dt++)
+#pragma unroll
+        for (int i = 0; i < 16; i += 4) {
+          const int d = dt * 32 + 2 * i + 4 * half;
+          const f32x16 &y = dk[x][dt], &z = dv[x][dt];
+          *reinterpret_cast<f32x4 *>(dst + d) = f32x4{y[i], y[i + 1], y[i + 2], y[i + 3]};
+          *reinterpret_cast<f32x4 *>(dst + KEYS * D + d) = f32x4{z[i], z[i + 1], z[i + 2], z[i + 3]};
+        }
+    } else if (key + 32 * x < k_len) {
+      store_column<E, D>(dk[x], a.scale, a.dk.at(t.first + key + 32 * x, kv_head), a.dim);
+      store_column<E, D>(dv[x], 1.0f, a.dv.at(t.first + key + 32 * x, kv_head), a.dim);
+    }
   }
 }
 
 // Adds the parts of the split key tiles: a block an eighth of a tile, four components a thread.
 template <class E, int D> __global__ __launch_bounds__(AG_THREADS) void attention_dkv_join_kernel(GradArgs a) {
+  constexpr int KEYS = KeyTile<D>::KEYS;
   const int kv_head = blockIdx.x % a.kv_heads;
   SegTile t;
-  if (!find_tile(a.k_offsets, a.k_lens, a.k_rows, a.q_offsets, a.q_lens, a.q_rows, a.m, AG_ROWS,
+  if (!find_tile(a.k_offsets, a.k_lens, a.k_rows, a.q_offsets, a.q_lens, a.q_rows, a.m, KEYS,
                  blockIdx.x / a.kv_heads, t))
     return;
-  const int k_len = (int)t.len, q_len = (int)t.len2, key0 = (int)t.tile * AG_ROWS;
+  const int k_len = (int)t.len, q_len = (int)t.len2, key0 = (int)t.tile * KEYS;
   const int parts = parts_of(RowSteps(a.group, q_len, first_token(a, key0, q_len, k_len)).count(), a.parts);
   if (parts == 1) return;
-  constexpr int ROWS = AG_ROWS / 8, FOURS = D / 4;
+  constexpr int ROWS = KEYS / 8, FOURS = D / 4;
   for (int i = threadIdx.x; i < ROWS * FOURS; i += AG_THREADS) {
     const int row = blockIdx.y * ROWS + i / FOURS, d = i % FOURS * 4;
     if (key0 + row >= k_len || d >= a.dim) continue;
@@ -388,7 +417,7 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS) void attentio
     for (int p = 0; p < parts; p++) {
       const float *src = part_sums<D>(a, blockIdx.x, p) + row * D + d;
       dk += *reinterpret_cast<const f32x4 *>(src);
-      dv += *reinterpret_cast<const f32x4 *>(src + AG_ROWS * D);
+      dv += *reinterpret_cast<const f32x4 *>(src + KEYS * D);
     }
     uint32_t x[4], y[4];
 #pragma unroll
@@ -411,7 +440,8 @@ struct GradPlan {
 };
 static GradPlan grad_plan(int64_t q_rows, int64_t k_rows, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t m) {
   GradPlan p;
-  p.tiles = most_tiles(k_rows, m, AG_ROWS) * kv_heads;
+  const int keys = head_dim <= 64 ? KeyTile<64>::KEYS : KeyTile<128>::KEYS;
+  p.tiles = most_tiles(k_rows, m, keys) * kv_heads;
   const int64_t wanted = p.tiles > 0 ? ceil_div(8 * NUM_CUS_HINT, p.tiles) : 1;
   p.parts = (int)(wanted < 8 ? wanted : 8);
   // no tile has more steps than the rows of one head group make
@@ -420,7 +450,7 @@ static GradPlan grad_plan(int64_t q_rows, int64_t k_rows, int64_t heads, int64_t
   if (p.parts > ceil_div(steps, AG_PART_STEPS)) p.parts = (int)ceil_div(steps, AG_PART_STEPS);
   if (p.parts < 1) p.parts = 1;
   p.delta_bytes = (size_t)ceil_div(q_rows * heads, 4) * 16;
-  p.part_bytes = p.parts > 1 ? (size_t)p.tiles * p.parts * 2 * AG_ROWS * (head_dim <= 64 ? 64 : 128) * sizeof(float) : 0;
+  p.part_bytes = p.parts > 1 ? (size_t)p.tiles * p.parts * 2 * keys * (head_dim <= 64 ? 64 : 128) * sizeof(float) : 0;
   return p;
 }
 
