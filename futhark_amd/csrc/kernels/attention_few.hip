@@ -20,84 +20,102 @@
 namespace fa {
 
 constexpr int FEW_KEYS = 32;        // keys of a tile
-constexpr int FEW_LEAST_TILES = 8;  // a piece is at least this long
+// What beginning a unit costs a wave, in tiles: every unit is that much longer
+// on the line, or waves that meet many short sequences end last (64 ragged
+// sequences: the last wave at 121 us with the mean at 86 us).
+constexpr int FEW_START = 2;
+constexpr int FEW_LEAST = 4 + FEW_START;  // a piece is at least this long
 constexpr int FEW_THREADS = 256, FEW_WAVES = FEW_THREADS / WAVE;
 
 // Waves a launch has: what fits the LDS of the chip (four waves of 33 KiB a CU,
 // twice as many for D = 64).
 template <int D> constexpr int few_waves() { return NUM_CUS_HINT * FEW_WAVES * (D == 128 ? 1 : 2); }
+static_assert((NUM_CUS_HINT & (NUM_CUS_HINT - 1)) == 0, "a power of two");
 
 // LDS of a wave: two stages of K and V, four slots of page numbers.
 template <int D> struct FewLds {
   static constexpr int HALF = FEW_KEYS * D * 2, STAGE = 2 * HALF, IDS = 2 * STAGE, BYTES = IDS + 4 * WAVE * 4;
 };
 
-// A sequence as the line of tiles sees it.
+// A sequence as the line sees it: each of its row tiles and key heads is a unit
+// of FEW_START places and one for each of its key tiles.
 struct FewSeq {
-  int64_t first, past;
-  int len, row_tiles, key_tiles;
-  __device__ __forceinline__ int64_t tiles(int kv_heads) const { return (int64_t)row_tiles * key_tiles * kv_heads; }
+  int first, past, len, row_tiles;
+  __device__ __forceinline__ int key_tiles() const { return (int)(((int64_t)past + len + FEW_KEYS - 1) / FEW_KEYS); }
+  __device__ __forceinline__ int unit() const { return key_tiles() + FEW_START; }
+  __device__ __forceinline__ int64_t units(int kv_heads) const { return (int64_t)row_tiles * kv_heads; }
+  __device__ __forceinline__ int64_t places(int kv_heads) const { return units(kv_heads) * unit(); }
 };
 __device__ __forceinline__ FewSeq few_seq(const AttentionArgs &a, int per_tile, int64_t i, bool report) {
-  FewSeq s = {0, 0, 0, 0, 0};
+  FewSeq s = {0, 0, 0, 0};
   int64_t first, len;
-  bool ok = segment_ok(a.q_offsets, a.q_lens, i, a.q_rows, first, len);
   const int64_t past = a.pages.past_lens[i], room = a.pages.capacity();
+  bool ok = segment_ok(a.q_offsets, a.q_lens, i, a.q_rows, first, len);
   ok = ok && (len == 0 || (past >= 0 && past <= room && len <= room - past));
   if (ok) {
-    s.first = first;
-    s.past = past;
+    s.first = (int)first;
+    s.past = len > 0 ? (int)past : 0;
     s.len = (int)len;
-    s.row_tiles = (int)((len + per_tile - 1) / per_tile);
-    s.key_tiles = len > 0 ? (int)((past + len + FEW_KEYS - 1) / FEW_KEYS) : 0;
+    s.row_tiles = (int)(((uint32_t)len + (uint32_t)per_tile - 1) / (uint32_t)per_tile);
   } else if (report && a.failure != nullptr) {
     *a.failure = a.code;
   }
   return s;
 }
 
-// The line's length and the place where a block's threads look for a position:
-// thread t counts sequences t * each .. (t + 1) * each - 1, before[t] tiles precede them.
-struct FewLine {
-  int64_t total, piece, each;
-  int64_t *before;  // [FEW_THREADS] in LDS
+// What a block knows of the line.  Thread t counts the sequences t * each ..
+// (t + 1) * each - 1: before[t] places precede them (units[t] units, which the
+// second kernel asks for).  Up to FEW_THREADS sequences are kept.
+struct FewTable {
+  int64_t before[FEW_THREADS], wave_places[FEW_WAVES], wave_units[FEW_WAVES];
+  FewSeq seq[FEW_THREADS];
 };
-__device__ __forceinline__ FewLine few_line(const AttentionArgs &a, int per_tile, int waves, int64_t *before) {
+struct FewLine {
+  int64_t total, piece, each;  // places in all and of a piece
+  const FewTable *table;
+  __device__ __forceinline__ FewSeq seq(const AttentionArgs &a, int per_tile, int64_t i) const {
+    return each == 1 ? table->seq[i] : few_seq(a, per_tile, i, false);
+  }
+};
+__device__ __forceinline__ FewLine few_line(const AttentionArgs &a, int per_tile, int waves, FewTable &table,
+                                            int64_t *units_before = nullptr) {
   FewLine line;
   line.each = (a.m + FEW_THREADS - 1) / FEW_THREADS;
-  line.before = before;
-  int64_t mine = 0;
-  for (int64_t i = threadIdx.x * line.each; i < (threadIdx.x + 1) * line.each && i < a.m; i++)
-    mine += few_seq(a, per_tile, i, blockIdx.x == 0).tiles(a.kv_heads);
-  const int64_t upto = wave_incl_scan<int64_t, OpAdd<int64_t>>(mine);
-  __shared__ int64_t wave_total[FEW_WAVES];
-  if (lane_id() == WAVE - 1) wave_total[threadIdx.x / WAVE] = upto;
+  line.table = &table;
+  int64_t places = 0, units = 0;
+  for (int64_t i = threadIdx.x * line.each; i < (threadIdx.x + 1) * line.each && i < a.m; i++) {
+    const FewSeq s = few_seq(a, per_tile, i, blockIdx.x == 0);
+    places += s.places(a.kv_heads);
+    units += s.units(a.kv_heads);
+    table.seq[threadIdx.x] = s;
+  }
+  const int64_t places_upto = wave_incl_scan<int64_t, OpAdd<int64_t>>(places);
+  const int64_t units_upto = units_before == nullptr ? 0 : wave_incl_scan<int64_t, OpAdd<int64_t>>(units);
+  const int wave = threadIdx.x / WAVE;
+  if (lane_id() == WAVE - 1) table.wave_places[wave] = places_upto, table.wave_units[wave] = units_upto;
   __syncthreads();
-  int64_t base = 0;
+  int64_t places_base = 0, units_base = 0;
   line.total = 0;
   for (int w = 0; w < FEW_WAVES; w++) {
-    if (w < (int)(threadIdx.x / WAVE)) base += wave_total[w];
-    line.total += wave_total[w];
+    if (w < wave) places_base += table.wave_places[w], units_base += table.wave_units[w];
+    line.total += table.wave_places[w];
   }
-  before[threadIdx.x] = base + upto - mine;
+  table.before[threadIdx.x] = places_base + places_upto - places;
+  if (units_before != nullptr) units_before[threadIdx.x] = units_base + units_upto - units;
   __syncthreads();
-  const int64_t even = (line.total + waves - 1) / waves;
-  line.piece = even < FEW_LEAST_TILES ? FEW_LEAST_TILES : even;
+  const int64_t even = (line.total + waves - 1) >> __builtin_ctz(waves);  // a power of two
+  line.piece = even < FEW_LEAST ? FEW_LEAST : even;
   return line;
 }
-// The sequence that holds position `at` < total, and how many tiles precede it;
-// the same for the whole wave.
-__device__ __forceinline__ int64_t few_find(const AttentionArgs &a, int per_tile, const FewLine &line, int64_t at,
-                                            int64_t &precede) {
+// x / y where the quotient fits 32 bits; mostly both do.
+__device__ __forceinline__ uint32_t few_divide(int64_t x, int64_t y) {
+  return ((x | y) >> 32) == 0 ? (uint32_t)x / (uint32_t)y : (uint32_t)(x / y);
+}
+// The thread that counted place `at` of the line; the same for the whole wave.
+__device__ __forceinline__ int few_thread(const int64_t *starts, int64_t at) {
   int thread = -1;
-  for (int b = 0; b < FEW_THREADS; b += WAVE) thread += __popcll(__ballot(line.before[b + lane_id()] <= at));
-  int64_t i = thread * line.each;
-  precede = line.before[thread];
-  for (;; i++) {
-    const int64_t tiles = few_seq(a, per_tile, i, false).tiles(a.kv_heads);
-    if (at < precede + tiles || i + 1 >= a.m) return i;
-    precede += tiles;
-  }
+  for (int b = 0; b < FEW_THREADS; b += WAVE) thread += __popcll(__ballot(starts[b + lane_id()] <= at));
+  return thread;
 }
 
 // Where a wave leaves the part of the unit its piece begins in (slot 0) or ends
@@ -118,16 +136,19 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 ? 1 : 2) void attention_few_k
   constexpr int LOADS = L::HALF / (WAVE * 16);  // loads a lane and operand
   constexpr int LOAD_ROWS = FEW_KEYS / LOADS;
   extern __shared__ __align__(16) unsigned char lds[];
-  __shared__ int64_t before[FEW_THREADS];
+  __shared__ FewTable seqs;
   const int per_tile = ROWS / a.group;
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   const int quarter = lane >> 4, col = lane & 15;
-  const FewLine line = few_line(a, per_tile, gridDim.x * FEW_WAVES, before);
+  const FewLine line = few_line(a, per_tile, gridDim.x * FEW_WAVES, seqs);
   const int64_t number = (int64_t)blockIdx.x * FEW_WAVES + wave;
   int64_t at = number * line.piece;
   const int64_t end = at + line.piece < line.total ? at + line.piece : line.total;
   if (at >= end) return;
-  int64_t precede, seq = few_find(a, per_tile, line, at, precede);
+  // The sequence the piece begins in (the loop below walks on to it) and the
+  // tiles before that.
+  int64_t seq = few_thread(seqs.before, at), precede = seqs.before[seq];
+  seq *= line.each;
 
   unsigned char *mine = lds + wave * L::BYTES;
   const uint32_t lds_base = lds_address(mine);
@@ -135,6 +156,13 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 ? 1 : 2) void attention_few_k
   const int load_row = lane / (D / 8), load_slot = lane % (D / 8);
   const int64_t row_bytes = a.dim * 2, head_bytes = row_bytes << a.pages.page_shift;
   const int slot_mask = (1 << a.pages.page_shift) - 1;
+  // The usual case: whole rows, and pages of at least the rows a load covers.
+  // lane_at: this lane's place among them (the swizzle repeats every 16 rows).
+  const bool plain = a.dim == D && (LOAD_ROWS - 1 & ~slot_mask) == 0;
+  uint32_t lane_at[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++)
+    lane_at[i] = load_row * (D * 2) + (load_slot ^ tile_swizzle<D>(load_row + i * LOAD_ROWS)) * 16;
 
   // Operand places inside a tile.  Row m of a product's 16 keys is key
   // 4 s(m / 4) + m % 4 of them, s = 0 2 1 3: with that order the rows that two
@@ -153,53 +181,27 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 ? 1 : 2) void attention_few_k
     }
 
   while (at < end) {
-    const FewSeq s = few_seq(a, per_tile, seq, false);
-    const int64_t tiles = s.tiles(a.kv_heads);
-    if (at >= precede + tiles) {
-      precede += tiles;
+    const FewSeq s = line.seq(a, per_tile, seq);
+    const int64_t places = s.places(a.kv_heads);
+    if (at >= precede + places) {
+      precede += places;
       seq++;
       continue;
     }
-    // Position in the sequence: row tile, head, key tile.
-    const int64_t inside = at - precede, unit = inside / s.key_tiles;
-    const int from = (int)(inside - unit * s.key_tiles);
-    const int to = end - at < s.key_tiles - from ? (int)(from + (end - at)) : s.key_tiles;
-    at += to - from;
-    const int head = (int)(unit % a.kv_heads), t0 = (int)(unit / a.kv_heads) * per_tile;
+    // Place in the sequence: row tile, head, key tile.
+    const int64_t inside = at - precede;
+    const uint32_t unit = few_divide(inside, s.unit());
+    const int place = (int)(inside - (int64_t)unit * s.unit());
+    const int next = end - at < s.unit() - place ? (int)(place + (end - at)) : s.unit();
+    at += next - place;
+    const int key_tiles = s.key_tiles();
+    const int from = place > FEW_START ? place - FEW_START : 0, to = next - FEW_START;
+    if (from >= to) continue;
+    const int head = (int)(unit % (uint32_t)a.kv_heads), t0 = (int)(unit / (uint32_t)a.kv_heads) * per_tile;
     const int tokens = s.len - t0 < per_tile ? s.len - t0 : per_tile, rows = tokens * a.group;
-    const int first_limit = (int)s.past + t0;         // last key the first token sees
+    const int first_limit = s.past + t0;              // last key the first token sees
     const int keys = first_limit + tokens;            // keys the last one sees
     const int64_t table = seq * a.pages.cols;
-
-    uint4 q[CT][D / 32];
-    int limit[CT];
-#pragma unroll
-    for (int ct = 0; ct < CT; ct++) {
-      const int row = ct * 16 + col < rows ? ct * 16 + col : rows - 1;
-      limit[ct] = first_limit + row / a.group;
-      const uint16_t *src = a.q.at(s.first + t0 + row / a.group, head * a.group + row % a.group);
-#pragma unroll
-      for (int k = 0; k < D / 32; k++) {
-        const int c = 32 * k + 8 * quarter;
-        q[ct][k] = c < a.dim ? *reinterpret_cast<const uint4 *>(src + c) : uint4{0, 0, 0, 0};
-      }
-    }
-    // The queries are here before the loop: inside it the compiler would wait for
-    // them, and with them for the tiles in flight, in every round.
-#pragma unroll
-    for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-      for (int k = 0; k < D / 32; k++)
-        asm volatile("" : "+v"(q[ct][k].x), "+v"(q[ct][k].y), "+v"(q[ct][k].z), "+v"(q[ct][k].w));
-    f32x4 o[CT][D / 16];
-    float top[CT], sum[CT];
-#pragma unroll
-    for (int ct = 0; ct < CT; ct++) {
-      top[ct] = -INFINITY;
-      sum[ct] = 0.0f;
-#pragma unroll
-      for (int dt = 0; dt < D / 16; dt++) o[ct][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
 
     // Page numbers of the keys of tile t (and of the next 32, not used).
     const auto fetch_ids = [&](int t) __attribute__((always_inline)) {
@@ -210,33 +212,71 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 ? 1 : 2) void attention_few_k
                    "v"(src)
                    : "memory", "m0");
     };
+    fetch_ids(from);
+    fetch_ids(from + 1);
+    uint4 q[CT][D / 32];
+    int limit[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+      const int row = ct * 16 + col < rows ? ct * 16 + col : rows - 1;
+      limit[ct] = first_limit + row / a.group;
+      const uint16_t *src = a.q.at((int64_t)s.first + t0 + row / a.group, head * a.group + row % a.group);
+#pragma unroll
+      for (int k = 0; k < D / 32; k++) {
+        const int c = 32 * k + 8 * quarter;
+        q[ct][k] = c < a.dim ? *reinterpret_cast<const uint4 *>(src + c) : uint4{0, 0, 0, 0};
+      }
+    }
+    f32x4 o[CT][D / 16];
+    float top[CT], sum[CT];
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+      top[ct] = -INFINITY;
+      sum[ct] = 0.0f;
+#pragma unroll
+      for (int dt = 0; dt < D / 16; dt++) o[ct][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
     const auto fetch = [&](int t) __attribute__((always_inline)) {
       const uint32_t dst = lds_base + (t & 1) * L::STAGE;
-      bool bad = false;
+      const int key0 = t * FEW_KEYS, id = ids[(t & 3) * WAVE + (lane & (FEW_KEYS - 1))];
+      const bool there = key0 + (lane & (FEW_KEYS - 1)) < keys && t < to;
+      const bool named = id >= 0 && id < a.pages.n_pages;
+      if (plain && __all(there && named)) {
+        // A load's rows lie in one page: its base is the same for all lanes.
+#pragma unroll
+        for (int i = 0; i < LOADS; i++) {
+          const int64_t off = ((int64_t)__builtin_amdgcn_readlane(id, i * LOAD_ROWS) * a.kv_heads + head) * head_bytes +
+                              ((key0 + i * LOAD_ROWS) & slot_mask) * row_bytes;
+          load_to_lds(a.pages.k, off, lane_at[i % 4], dst + i * (WAVE * 16));
+          load_to_lds(a.pages.v, off, lane_at[i % 4], dst + L::HALF + i * (WAVE * 16));
+        }
+        return;
+      }
+      if (there && !named && a.failure != nullptr) *a.failure = a.code;
 #pragma unroll
       for (int i = 0; i < LOADS; i++) {
-        const int r = load_row + i * LOAD_ROWS, key = t * FEW_KEYS + r;
-        const int unit8 = load_slot ^ tile_swizzle<D>(r);
-        const int id = ids[(t & 3) * WAVE + r];
-        const bool named = id >= 0 && id < a.pages.n_pages, there = key < keys && t < to;
-        bad = bad || (there && !named);
-        const int64_t off = ((int64_t)id * a.kv_heads + head) * head_bytes + (key & slot_mask) * row_bytes + unit8 * 16;
-        const bool live = there && named && unit8 * 8 < a.dim;
-        const void *ks = live ? (const void *)((const char *)a.pages.k + off) : (const void *)&g_zeros;
-        const void *vs = live ? (const void *)((const char *)a.pages.v + off) : (const void *)&g_zeros;
-        load_to_lds(ks, dst + i * (WAVE * 16));
-        load_to_lds(vs, dst + L::HALF + i * (WAVE * 16));
+        const int r = load_row + i * LOAD_ROWS, unit8 = load_slot ^ tile_swizzle<D>(r);
+        const int page = __shfl(id, r);
+        const int64_t off = ((int64_t)page * a.kv_heads + head) * head_bytes + ((key0 + r) & slot_mask) * row_bytes + unit8 * 16;
+        const bool live = key0 + r < keys && t < to && page >= 0 && page < a.pages.n_pages && unit8 * 8 < a.dim;
+        load_to_lds(live ? (const void *)((const char *)a.pages.k + off) : (const void *)&g_zeros, dst + i * (WAVE * 16));
+        load_to_lds(live ? (const void *)((const char *)a.pages.v + off) : (const void *)&g_zeros,
+                    dst + L::HALF + i * (WAVE * 16));
       }
-      if (bad && a.failure != nullptr) *a.failure = a.code;
     };
 
     // In flight while tile t is multiplied: the page numbers of t + 2 (older),
     // then the 2 LOADS loads of tile t + 1.
-    fetch_ids(from);
+    // The queries have arrived before the loop: inside it the compiler would wait for
+    // them, and with them for the tiles in flight, in every round.
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+      for (int k = 0; k < D / 32; k++)
+        asm volatile("" : "+v"(q[ct][k].x), "+v"(q[ct][k].y), "+v"(q[ct][k].z), "+v"(q[ct][k].w));
     wait_loads();
-    fetch_ids(from + 1);
     fetch(from);
-    wait_older_than<2 * LOADS>();
     fetch_ids(from + 2);
     fetch(from + 1);
     for (int t = from; t < to; t++) {
@@ -339,7 +379,7 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 ? 1 : 2) void attention_few_k
     }
     wait_loads();
 
-    const bool whole = from == 0 && to == s.key_tiles;
+    const bool whole = from == 0 && to == key_tiles;
     const int64_t part = few_slot(number, from == 0 ? 1 : 0, ROWS);
 #pragma unroll
     for (int ct = 0; ct < CT; ct++) {
@@ -356,7 +396,7 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 ? 1 : 2) void attention_few_k
         }
         continue;
       }
-      const int64_t out_row = s.first + t0 + row / a.group;
+      const int64_t out_row = (int64_t)s.first + t0 + row / a.group;
       const int q_head = head * a.group + row % a.group;
       const bool empty = top[ct] == -INFINITY;  // only scores of -inf
       const float inverse = empty ? 0.0f : 1.0f / all;
@@ -375,58 +415,103 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 ? 1 : 2) void attention_few_k
   }
 }
 
-// Joins the parts: a block a unit, a wave a query row.
-template <class E, int D, int ROWS> __global__ __launch_bounds__(FEW_THREADS) void attention_few_join_kernel(AttentionArgs a, int waves) {
-  __shared__ int64_t before[FEW_THREADS];
-  const int per_tile = ROWS / a.group, lane = lane_id();
-  const FewLine line = few_line(a, per_tile, waves, before);
-  // Units in the order of the line: a sequence's row tiles, heads inside them.
-  SegTile t;
-  if (!find_tile(a.q_offsets, a.q_lens, a.q_rows, nullptr, nullptr, 0, a.m, per_tile, blockIdx.x / a.kv_heads, t)) return;
-  const FewSeq s = few_seq(a, per_tile, t.seg, false);
-  if (s.key_tiles == 0) return;
-  const int head = blockIdx.x % a.kv_heads;
-  int64_t precede = line.before[t.seg / line.each];
-  for (int64_t i = t.seg / line.each * line.each; i < t.seg; i++) precede += few_seq(a, per_tile, i, false).tiles(a.kv_heads);
-  const int64_t begin = precede + (t.tile * a.kv_heads + head) * s.key_tiles;
-  const int64_t w0 = begin / line.piece, w1 = (begin + s.key_tiles - 1) / line.piece;
-  if (w0 == w1) return;  // one wave had it all
-  const int t0 = (int)t.tile * per_tile, tokens = s.len - t0 < per_tile ? s.len - t0 : per_tile;
-  for (int row = threadIdx.x / WAVE; row < tokens * a.group; row += FEW_WAVES) {
-    const auto part = [&](int64_t w) { return few_slot(w, w * line.piece <= begin ? 1 : 0, ROWS) + row; };
-    float top = -INFINITY;
-    for (int64_t w = w0 + lane; w <= w1; w += WAVE) top = fmaxf(top, a.part_ml[2 * part(w)]);
-    for (int step = 1; step < WAVE; step *= 2) top = fmaxf(top, __shfl_xor(top, step));
-    float sum = 0.0f, o[D / WAVE] = {};
-    if (top != -INFINITY) {
-      for (int64_t base = w0; base <= w1; base += WAVE) {
-        const int64_t w = base + lane;
-        float f = 0.0f;
-        if (w <= w1) {
-          f = exp2f(a.part_ml[2 * part(w)] - top);
-          sum += f * a.part_ml[2 * part(w) + 1];
-        }
-        const int count = w1 - base + 1 < WAVE ? (int)(w1 - base + 1) : WAVE;
-#pragma unroll 8
-        for (int j = 0; j < count; j++) {
-          const float g = read_lane(f, j);
-          const float *src = a.part_o + part(base + j) * D + lane;
-#pragma unroll
-          for (int c = 0; c < D / WAVE; c++) o[c] += g * src[c * WAVE];
-        }
-      }
-      for (int step = 1; step < WAVE; step *= 2) sum += __shfl_xor(sum, step);
-    }
-    const int64_t out_row = s.first + t0 + row / a.group;
-    const int q_head = head * a.group + row % a.group;
-#pragma unroll
-    for (int c = 0; c < D / WAVE; c++) {
-      const int d = c * WAVE + lane;
-      if (d < a.dim) a.out.at(out_row, q_head)[d] = E::store(top == -INFINITY ? 0.0f : o[c] / sum);
-    }
-    if (a.lse != nullptr && lane == 0)
-      a.lse[out_row * a.heads + q_head] = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * LN2;
+// Joins the parts: a block a unit and join_rows of its rows.  A thread takes
+// four components of a row; where there are fewer rows several threads share the
+// parts of one.  Parts are taken in order, WAVE at a time, with the running
+// maximum and sum.
+template <class E, int D, int ROWS>
+__global__ __launch_bounds__(FEW_THREADS) void attention_few_join_kernel(AttentionArgs a, int waves, int join_rows) {
+  constexpr int FOURS = D / 4, JOIN_ROWS = FEW_THREADS / FOURS, BATCH = 8;
+  __shared__ FewTable seqs;
+  __shared__ int64_t units_before[FEW_THREADS];
+  __shared__ float tops[JOIN_ROWS], sums[JOIN_ROWS], factors[JOIN_ROWS], weights[JOIN_ROWS][WAVE];
+  __shared__ f32x4 shared[FEW_THREADS];
+  const int per_tile = ROWS / a.group;
+  const FewLine line = few_line(a, per_tile, waves, seqs, units_before);
+  // The unit of this number, in the order of the line: the row tiles of a
+  // sequence, heads inside them.
+  const int thread = few_thread(units_before, blockIdx.x);
+  int64_t number = blockIdx.x - units_before[thread], precede = seqs.before[thread];
+  FewSeq s;
+  for (int64_t i = thread * line.each;; i++) {
+    if (i >= (thread + 1) * line.each || i >= a.m) return;
+    s = line.seq(a, per_tile, i);
+    const int64_t units = s.units(a.kv_heads);
+    if (number < units) break;
+    number -= units;
+    precede += s.places(a.kv_heads);
   }
+  const int head = (int)(number % a.kv_heads), t0 = (int)(number / a.kv_heads) * per_tile;
+  // Its first and last tile, and the waves that had them.
+  const int64_t begin = precede + number * s.unit() + FEW_START, last = begin + s.key_tiles() - 1;
+  const int64_t w0 = few_divide(begin, line.piece), w1 = few_divide(last, line.piece);
+  const int row0 = blockIdx.y * join_rows;
+  int rows = (s.len - t0 < per_tile ? s.len - t0 : per_tile) * a.group - row0;
+  if (w0 == w1 || rows <= 0) return;  // one wave had it all
+  if (rows > join_rows) rows = join_rows;
+  const auto part = [&](int64_t w) { return few_slot(w, w * line.piece <= begin ? 1 : 0, ROWS) + row0; };
+  if (threadIdx.x < JOIN_ROWS) tops[threadIdx.x] = -INFINITY, sums[threadIdx.x] = 0.0f;
+  int share = 1;  // threads that share the parts of one place
+  while (2 * share * rows * FOURS <= FEW_THREADS) share *= 2;
+  const int row = threadIdx.x / share / FOURS, four = threadIdx.x % (share * FOURS) / share, turn = threadIdx.x % share;
+  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int64_t base = w0; base <= w1; base += WAVE) {
+    const int count = w1 - base + 1 < WAVE ? (int)(w1 - base + 1) : WAVE;
+    int group = 1;  // lanes for the parts of a row
+    while (group < count) group *= 2;
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * group; i += FEW_THREADS) {
+      const int r = i / group, j = i % group;
+      const float *ml = a.part_ml + 2 * (part(base + (j < count ? j : 0)) + r);
+      float top = j < count ? ml[0] : -INFINITY, sum = ml[1];
+      float f = top;
+      for (int step = 1; step < group; step *= 2) top = fmaxf(top, __shfl_xor(top, step));
+      top = fmaxf(top, tops[r]);
+      f = top == -INFINITY ? 0.0f : exp2f(f - top);
+      weights[r][j] = f;
+      sum *= f;
+      for (int step = 1; step < group; step *= 2) sum += __shfl_xor(sum, step);
+      if (j == 0) {
+        factors[r] = top == -INFINITY ? 1.0f : exp2f(tops[r] - top);
+        sums[r] = sums[r] * factors[r] + sum;
+        tops[r] = top;
+      }
+    }
+    __syncthreads();
+    if (row >= rows) continue;
+    o *= factors[row];
+    for (int j0 = turn; j0 < count; j0 += BATCH * share) {
+      f32x4 x[BATCH];
+#pragma unroll
+      for (int i = 0; i < BATCH; i++) {
+        const int j = j0 + i * share;
+        x[i] = *reinterpret_cast<const f32x4 *>(a.part_o + (part(base + (j < count ? j : turn)) + row) * D + 4 * four);
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; i++) {
+        const int j = j0 + i * share;
+        if (j < count) o += weights[row][j] * x[i];
+      }
+    }
+  }
+  for (int step = share / 2; step > 0; step /= 2) {
+    __syncthreads();
+    shared[threadIdx.x] = o;
+    __syncthreads();
+    if (turn < step) o += shared[threadIdx.x + step];
+  }
+  if (row >= rows || turn != 0) return;
+  const bool empty = tops[row] == -INFINITY;
+  const float inverse = empty ? 0.0f : 1.0f / sums[row];
+  const int64_t out_row = (int64_t)s.first + t0 + (row0 + row) / a.group;
+  const int q_head = head * a.group + (row0 + row) % a.group;
+  uint32_t x[4];
+#pragma unroll
+  for (int i = 0; i < 4; i++) x[i] = E::store(empty ? 0.0f : o[i] * inverse);
+  if (4 * four < a.dim)
+    *reinterpret_cast<uint2 *>(a.out.at(out_row, q_head) + 4 * four) = uint2{x[0] | x[1] << 16, x[2] | x[3] << 16};
+  if (a.lse != nullptr && four == 0)
+    a.lse[out_row * a.heads + q_head] = empty ? -INFINITY : (tops[row] + log2f(sums[row])) * LN2;
 }
 
 int few_rows(int64_t n, int64_t heads, int64_t kv_heads, int64_t m) {
@@ -455,7 +540,13 @@ static int launch_few_of(hipStream_t stream, AttentionArgs a, void *workspace) {
   kernel<<<dim3(few_waves<D>() / FEW_WAVES), FEW_THREADS, LDS, stream>>>(a);
   const int rc = launch_status();
   if (rc != 0) return rc;
-  attention_few_join_kernel<E, D, ROWS><<<dim3((unsigned)units), FEW_THREADS, 0, stream>>>(a, few_waves<D>());
+  // Rows a block of the second kernel joins: as many as its threads hold, fewer
+  // while there are blocks to spare.
+  const int64_t rows = ROWS / a.group * a.group;  // of a unit, at most
+  int join_rows = FEW_THREADS / (D / 4);
+  while (join_rows > 1 && units * ceil_div(rows, join_rows) < NUM_CUS_HINT) join_rows /= 2;
+  const dim3 grid((unsigned)units, (unsigned)ceil_div(rows, join_rows));
+  attention_few_join_kernel<E, D, ROWS><<<grid, FEW_THREADS, 0, stream>>>(a, few_waves<D>(), join_rows);
   return launch_status();
 }
 
