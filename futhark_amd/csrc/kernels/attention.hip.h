@@ -87,6 +87,7 @@ struct AttentionArgs {
   Pages pages;
   int chunk, splits;
   float *part_o, *part_ml;
+  int64_t most_units;
 };
 
 // A wave rescales its output only when a maximum has grown by 2^8 since it last
@@ -97,7 +98,7 @@ constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
 // attention_few.hip: attention over the cache for few query rows a sequence.
 // Rows a unit of work holds for such a call, or 0 if the other kernel should take it.
 int few_rows(int64_t n, int64_t heads, int64_t kv_heads, int64_t m);
-size_t few_workspace(int rows, int64_t head_dim);
+size_t few_workspace(int rows, int64_t n, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t m);
 int launch_few(hipStream_t stream, fa_dtype t, int rows, const AttentionArgs &a, void *workspace);
 
 // ------------------------------------------------------------------ segments

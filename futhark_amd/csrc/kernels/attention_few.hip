@@ -20,11 +20,16 @@
 namespace fa {
 
 constexpr int FEW_KEYS = 32;        // keys of a tile
-// What beginning a unit costs a wave, in tiles: every unit is that much longer
-// on the line, or waves that meet many short sequences end last (64 ragged
+// What beginning a unit costs a wave, in tiles: on a long line every unit is that
+// much longer, or waves that meet many short sequences end last (64 ragged
 // sequences: the last wave at 121 us with the mean at 86 us).
 constexpr int FEW_START = 2;
-constexpr int FEW_LEAST = 4 + FEW_START;  // a piece is at least this long
+// On a short line, where a wave need not begin more than one unit, pieces end
+// with their units and have at least FEW_LEAST tiles.  Short: up to FEW_SHORT of them.
+constexpr int FEW_LEAST = 2, FEW_SHORT = 16;
+// Tables of up to this many keys are attended in one launch, if the units fit the
+// chip at once.
+constexpr int FEW_SHORT_KEYS = 1024;
 constexpr int FEW_THREADS = 256, FEW_WAVES = FEW_THREADS / WAVE;
 
 // Waves a launch has: what fits the LDS of the chip (four waves of 33 KiB a CU,
@@ -37,14 +42,11 @@ template <int D> struct FewLds {
   static constexpr int HALF = FEW_KEYS * D * 2, STAGE = 2 * HALF, IDS = 2 * STAGE, BYTES = IDS + 4 * WAVE * 4;
 };
 
-// A sequence as the line sees it: each of its row tiles and key heads is a unit
-// of FEW_START places and one for each of its key tiles.
+// A sequence: each of its row tiles and key heads is a unit of key_tiles() tiles.
 struct FewSeq {
   int first, past, len, row_tiles;
   __device__ __forceinline__ int key_tiles() const { return (int)(((int64_t)past + len + FEW_KEYS - 1) / FEW_KEYS); }
-  __device__ __forceinline__ int unit() const { return key_tiles() + FEW_START; }
   __device__ __forceinline__ int64_t units(int kv_heads) const { return (int64_t)row_tiles * kv_heads; }
-  __device__ __forceinline__ int64_t places(int kv_heads) const { return units(kv_heads) * unit(); }
 };
 __device__ __forceinline__ FewSeq few_seq(const AttentionArgs &a, int per_tile, int64_t i, bool report) {
   FewSeq s = {0, 0, 0, 0};
@@ -64,63 +66,118 @@ __device__ __forceinline__ FewSeq few_seq(const AttentionArgs &a, int per_tile, 
 }
 
 // What a block knows of the line.  Thread t counts the sequences t * each ..
-// (t + 1) * each - 1: before[t] places precede them (units[t] units, which the
-// second kernel asks for).  Up to FEW_THREADS sequences are kept.
+// (t + 1) * each - 1.  Up to FEW_THREADS sequences are kept.
 struct FewTable {
-  int64_t before[FEW_THREADS], wave_places[FEW_WAVES], wave_units[FEW_WAVES];
+  int64_t tiles[FEW_WAVES], units[FEW_WAVES], places[FEW_WAVES];  // a wave's threads count
+  // Where the pieces of the block's waves begin: the thread that counts the
+  // place, and the places and units before those it counts.
+  int thread[FEW_WAVES];
+  int64_t before[FEW_WAVES], units_before[FEW_WAVES];
   FewSeq seq[FEW_THREADS];
 };
 struct FewLine {
-  int64_t total, piece, each;  // places in all and of a piece
+  int64_t each;
+  int64_t total, piece;  // places in all and of a wave
+  int64_t units;         // units in all
+  int start;             // places of a unit before its tiles
+  bool is_short;
   const FewTable *table;
   __device__ __forceinline__ FewSeq seq(const AttentionArgs &a, int per_tile, int64_t i) const {
     return each == 1 ? table->seq[i] : few_seq(a, per_tile, i, false);
   }
+  // Places of a unit; a short line pads it to whole pieces.
+  __device__ __forceinline__ int unit(const FewSeq &s) const {
+    const int tiles = s.key_tiles();
+    return is_short ? (int)(((uint32_t)tiles + (uint32_t)piece - 1) / (uint32_t)piece * (uint32_t)piece) : tiles + start;
+  }
 };
-__device__ __forceinline__ FewLine few_line(const AttentionArgs &a, int per_tile, int waves, FewTable &table,
-                                            int64_t *units_before = nullptr) {
+__device__ __forceinline__ int64_t few_sum(const int64_t (&x)[FEW_WAVES], int to) {
+  int64_t sum = 0;
+#pragma unroll
+  for (int w = 0; w < FEW_WAVES; w++) sum += w < to ? x[w] : 0;
+  return sum;
+}
+// Lays out the line, and finds for each wave of the block the thread that counts
+// the place where the wave's piece begins, with the places and units before that.
+__device__ __forceinline__ FewLine few_line(const AttentionArgs &a, int per_tile, FewTable &table) {
+  const int waves = gridDim.x * FEW_WAVES;
   FewLine line;
   line.each = (a.m + FEW_THREADS - 1) / FEW_THREADS;
   line.table = &table;
-  int64_t places = 0, units = 0;
-  for (int64_t i = threadIdx.x * line.each; i < (threadIdx.x + 1) * line.each && i < a.m; i++) {
-    const FewSeq s = few_seq(a, per_tile, i, blockIdx.x == 0);
-    places += s.places(a.kv_heads);
+  const int64_t i0 = threadIdx.x * line.each, i1 = i0 + line.each < a.m ? i0 + line.each : a.m;
+  const int wave = threadIdx.x / WAVE;
+  FewSeq s = {0, 0, 0, 0};
+  int64_t tiles = 0, units = 0;
+  for (int64_t i = i0; i < i1; i++) {
+    s = few_seq(a, per_tile, i, blockIdx.x == 0);
     units += s.units(a.kv_heads);
-    table.seq[threadIdx.x] = s;
+    tiles += s.units(a.kv_heads) * s.key_tiles();
+  }
+  table.seq[threadIdx.x] = s;
+  const int64_t units_upto = wave_incl_scan<int64_t, OpAdd<int64_t>>(units);
+  const int64_t tiles_upto = wave_incl_scan<int64_t, OpAdd<int64_t>>(tiles);
+  if (lane_id() == WAVE - 1) table.tiles[wave] = tiles_upto, table.units[wave] = units_upto;
+  __syncthreads();
+  const int64_t all_units = few_sum(table.units, FEW_WAVES), all_tiles = few_sum(table.tiles, FEW_WAVES);
+  // Pieces of this many tiles are at most as many as there are waves: every unit
+  // has at most one that is not full.
+  line.units = all_units;
+  const int64_t spare = waves - all_units;
+  line.is_short = spare > 0 && all_tiles <= spare * FEW_SHORT;
+  int64_t places = tiles + units * FEW_START;
+  line.start = FEW_START;
+  if (line.is_short) {
+    const uint32_t even = ((uint32_t)all_tiles + (uint32_t)spare - 1) / (uint32_t)spare;
+    line.piece = even < FEW_LEAST ? FEW_LEAST : even;
+    line.start = 0;
+    places = 0;
+    for (int64_t i = i0; i < i1; i++) {
+      if (line.each > 1) s = few_seq(a, per_tile, i, false);
+      places += s.units(a.kv_heads) * line.unit(s);
+    }
   }
   const int64_t places_upto = wave_incl_scan<int64_t, OpAdd<int64_t>>(places);
-  const int64_t units_upto = units_before == nullptr ? 0 : wave_incl_scan<int64_t, OpAdd<int64_t>>(units);
-  const int wave = threadIdx.x / WAVE;
-  if (lane_id() == WAVE - 1) table.wave_places[wave] = places_upto, table.wave_units[wave] = units_upto;
+  if (lane_id() == WAVE - 1) table.places[wave] = places_upto;
   __syncthreads();
-  int64_t places_base = 0, units_base = 0;
-  line.total = 0;
+  line.total = few_sum(table.places, FEW_WAVES);
+  if (!line.is_short) line.piece = (line.total + waves - 1) >> __builtin_ctz(waves);  // a power of two
+  const int64_t before = few_sum(table.places, wave) + places_upto - places;
+  const int64_t units_here = few_sum(table.units, wave) + units_upto - units;
+#pragma unroll
   for (int w = 0; w < FEW_WAVES; w++) {
-    if (w < wave) places_base += table.wave_places[w], units_base += table.wave_units[w];
-    line.total += table.wave_places[w];
+    const int64_t at = ((int64_t)blockIdx.x * FEW_WAVES + w) * line.piece;
+    if (at >= before && at < before + places) {
+      table.thread[w] = threadIdx.x;
+      table.before[w] = before;
+      table.units_before[w] = units_here;
+    }
   }
-  table.before[threadIdx.x] = places_base + places_upto - places;
-  if (units_before != nullptr) units_before[threadIdx.x] = units_base + units_upto - units;
   __syncthreads();
-  const int64_t even = (line.total + waves - 1) >> __builtin_ctz(waves);  // a power of two
-  line.piece = even < FEW_LEAST ? FEW_LEAST : even;
   return line;
 }
+
 // x / y where the quotient fits 32 bits; mostly both do.
 __device__ __forceinline__ uint32_t few_divide(int64_t x, int64_t y) {
   return ((x | y) >> 32) == 0 ? (uint32_t)x / (uint32_t)y : (uint32_t)(x / y);
 }
-// The thread that counted place `at` of the line; the same for the whole wave.
-__device__ __forceinline__ int few_thread(const int64_t *starts, int64_t at) {
-  int thread = -1;
-  for (int b = 0; b < FEW_THREADS; b += WAVE) thread += __popcll(__ballot(starts[b + lane_id()] <= at));
-  return thread;
+// The workspace: where a wave leaves the part of the unit its piece begins in
+// (slot 0) or ends in (slot 1), [rows][D] sums and [rows][2] maximum and sum; then
+// the number of units, and of each what the second kernel needs to join it.
+struct FewUnit {
+  int64_t row;  // of its first token
+  int w0, w1;   // the first and last wave that had a part (w0 == w1: nothing to join)
+  int rows, head, unused[2];
+};
+__host__ __device__ constexpr int64_t few_part_floats(int waves, int rows, int d) {
+  return (int64_t)2 * waves * rows * (d + 2);
 }
-
-// Where a wave leaves the part of the unit its piece begins in (slot 0) or ends
-// in (slot 1): [rows][D] sums and [rows][2] maximum and sum.
 __device__ __forceinline__ int64_t few_slot(int64_t wave, int slot, int rows) { return (2 * wave + slot) * rows; }
+__device__ __forceinline__ int64_t *few_units(const AttentionArgs &a, int rows, int d) {
+  return (int64_t *)(a.part_o + few_part_floats(d == 128 ? few_waves<128>() : few_waves<64>(), rows, d));
+}
+__device__ __forceinline__ FewUnit *few_unit(const AttentionArgs &a, int rows, int d) {
+  return (FewUnit *)(few_units(a, rows, d) + 2);
+}
 
 template <int N> __device__ __forceinline__ void wait_older_than() {
   // all but the N youngest loads have arrived
@@ -129,28 +186,42 @@ template <int N> __device__ __forceinline__ void wait_older_than() {
   static_assert(N == 16 || N == 8, "loads of a tile");
 }
 
+// A wave's work on a unit: tiles from .. to - 1 of a sequence's keys for some of
+// its tokens and one key head.
+struct FewRun {
+  int64_t seq, row;  // the row of the first token
+  int head, tokens, rows;
+  int first_limit, keys;  // last key the first token sees, keys the last one sees
+  int from, to;
+  __device__ __forceinline__ FewRun(const AttentionArgs &a, int per_tile, const FewSeq &s, int64_t seq, uint32_t unit,
+                                    int from, int to)
+      : seq(seq), from(from), to(to) {
+    head = (int)(unit % (uint32_t)a.kv_heads);
+    const int t0 = (int)(unit / (uint32_t)a.kv_heads) * per_tile;
+    row = (int64_t)s.first + t0;
+    tokens = s.len - t0 < per_tile ? s.len - t0 : per_tile;
+    rows = tokens * a.group;
+    first_limit = s.past + t0;
+    keys = first_limit + tokens;
+  }
+};
+// What comes of it, by query rows (columns) ct * 16 + lane % 16: components
+// dt * 16 + 4 (lane / 16) + i of the sums, maxima of scores times log2(e), and
+// this lane's share of the sum of weights.
+template <int D, int ROWS> struct FewResult {
+  f32x4 o[ROWS / 16][D / 16];
+  float top[ROWS / 16], sum[ROWS / 16];
+};
+
 template <class E, int D, int ROWS>
-__global__ __launch_bounds__(FEW_THREADS, D == 128 ? 1 : 2) void attention_few_kernel(AttentionArgs a) {
+__device__ __forceinline__ void few_attend(const AttentionArgs &a, unsigned char *mine, const FewRun &u,
+                                           FewResult<D, ROWS> &r) {
   using L = FewLds<D>;
   constexpr int CT = ROWS / 16;                 // column tiles of 16 query rows
   constexpr int LOADS = L::HALF / (WAVE * 16);  // loads a lane and operand
   constexpr int LOAD_ROWS = FEW_KEYS / LOADS;
-  extern __shared__ __align__(16) unsigned char lds[];
-  __shared__ FewTable seqs;
-  const int per_tile = ROWS / a.group;
-  const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
-  const int quarter = lane >> 4, col = lane & 15;
-  const FewLine line = few_line(a, per_tile, gridDim.x * FEW_WAVES, seqs);
-  const int64_t number = (int64_t)blockIdx.x * FEW_WAVES + wave;
-  int64_t at = number * line.piece;
-  const int64_t end = at + line.piece < line.total ? at + line.piece : line.total;
-  if (at >= end) return;
-  // The sequence the piece begins in (the loop below walks on to it) and the
-  // tiles before that.
-  int64_t seq = few_thread(seqs.before, at), precede = seqs.before[seq];
-  seq *= line.each;
-
-  unsigned char *mine = lds + wave * L::BYTES;
+  const int lane = lane_id(), quarter = lane >> 4, col = lane & 15;
+  const int32_t *table = a.pages.table + u.seq * a.pages.cols;
   const uint32_t lds_base = lds_address(mine);
   int *ids = reinterpret_cast<int *>(mine + L::IDS);
   const int load_row = lane / (D / 8), load_slot = lane % (D / 8);
@@ -180,238 +251,341 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 ? 1 : 2) void attention_few_k
       v_at[dt][h] = L::HALF + tile_offset<D>(16 * h + 4 * sigma + (col >> 2), c >> 3) + (c & 7) * 2;
     }
 
-  while (at < end) {
-    const FewSeq s = line.seq(a, per_tile, seq);
-    const int64_t places = s.places(a.kv_heads);
-    if (at >= precede + places) {
-      precede += places;
-      seq++;
-      continue;
+  // Page numbers of the keys of tile t (and of the next 32, not used).
+  const auto fetch_ids = [&](int t) __attribute__((always_inline)) {
+    const int key = t * FEW_KEYS + lane < u.keys ? t * FEW_KEYS + lane : u.keys - 1;
+    const int32_t *src = table + (key >> a.pages.page_shift);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(
+                     __builtin_amdgcn_readfirstlane(lds_base + L::IDS + (t & 3) * (WAVE * 4))),
+                 "v"(src)
+                 : "memory", "m0");
+  };
+  fetch_ids(u.from);
+  fetch_ids(u.from + 1);
+  uint4 q[CT][D / 32];
+  int limit[CT];
+#pragma unroll
+  for (int ct = 0; ct < CT; ct++) {
+    const int row = ct * 16 + col < u.rows ? ct * 16 + col : u.rows - 1;
+    limit[ct] = u.first_limit + row / a.group;
+    const uint16_t *src = a.q.at(u.row + row / a.group, u.head * a.group + row % a.group);
+#pragma unroll
+    for (int k = 0; k < D / 32; k++) {
+      const int c = 32 * k + 8 * quarter;
+      q[ct][k] = c < a.dim ? *reinterpret_cast<const uint4 *>(src + c) : uint4{0, 0, 0, 0};
     }
-    // Place in the sequence: row tile, head, key tile.
-    const int64_t inside = at - precede;
-    const uint32_t unit = few_divide(inside, s.unit());
-    const int place = (int)(inside - (int64_t)unit * s.unit());
-    const int next = end - at < s.unit() - place ? (int)(place + (end - at)) : s.unit();
-    at += next - place;
-    const int key_tiles = s.key_tiles();
-    const int from = place > FEW_START ? place - FEW_START : 0, to = next - FEW_START;
-    if (from >= to) continue;
-    const int head = (int)(unit % (uint32_t)a.kv_heads), t0 = (int)(unit / (uint32_t)a.kv_heads) * per_tile;
-    const int tokens = s.len - t0 < per_tile ? s.len - t0 : per_tile, rows = tokens * a.group;
-    const int first_limit = s.past + t0;              // last key the first token sees
-    const int keys = first_limit + tokens;            // keys the last one sees
-    const int64_t table = seq * a.pages.cols;
+  }
+  #pragma unroll
+  for (int ct = 0; ct < CT; ct++) {
+    r.top[ct] = -INFINITY;
+    r.sum[ct] = 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; dt++) r.o[ct][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
 
-    // Page numbers of the keys of tile t (and of the next 32, not used).
-    const auto fetch_ids = [&](int t) __attribute__((always_inline)) {
-      const int key = t * FEW_KEYS + lane < keys ? t * FEW_KEYS + lane : keys - 1;
-      const int32_t *src = a.pages.table + table + (key >> a.pages.page_shift);
-      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(
-                       __builtin_amdgcn_readfirstlane(lds_base + L::IDS + (t & 3) * (WAVE * 4))),
-                   "v"(src)
-                   : "memory", "m0");
-    };
-    fetch_ids(from);
-    fetch_ids(from + 1);
-    uint4 q[CT][D / 32];
-    int limit[CT];
-#pragma unroll
-    for (int ct = 0; ct < CT; ct++) {
-      const int row = ct * 16 + col < rows ? ct * 16 + col : rows - 1;
-      limit[ct] = first_limit + row / a.group;
-      const uint16_t *src = a.q.at((int64_t)s.first + t0 + row / a.group, head * a.group + row % a.group);
-#pragma unroll
-      for (int k = 0; k < D / 32; k++) {
-        const int c = 32 * k + 8 * quarter;
-        q[ct][k] = c < a.dim ? *reinterpret_cast<const uint4 *>(src + c) : uint4{0, 0, 0, 0};
-      }
-    }
-    f32x4 o[CT][D / 16];
-    float top[CT], sum[CT];
-#pragma unroll
-    for (int ct = 0; ct < CT; ct++) {
-      top[ct] = -INFINITY;
-      sum[ct] = 0.0f;
-#pragma unroll
-      for (int dt = 0; dt < D / 16; dt++) o[ct][dt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
-
-    const auto fetch = [&](int t) __attribute__((always_inline)) {
-      const uint32_t dst = lds_base + (t & 1) * L::STAGE;
-      const int key0 = t * FEW_KEYS, id = ids[(t & 3) * WAVE + (lane & (FEW_KEYS - 1))];
-      const bool there = key0 + (lane & (FEW_KEYS - 1)) < keys && t < to;
-      const bool named = id >= 0 && id < a.pages.n_pages;
-      if (plain && __all(there && named)) {
-        // A load's rows lie in one page: its base is the same for all lanes.
-#pragma unroll
-        for (int i = 0; i < LOADS; i++) {
-          const int64_t off = ((int64_t)__builtin_amdgcn_readlane(id, i * LOAD_ROWS) * a.kv_heads + head) * head_bytes +
-                              ((key0 + i * LOAD_ROWS) & slot_mask) * row_bytes;
-          load_to_lds(a.pages.k, off, lane_at[i % 4], dst + i * (WAVE * 16));
-          load_to_lds(a.pages.v, off, lane_at[i % 4], dst + L::HALF + i * (WAVE * 16));
-        }
-        return;
-      }
-      if (there && !named && a.failure != nullptr) *a.failure = a.code;
+  const auto fetch = [&](int t) __attribute__((always_inline)) {
+    const uint32_t dst = lds_base + (t & 1) * L::STAGE;
+    const int key0 = t * FEW_KEYS, id = ids[(t & 3) * WAVE + (lane & (FEW_KEYS - 1))];
+    const bool there = key0 + (lane & (FEW_KEYS - 1)) < u.keys;
+    const bool named = id >= 0 && id < a.pages.n_pages;
+    if (plain && __all(there && named)) {
+      // A load's rows lie in one page: its base is the same for all lanes.
 #pragma unroll
       for (int i = 0; i < LOADS; i++) {
-        const int r = load_row + i * LOAD_ROWS, unit8 = load_slot ^ tile_swizzle<D>(r);
-        const int page = __shfl(id, r);
-        const int64_t off = ((int64_t)page * a.kv_heads + head) * head_bytes + ((key0 + r) & slot_mask) * row_bytes + unit8 * 16;
-        const bool live = key0 + r < keys && t < to && page >= 0 && page < a.pages.n_pages && unit8 * 8 < a.dim;
-        load_to_lds(live ? (const void *)((const char *)a.pages.k + off) : (const void *)&g_zeros, dst + i * (WAVE * 16));
-        load_to_lds(live ? (const void *)((const char *)a.pages.v + off) : (const void *)&g_zeros,
-                    dst + L::HALF + i * (WAVE * 16));
+        const int64_t off = ((int64_t)__builtin_amdgcn_readlane(id, i * LOAD_ROWS) * a.kv_heads + u.head) * head_bytes +
+                            ((key0 + i * LOAD_ROWS) & slot_mask) * row_bytes;
+        load_to_lds(a.pages.k, off, lane_at[i % 4], dst + i * (WAVE * 16));
+        load_to_lds(a.pages.v, off, lane_at[i % 4], dst + L::HALF + i * (WAVE * 16));
       }
-    };
+      return;
+    }
+    if (there && !named && a.failure != nullptr) *a.failure = a.code;
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) {
+      const int r = load_row + i * LOAD_ROWS, unit8 = load_slot ^ tile_swizzle<D>(r);
+      const int page = __shfl(id, r);
+      const int64_t off = ((int64_t)page * a.kv_heads + u.head) * head_bytes + ((key0 + r) & slot_mask) * row_bytes + unit8 * 16;
+      const bool live = key0 + r < u.keys && page >= 0 && page < a.pages.n_pages && unit8 * 8 < a.dim;
+      load_to_lds(live ? (const void *)((const char *)a.pages.k + off) : (const void *)&g_zeros, dst + i * (WAVE * 16));
+      load_to_lds(live ? (const void *)((const char *)a.pages.v + off) : (const void *)&g_zeros,
+                  dst + L::HALF + i * (WAVE * 16));
+    }
+  };
 
-    // In flight while tile t is multiplied: the page numbers of t + 2 (older),
-    // then the 2 LOADS loads of tile t + 1.
-    // The queries have arrived before the loop: inside it the compiler would wait for
-    // them, and with them for the tiles in flight, in every round.
+  // In flight while tile t is multiplied: the page numbers of t + 2 (older),
+  // then the 2 LOADS loads of tile t + 1.
+  // The queries have arrived before the loop: inside it the compiler would wait for
+  // them, and with them for the tiles in flight, in every round.
 #pragma unroll
-    for (int ct = 0; ct < CT; ct++)
+  for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-      for (int k = 0; k < D / 32; k++)
-        asm volatile("" : "+v"(q[ct][k].x), "+v"(q[ct][k].y), "+v"(q[ct][k].z), "+v"(q[ct][k].w));
-    wait_loads();
-    fetch(from);
-    fetch_ids(from + 2);
-    fetch(from + 1);
-    for (int t = from; t < to; t++) {
-      wait_older_than<2 * LOADS>();
-      unsigned char *kt = mine + (t & 1) * L::STAGE;
-      const int key0 = t * FEW_KEYS;
-      f32x4 w[CT][2];
+    for (int k = 0; k < D / 32; k++)
+      asm volatile("" : "+v"(q[ct][k].x), "+v"(q[ct][k].y), "+v"(q[ct][k].z), "+v"(q[ct][k].w));
+  wait_loads();
+  fetch(u.from);
+  fetch_ids(u.from + 2);
+  if (u.from + 1 < u.to) fetch(u.from + 1);
+  for (int t = u.from; t < u.to; t++) {
+    if (t + 1 < u.to) wait_older_than<2 * LOADS>();
+    else wait_loads();
+    unsigned char *kt = mine + (t & 1) * L::STAGE;
+    const int key0 = t * FEW_KEYS;
+    f32x4 w[CT][2];
 #pragma unroll
-      for (int b = 0; b < 2; b++) {
+    for (int b = 0; b < 2; b++) {
 #pragma unroll
-        for (int ct = 0; ct < CT; ct++) w[ct][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int ct = 0; ct < CT; ct++) w[ct][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int k = 0; k < D / 32; k++) {
-          const uint4 x = *reinterpret_cast<const uint4 *>(kt + k_at[k] + b * (16 * D * 2));
+      for (int k = 0; k < D / 32; k++) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(kt + k_at[k] + b * (16 * D * 2));
 #pragma unroll
-          for (int ct = 0; ct < CT; ct++) w[ct][b] = E::mfma16(x, q[ct][k], w[ct][b]);
-        }
+        for (int ct = 0; ct < CT; ct++) w[ct][b] = E::mfma16(x, q[ct][k], w[ct][b]);
       }
-      const bool masked = key0 + FEW_KEYS - 1 > first_limit;
-      if (masked) {
+    }
+    const bool masked = key0 + FEW_KEYS - 1 > u.first_limit;
+    if (masked) {
 #pragma unroll
-        for (int ct = 0; ct < CT; ct++)
+      for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-          for (int b = 0; b < 2; b++)
+        for (int b = 0; b < 2; b++)
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-              if (key0 + 16 * b + 4 * sigma + i > limit[ct]) w[ct][b][i] = -INFINITY;
-        // Tokens of the unit see different keys of this tile: a value that a row
-        // does not see must not reach it, and 0 * NaN would.  Values that are not
-        // finite are added one by one and taken out of the tile.
-        if (tokens > 1) {
-          bool found = false;
+          for (int i = 0; i < 4; i++)
+            if (key0 + 16 * b + 4 * sigma + i > limit[ct]) w[ct][b][i] = -INFINITY;
+    }
+    uint4 p[CT];
 #pragma unroll
-          for (int i = 0; i < LOADS; i++) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(kt + L::HALF + (i * WAVE + lane) * 16);
-            for (uint32_t y : {x.x, x.y, x.z, x.w})
-              found = found || (y & E::exponent) == E::exponent || (y >> 16 & E::exponent) == E::exponent;
-          }
-          if (__any(found)) {
-            for (int j = 0; j < FEW_KEYS; j++)
+    for (int ct = 0; ct < CT; ct++) {
+      float high = w[ct][0][0];
 #pragma unroll
-              for (int dt = 0; dt < D / 16; dt++)
+      for (int i = 1; i < 8; i++) high = fmaxf(high, w[ct][i >> 2][i & 3]);
+      high = fold_quarters(high, FMax()) * a.scale_log2;
+      if (__any(high > r.top[ct] + AT_RESCALE)) {
+        const float now = fmaxf(r.top[ct], high);
+        const float factor = now == -INFINITY ? 1.0f : exp2f(r.top[ct] - now);
+        r.top[ct] = now;
+        r.sum[ct] *= factor;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                  const int d = dt * 16 + 4 * quarter + i;
-                  const uint16_t bits =
-                      *reinterpret_cast<const uint16_t *>(kt + L::HALF + tile_offset<D>(j, d >> 3) + (d & 7) * 2);
+        for (int dt = 0; dt < D / 16; dt++) r.o[ct][dt] *= factor;
+      }
+      const float shift = r.top[ct] == -INFINITY ? 0.0f : r.top[ct];
+      f32x8 x;
 #pragma unroll
-                  for (int ct = 0; ct < CT; ct++)
-                    if ((bits & E::exponent) == E::exponent && key0 + j <= limit[ct]) o[ct][dt][i] += E::load(bits);
-                }
+      for (int i = 0; i < 8; i++) {
+        x[i] = __builtin_amdgcn_exp2f(fmaf(w[ct][i >> 2][i & 3], a.scale_log2, -shift));
+        r.sum[ct] += x[i];
+      }
+      p[ct] = E::pack(x);
+    }
+    // Tokens of the unit see different keys of this tile: a value that a row
+    // does not see must not reach it, and 0 * NaN would.  Values that are not
+    // finite are added one by one and taken out of the tile.
+    if (masked && u.tokens > 1) {
+      bool found = false;
 #pragma unroll
-            for (int i = 0; i < LOADS * 8; i++) {
-              uint16_t *x = reinterpret_cast<uint16_t *>(kt + L::HALF) + (i / 8 * WAVE + lane) * 8 + i % 8;
-              if ((*x & E::exponent) == E::exponent) *x = 0;
+      for (int i = 0; i < LOADS; i++) {
+        const uint4 x = *reinterpret_cast<const uint4 *>(kt + L::HALF + (i * WAVE + lane) * 16);
+        for (uint32_t y : {x.x, x.y, x.z, x.w})
+          found = found || (y & E::exponent) == E::exponent || (y >> 16 & E::exponent) == E::exponent;
+      }
+      if (__any(found)) {
+        for (int j = 0; j < FEW_KEYS; j++)
+#pragma unroll
+          for (int dt = 0; dt < D / 16; dt++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const int d = dt * 16 + 4 * quarter + i;
+              const uint16_t bits =
+                  *reinterpret_cast<const uint16_t *>(kt + L::HALF + tile_offset<D>(j, d >> 3) + (d & 7) * 2);
+#pragma unroll
+              for (int ct = 0; ct < CT; ct++)
+                if ((bits & E::exponent) == E::exponent && key0 + j <= limit[ct]) r.o[ct][dt][i] += E::load(bits);
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-          }
+#pragma unroll
+        for (int i = 0; i < LOADS * 8; i++) {
+          uint16_t *x = reinterpret_cast<uint16_t *>(kt + L::HALF) + (i / 8 * WAVE + lane) * 8 + i % 8;
+          if ((*x & E::exponent) == E::exponent) *x = 0;
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       }
-      uint4 p[CT];
+    }
 #pragma unroll
-      for (int ct = 0; ct < CT; ct++) {
-        float high = w[ct][0][0];
+    for (int dt = 0; dt < D / 16; dt++) {
+      const auto read = [&](int h) __attribute__((always_inline)) {
+        return bit_cast<uint2>(__builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (i16x4 __attribute__((address_space(3))) *)(kt + v_at[dt][h])));
+      };
+      const uint2 lo = read(0), hi = read(1);
 #pragma unroll
-        for (int i = 1; i < 8; i++) high = fmaxf(high, w[ct][i >> 2][i & 3]);
-        high = fold_quarters(high, FMax()) * a.scale_log2;
-        if (__any(high > top[ct] + AT_RESCALE)) {
-          const float now = fmaxf(top[ct], high);
-          const float factor = now == -INFINITY ? 1.0f : exp2f(top[ct] - now);
-          top[ct] = now;
-          sum[ct] *= factor;
-#pragma unroll
-          for (int dt = 0; dt < D / 16; dt++) o[ct][dt] *= factor;
-        }
-        const float shift = top[ct] == -INFINITY ? 0.0f : top[ct];
-        f32x8 x;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          x[i] = __builtin_amdgcn_exp2f(fmaf(w[ct][i >> 2][i & 3], a.scale_log2, -shift));
-          sum[ct] += x[i];
-        }
-        p[ct] = E::pack(x);
-      }
-#pragma unroll
-      for (int dt = 0; dt < D / 16; dt++) {
-        const auto read = [&](int h) __attribute__((always_inline)) {
-          return bit_cast<uint2>(__builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (i16x4 __attribute__((address_space(3))) *)(kt + v_at[dt][h])));
-        };
-        const uint2 lo = read(0), hi = read(1);
-#pragma unroll
-        for (int ct = 0; ct < CT; ct++) o[ct][dt] = E::mfma16(uint4{lo.x, lo.y, hi.x, hi.y}, p[ct], o[ct][dt]);
-      }
-      // The tile has been read (its reads have returned before its products); the
-      // stage takes the next but one.
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      for (int ct = 0; ct < CT; ct++) r.o[ct][dt] = E::mfma16(uint4{lo.x, lo.y, hi.x, hi.y}, p[ct], r.o[ct][dt]);
+    }
+    // The tile has been read (its reads have returned before its products); the
+    // stage takes the next but one.
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (t + 2 < u.to) {
       fetch_ids(t + 3);
       fetch(t + 2);
     }
-    wait_loads();
+  }
+  wait_loads();
+}
 
-    const bool whole = from == 0 && to == key_tiles;
-    const int64_t part = few_slot(number, from == 0 ? 1 : 0, ROWS);
+// Rows of a result, straight to the output.
+template <class E, int D, int ROWS>
+__device__ __forceinline__ void few_store(const AttentionArgs &a, const FewRun &u, const FewResult<D, ROWS> &r) {
+  const int quarter = lane_id() >> 4;
 #pragma unroll
-    for (int ct = 0; ct < CT; ct++) {
-      const int row = ct * 16 + col;
-      const float all = fold_quarters(sum[ct], FAdd());
-      if (row >= rows) continue;
-      if (!whole) {
+  for (int ct = 0; ct < ROWS / 16; ct++) {
+    const int row = ct * 16 + (lane_id() & 15);
+    const float all = fold_quarters(r.sum[ct], FAdd());
+    if (row >= u.rows) continue;
+    const int64_t out_row = u.row + row / a.group;
+    const int q_head = u.head * a.group + row % a.group;
+    const bool empty = r.top[ct] == -INFINITY;  // only scores of -inf
+    const float inverse = empty ? 0.0f : 1.0f / all;
+    uint16_t *dst = a.out.at(out_row, q_head);
 #pragma unroll
-        for (int dt = 0; dt < D / 16; dt++)
-          *reinterpret_cast<f32x4 *>(a.part_o + (part + row) * D + dt * 16 + 4 * quarter) = o[ct][dt];
-        if (quarter == 0) {
-          a.part_ml[2 * (part + row)] = top[ct];
-          a.part_ml[2 * (part + row) + 1] = all;
-        }
-        continue;
-      }
-      const int64_t out_row = (int64_t)s.first + t0 + row / a.group;
-      const int q_head = head * a.group + row % a.group;
-      const bool empty = top[ct] == -INFINITY;  // only scores of -inf
-      const float inverse = empty ? 0.0f : 1.0f / all;
-      uint16_t *dst = a.out.at(out_row, q_head);
+    for (int dt = 0; dt < D / 16; dt++) {
+      const int d = dt * 16 + 4 * quarter;
+      uint32_t x[4];
 #pragma unroll
-      for (int dt = 0; dt < D / 16; dt++) {
-        const int d = dt * 16 + 4 * quarter;
-        uint32_t x[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = E::store(empty ? 0.0f : o[ct][dt][i] * inverse);
-        if (d < a.dim) *reinterpret_cast<uint2 *>(dst + d) = uint2{x[0] | x[1] << 16, x[2] | x[3] << 16};
-      }
-      if (a.lse != nullptr && quarter == 0)
-        a.lse[out_row * a.heads + q_head] = empty ? -INFINITY : (top[ct] + log2f(all)) * LN2;
+      for (int i = 0; i < 4; i++) x[i] = E::store(empty ? 0.0f : r.o[ct][dt][i] * inverse);
+      if (d < a.dim) *reinterpret_cast<uint2 *>(dst + d) = uint2{x[0] | x[1] << 16, x[2] | x[3] << 16};
     }
+    if (a.lse != nullptr && quarter == 0)
+      a.lse[out_row * a.heads + q_head] = empty ? -INFINITY : (r.top[ct] + log2f(all)) * LN2;
+  }
+}
+// Rows of a result as a part: sums at o + row * D, maximum and sum at ml + 2 * row.
+template <int D, int ROWS>
+__device__ __forceinline__ void few_store_part(const FewRun &u, const FewResult<D, ROWS> &r, float *o, float *ml) {
+  const int quarter = lane_id() >> 4;
+#pragma unroll
+  for (int ct = 0; ct < ROWS / 16; ct++) {
+    const int row = ct * 16 + (lane_id() & 15);
+    const float all = fold_quarters(r.sum[ct], FAdd());
+    if (row >= u.rows) continue;
+#pragma unroll
+    for (int dt = 0; dt < D / 16; dt++) *reinterpret_cast<f32x4 *>(o + row * D + dt * 16 + 4 * quarter) = r.o[ct][dt];
+    if (quarter == 0) {
+      ml[2 * row] = r.top[ct];
+      ml[2 * row + 1] = all;
+    }
+  }
+}
+
+template <class E, int D, int ROWS>
+__global__ __launch_bounds__(FEW_THREADS, D == 128 ? 1 : 2) void attention_few_kernel(AttentionArgs a) {
+  extern __shared__ __align__(16) unsigned char lds[];
+  __shared__ FewTable seqs;
+  const int per_tile = ROWS / a.group;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  const int64_t number = (int64_t)blockIdx.x * FEW_WAVES + wave;
+  const FewLine line = few_line(a, per_tile, seqs);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *few_units(a, ROWS, D) = line.units;
+  int64_t at = number * line.piece;
+  const int64_t end = at + line.piece < line.total ? at + line.piece : line.total;
+  if (at >= end) return;
+  // The first of the sequences among which the piece begins (the loop below walks
+  // on to the one), and the places and units before it.
+  int64_t seq = __builtin_amdgcn_readfirstlane(seqs.thread[wave]) * line.each;
+  int64_t precede = seqs.before[wave], units_before = seqs.units_before[wave];
+  while (at < end) {
+    const FewSeq s = line.seq(a, per_tile, seq);
+    const int length = line.unit(s);
+    const int64_t places = s.units(a.kv_heads) * length;
+    if (at >= precede + places) {
+      precede += places;
+      units_before += s.units(a.kv_heads);
+      seq++;
+      continue;
+    }
+    // Place in the sequence: unit and tile.
+    const int64_t inside = at - precede;
+    const uint32_t unit = few_divide(inside, length);
+    const int place = (int)(inside - (int64_t)unit * length);
+    const int next = end - at < length - place ? (int)(place + (end - at)) : length;
+    at += next - place;
+    const int key_tiles = s.key_tiles();
+    const int from = place > line.start ? place - line.start : 0;
+    const int to = next - line.start < key_tiles ? next - line.start : key_tiles;
+    if (from >= to) continue;
+    const FewRun u(a, per_tile, s, seq, unit, from, to);
+    if (from == 0 && lane_id() == 0 && units_before + unit < a.most_units) {
+      const int64_t begin = at - (next - line.start);  // the place of the unit's first tile
+      few_unit(a, ROWS, D)[units_before + unit] = FewUnit{
+          u.row, (int)number, (int)few_divide(begin + key_tiles - 1, line.piece), u.rows, u.head, {}};
+    }
+    FewResult<D, ROWS> r;
+    few_attend<E, D, ROWS>(a, lds + wave * FewLds<D>::BYTES, u, r);
+    if (from == 0 && to == key_tiles) {
+      few_store<E, D, ROWS>(a, u, r);
+    } else {
+      const int64_t part = few_slot(number, from == 0 ? 1 : 0, ROWS);
+      few_store_part<D, ROWS>(u, r, a.part_o + part * D, a.part_ml + 2 * part);
+    }
+  }
+}
+
+// A block a unit, its waves a quarter of the keys each, joined in LDS: one launch
+// where contexts are short and the units fit the chip at once.
+template <class E, int D, int ROWS>
+__global__ __launch_bounds__(FEW_THREADS, D == 128 ? 1 : 2) void attention_few_short_kernel(AttentionArgs a) {
+  extern __shared__ __align__(16) unsigned char lds[];
+  const int per_tile = ROWS / a.group, lane = lane_id();
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  if (blockIdx.x == 0)
+    for (int64_t i = threadIdx.x; i < a.m; i += FEW_THREADS) few_seq(a, per_tile, i, true);
+  // The sequence of this unit; every wave looks.
+  FewSeq s;
+  int64_t seq = -1, before = 0;
+  for (int64_t base = 0; base < a.m && seq < 0; base += WAVE) {
+    const int64_t i = base + lane;
+    const FewSeq mine = i < a.m ? few_seq(a, per_tile, i, false) : FewSeq{0, 0, 0, 0};
+    const int64_t units = mine.units(a.kv_heads);
+    const int64_t upto = before + wave_incl_scan<int64_t, OpAdd<int64_t>>(units);
+    const uint64_t past = __ballot(upto > (int64_t)blockIdx.x);
+    if (past == 0) {
+      before = read_lane(upto, WAVE - 1);
+      continue;
+    }
+    const int at = __builtin_ctzll(past);
+    seq = base + at;
+    before = read_lane(upto, at) - read_lane(units, at);
+    s = FewSeq{read_lane(mine.first, at), read_lane(mine.past, at), read_lane(mine.len, at), read_lane(mine.row_tiles, at)};
+  }
+  if (seq < 0) return;
+  const int64_t tiles = s.key_tiles();
+  const FewRun u(a, per_tile, s, seq, (uint32_t)(blockIdx.x - before), (int)(tiles * wave / FEW_WAVES),
+                 (int)(tiles * (wave + 1) / FEW_WAVES));
+  FewResult<D, ROWS> r;
+  few_attend<E, D, ROWS>(a, lds + wave * FewLds<D>::BYTES, u, r);
+  __syncthreads();
+  float *o = reinterpret_cast<float *>(lds), *ml = o + FEW_WAVES * ROWS * D;
+  static_assert(FEW_WAVES * ROWS * (D + 2) * 4 <= FewLds<D>::BYTES * FEW_WAVES, "the parts fit where the tiles were");
+  few_store_part<D, ROWS>(u, r, o + wave * ROWS * D, ml + 2 * wave * ROWS);
+  __syncthreads();
+  for (int i = threadIdx.x; i < u.rows * (D / 4); i += FEW_THREADS) {
+    const int row = i / (D / 4), d = i % (D / 4) * 4;
+    float top = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < FEW_WAVES; w++) top = fmaxf(top, ml[2 * (w * ROWS + row)]);
+    const bool empty = top == -INFINITY;
+    f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < FEW_WAVES; w++) {
+      const float f = empty ? 0.0f : exp2f(ml[2 * (w * ROWS + row)] - top);
+      sum += f * ml[2 * (w * ROWS + row) + 1];
+      x += f * *reinterpret_cast<const f32x4 *>(o + (w * ROWS + row) * D + d);
+    }
+    const float inverse = empty ? 0.0f : 1.0f / sum;
+    const int64_t out_row = u.row + row / a.group;
+    const int q_head = u.head * a.group + row % a.group;
+    uint32_t y[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) y[j] = E::store(empty ? 0.0f : x[j] * inverse);
+    if (d < a.dim) *reinterpret_cast<uint2 *>(a.out.at(out_row, q_head) + d) = uint2{y[0] | y[1] << 16, y[2] | y[3] << 16};
+    if (a.lse != nullptr && d == 0) a.lse[out_row * a.heads + q_head] = empty ? -INFINITY : (top + log2f(sum)) * LN2;
   }
 }
 
@@ -420,36 +594,20 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 ? 1 : 2) void attention_few_k
 // parts of one.  Parts are taken in order, WAVE at a time, with the running
 // maximum and sum.
 template <class E, int D, int ROWS>
-__global__ __launch_bounds__(FEW_THREADS) void attention_few_join_kernel(AttentionArgs a, int waves, int join_rows) {
+__global__ __launch_bounds__(FEW_THREADS) void attention_few_join_kernel(AttentionArgs a, int join_rows) {
   constexpr int FOURS = D / 4, JOIN_ROWS = FEW_THREADS / FOURS, BATCH = 8;
-  __shared__ FewTable seqs;
-  __shared__ int64_t units_before[FEW_THREADS];
   __shared__ float tops[JOIN_ROWS], sums[JOIN_ROWS], factors[JOIN_ROWS], weights[JOIN_ROWS][WAVE];
   __shared__ f32x4 shared[FEW_THREADS];
-  const int per_tile = ROWS / a.group;
-  const FewLine line = few_line(a, per_tile, waves, seqs, units_before);
-  // The unit of this number, in the order of the line: the row tiles of a
-  // sequence, heads inside them.
-  const int thread = few_thread(units_before, blockIdx.x);
-  int64_t number = blockIdx.x - units_before[thread], precede = seqs.before[thread];
-  FewSeq s;
-  for (int64_t i = thread * line.each;; i++) {
-    if (i >= (thread + 1) * line.each || i >= a.m) return;
-    s = line.seq(a, per_tile, i);
-    const int64_t units = s.units(a.kv_heads);
-    if (number < units) break;
-    number -= units;
-    precede += s.places(a.kv_heads);
-  }
-  const int head = (int)(number % a.kv_heads), t0 = (int)(number / a.kv_heads) * per_tile;
-  // Its first and last tile, and the waves that had them.
-  const int64_t begin = precede + number * s.unit() + FEW_START, last = begin + s.key_tiles() - 1;
-  const int64_t w0 = few_divide(begin, line.piece), w1 = few_divide(last, line.piece);
+  // (both loads at once: the array has a place for every block)
+  const int64_t units = *few_units(a, ROWS, D);
+  const FewUnit u = few_unit(a, ROWS, D)[blockIdx.x];
+  if (blockIdx.x >= units || u.w0 == u.w1) return;
+  const int64_t w0 = u.w0, w1 = u.w1;
   const int row0 = blockIdx.y * join_rows;
-  int rows = (s.len - t0 < per_tile ? s.len - t0 : per_tile) * a.group - row0;
-  if (w0 == w1 || rows <= 0) return;  // one wave had it all
+  int rows = u.rows - row0;
+  if (rows <= 0) return;
   if (rows > join_rows) rows = join_rows;
-  const auto part = [&](int64_t w) { return few_slot(w, w * line.piece <= begin ? 1 : 0, ROWS) + row0; };
+  const auto part = [&](int64_t w) { return few_slot(w, w == w0 ? 1 : 0, ROWS) + row0; };
   if (threadIdx.x < JOIN_ROWS) tops[threadIdx.x] = -INFINITY, sums[threadIdx.x] = 0.0f;
   int share = 1;  // threads that share the parts of one place
   while (2 * share * rows * FOURS <= FEW_THREADS) share *= 2;
@@ -503,8 +661,8 @@ __global__ __launch_bounds__(FEW_THREADS) void attention_few_join_kernel(Attenti
   if (row >= rows || turn != 0) return;
   const bool empty = tops[row] == -INFINITY;
   const float inverse = empty ? 0.0f : 1.0f / sums[row];
-  const int64_t out_row = (int64_t)s.first + t0 + (row0 + row) / a.group;
-  const int q_head = head * a.group + (row0 + row) % a.group;
+  const int64_t out_row = u.row + (row0 + row) / a.group;
+  const int q_head = u.head * a.group + (row0 + row) % a.group;
   uint32_t x[4];
 #pragma unroll
   for (int i = 0; i < 4; i++) x[i] = E::store(empty ? 0.0f : o[i] * inverse);
@@ -521,22 +679,36 @@ int few_rows(int64_t n, int64_t heads, int64_t kv_heads, int64_t m) {
   return 0;
 }
 
-size_t few_workspace(int rows, int64_t head_dim) {
-  const int64_t waves = head_dim <= 64 ? few_waves<64>() : few_waves<128>();
-  return (size_t)(2 * waves * rows) * ((head_dim <= 64 ? 64 : 128) + 2) * sizeof(float);
+static int64_t few_most_units(int rows, int64_t n, int64_t group, int64_t kv_heads, int64_t m) {
+  return most_tiles(n, m, rows / group) * kv_heads;
+}
+
+size_t few_workspace(int rows, int64_t n, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t m) {
+  const int64_t floats = head_dim <= 64 ? few_part_floats(few_waves<64>(), rows, 64)
+                                        : few_part_floats(few_waves<128>(), rows, 128);
+  return (size_t)floats * sizeof(float) + 16 +
+         (size_t)few_most_units(rows, n, heads / kv_heads, kv_heads, m) * sizeof(FewUnit);
 }
 
 template <class E, int D, int ROWS>
 static int launch_few_of(hipStream_t stream, AttentionArgs a, void *workspace) {
   constexpr int LDS = FewLds<D>::BYTES * FEW_WAVES;
-  const auto kernel = attention_few_kernel<E, D, ROWS>;
+  const auto kernel = attention_few_kernel<E, D, ROWS>, short_kernel = attention_few_short_kernel<E, D, ROWS>;
   static const hipError_t raised =
       hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+  static const hipError_t raised_short =
+      hipFuncSetAttribute((const void *)short_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   if (raised != hipSuccess) return (int)raised;
+  if (raised_short != hipSuccess) return (int)raised_short;
+  const int64_t units = few_most_units(ROWS, a.q_rows, a.group, a.kv_heads, a.m);
+  if (units > INT32_MAX) return FA_ENOTSUP;
+  if (units * FEW_WAVES <= few_waves<D>() && a.pages.cols << a.pages.page_shift <= FEW_SHORT_KEYS) {
+    short_kernel<<<dim3((unsigned)units), FEW_THREADS, LDS, stream>>>(a);
+    return launch_status();
+  }
   a.part_o = (float *)workspace;
   a.part_ml = a.part_o + (int64_t)2 * few_waves<D>() * ROWS * D;
-  const int64_t units = most_tiles(a.q_rows, a.m, ROWS / a.group) * a.kv_heads;
-  if (units > INT32_MAX) return FA_ENOTSUP;
+  a.most_units = units;
   kernel<<<dim3(few_waves<D>() / FEW_WAVES), FEW_THREADS, LDS, stream>>>(a);
   const int rc = launch_status();
   if (rc != 0) return rc;
@@ -546,7 +718,7 @@ static int launch_few_of(hipStream_t stream, AttentionArgs a, void *workspace) {
   int join_rows = FEW_THREADS / (D / 4);
   while (join_rows > 1 && units * ceil_div(rows, join_rows) < NUM_CUS_HINT) join_rows /= 2;
   const dim3 grid((unsigned)units, (unsigned)ceil_div(rows, join_rows));
-  attention_few_join_kernel<E, D, ROWS><<<grid, FEW_THREADS, 0, stream>>>(a, few_waves<D>(), join_rows);
+  attention_few_join_kernel<E, D, ROWS><<<grid, FEW_THREADS, 0, stream>>>(a, join_rows);
   return launch_status();
 }
 
