@@ -204,12 +204,13 @@ __device__ __forceinline__ void load_to_lds(const void *src, uint32_t lds) {
                "v"(src)
                : "memory", "m0");
 }
-// The same from base + off (wave uniform) + lane_off.
-__device__ __forceinline__ void load_to_lds(const void *base, int64_t off, uint32_t lane_off, uint32_t lds) {
+// The same from base + off (wave uniform) + lane_off, for data that is read once:
+// the non-temporal policy (decoding 64 sequences 98.8 -> 87.3 us, 5.9 TB/s).
+__device__ __forceinline__ void stream_to_lds(const void *base, int64_t off, uint32_t lane_off, uint32_t lds) {
   const uint64_t at = (uint64_t)base + off;
   const uint64_t sat = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32)) << 32) |
                        (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(
                    __builtin_amdgcn_readfirstlane(lds)),
                "v"(lane_off), "s"(sat)
                : "memory", "m0");

@@ -294,8 +294,8 @@ __device__ __forceinline__ void few_attend(const AttentionArgs &a, unsigned char
       for (int i = 0; i < LOADS; i++) {
         const int64_t off = ((int64_t)__builtin_amdgcn_readlane(id, i * LOAD_ROWS) * a.kv_heads + u.head) * head_bytes +
                             ((key0 + i * LOAD_ROWS) & slot_mask) * row_bytes;
-        load_to_lds(a.pages.k, off, lane_at[i % 4], dst + i * (WAVE * 16));
-        load_to_lds(a.pages.v, off, lane_at[i % 4], dst + L::HALF + i * (WAVE * 16));
+        stream_to_lds(a.pages.k, off, lane_at[i % 4], dst + i * (WAVE * 16));
+        stream_to_lds(a.pages.v, off, lane_at[i % 4], dst + L::HALF + i * (WAVE * 16));
       }
       return;
     }
