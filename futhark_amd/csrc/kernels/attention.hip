@@ -96,6 +96,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
   }
 
   const TileLoads<D, AT_THREADS> loads(a.dim);
+  const TileReads<D> reads;
   const uint32_t lds_base = lds_address(lds);
   int32_t page[LOADS];
   const auto fetch_pages = [&](int key0) __attribute__((always_inline)) {
@@ -107,28 +108,49 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
       }
     }
   };
+  // Contiguous keys: this lane's next row of either array.
+  const char *k_next = nullptr, *v_next = nullptr;
+  int64_t k_step = 0, v_step = 0;
+  if constexpr (!PAGED) {
+    k_next = loads.start(a.k.at(u.k_first + from, u.kv_head), a.k.row_stride);
+    v_next = loads.start(a.v.at(u.k_first + from, u.kv_head), a.v.row_stride);
+    k_step = loads.step(a.k.row_stride);
+    v_step = loads.step(a.v.row_stride);
+  }
+  // The tile from key0 on: the next after the one fetched last.
   const auto fetch = [&](int key0, int stage) __attribute__((always_inline)) {
     const uint32_t dst = lds_base + stage * (2 * TILE);
+    if constexpr (PAGED) {
 #pragma unroll
-    for (int i = 0; i < LOADS; i++) {
-      const int key = key0 + loads.row + i * loads.STEP;
-      bool there = key < to;
-      const uint16_t *ks, *vs;
-      if constexpr (PAGED) {
+      for (int i = 0; i < LOADS; i++) {
+        const int key = key0 + loads.row + i * loads.STEP;
+        bool there = key < to;
         if (there && (page[i] < 0 || page[i] >= a.pages.n_pages)) {
           there = false;
           if (a.failure != nullptr) *a.failure = a.code;
         }
         const int64_t at = (a.pages.row_of(page[i], u.kv_head, a.kv_heads) +
                             (key & ((1 << a.pages.page_shift) - 1))) * a.dim;
-        ks = a.pages.k + at;
-        vs = a.pages.v + at;
-      } else {
-        ks = a.k.at(u.k_first + key, u.kv_head);
-        vs = a.v.at(u.k_first + key, u.kv_head);
+        loads.load(a.pages.k + at, there, dst, i);
+        loads.load(a.pages.v + at, there, dst + TILE, i);
       }
-      loads.load(ks, there, dst, i);
-      loads.load(vs, there, dst + TILE, i);
+    } else if (key0 + AT_KEYS <= to) {
+#pragma unroll
+      for (int i = 0; i < LOADS; i++) {
+        loads.load(k_next, dst, i);
+        loads.load(v_next, dst + TILE, i);
+        k_next += k_step;
+        v_next += v_step;
+      }
+    } else {  // the last: rows past the end are zeros
+#pragma unroll
+      for (int i = 0; i < LOADS; i++) {
+        const bool there = key0 + loads.row + i * loads.STEP < to;
+        loads.load(there ? (const void *)k_next : (const void *)&g_zeros, dst, i);
+        loads.load(there ? (const void *)v_next : (const void *)&g_zeros, dst + TILE, i);
+        k_next += k_step;
+        v_next += v_step;
+      }
     }
   };
 
@@ -151,8 +173,10 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
   fetch_pages(from);
   if (from < to) fetch(from, 0);
   fetch_pages(from + AT_KEYS);
-  int stage = 0;
-  for (int key0 = from; key0 < to; key0 += AT_KEYS, stage ^= 1) {
+
+  // One tile.  At the BORDER rows of the block see different keys of it, or not all.
+  const auto attend = [&](int key0, int stage, auto border) __attribute__((always_inline)) {
+    constexpr bool BORDER = decltype(border)::value;
     wait_loads();
     __syncthreads();
     if (key0 + AT_KEYS < to) {
@@ -160,11 +184,9 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
       fetch_pages(key0 + 2 * AT_KEYS);
     }
     unsigned char *kt = lds + stage * (2 * TILE), *vt = kt + TILE;
-    const int last = key0 + AT_KEYS - 1;
-    // Rows of the block see different keys of this tile: a value that a row does
-    // not see must not reach it, and 0 * NaN would.
+    // A value that a row does not see must not reach it, and 0 * NaN would.
     bool unsafe = false;
-    if (last > block_first && block_first < block_last) {
+    if (BORDER && block_first < block_last) {
       bool found = false;
 #pragma unroll
       for (int i = 0; i < LOADS; i++) {
@@ -174,7 +196,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
       }
       unsafe = __syncthreads_or(found);
     }
-    const bool active = wave_works && key0 <= wave_last;
+    const bool active = wave_works && (!BORDER || key0 <= wave_last);
     uint4 p[4];
     if (active) {
       f32x16 s[2];
@@ -183,9 +205,9 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
 #pragma unroll
         for (int i = 0; i < 16; i++) s[b][i] = 0.0f;
 #pragma unroll
-        for (int ks = 0; ks < D / 16; ks++) s[b] = E::mfma(tile_rows<D>(kt, b * 32 + (lane & 31), ks), q[ks], s[b]);
+        for (int ks = 0; ks < D / 16; ks++) s[b] = E::mfma(reads.rows(kt, b * 32, ks), q[ks], s[b]);
       }
-      if (last > wave_first) {
+      if (BORDER && key0 + AT_KEYS - 1 > wave_first) {
 #pragma unroll
         for (int b = 0; b < 2; b++)
 #pragma unroll
@@ -218,7 +240,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
         p[c] = E::pack(w);
       }
     }
-    if (unsafe) {
+    if (BORDER && unsafe) {
       // Add what the rows see of the values that are not finite, one by one, and
       // take them out of the tile.
       if (active) {
@@ -245,9 +267,22 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
 #pragma unroll
       for (int c = 0; c < 4; c++)
 #pragma unroll
-        for (int dt = 0; dt < D / 32; dt++) o[dt] = E::mfma(tile_columns<D>(vt, c * 16, dt * 32), p[c], o[dt]);
+        for (int dt = 0; dt < D / 32; dt++) o[dt] = E::mfma(reads.columns(vt, c * 16, dt), p[c], o[dt]);
     }
+  };
+  const int full = block_first + 1 < to ? block_first + 1 : to;  // keys before it are seen by all rows
+  int key0 = from, stage = 0;
+  for (;;) {  // a stage is a constant here
+    if (key0 + AT_KEYS > full) break;
+    attend(key0, 0, std::false_type());
+    key0 += AT_KEYS;
+    stage = 1;
+    if (key0 + AT_KEYS > full) break;
+    attend(key0, 1, std::false_type());
+    key0 += AT_KEYS;
+    stage = 0;
   }
+  for (; key0 < to; key0 += AT_KEYS, stage ^= 1) attend(key0, stage, std::true_type());
 
   sum = fold_halves(sum, FAdd());
   if (row >= rows) return;

@@ -221,25 +221,41 @@ __device__ __forceinline__ uint32_t lds_address(const void *p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char *)p;
 }
 
-// Operand of a product over components: row `r`, components 16 step + 8 (lane / 32) ...
-template <int D> __device__ __forceinline__ uint4 tile_rows(const unsigned char *tile, int r, int step) {
-  return *reinterpret_cast<const uint4 *>(tile + tile_offset<D>(r, 2 * step + (lane_id() >> 5)));
-}
-// Operand of a product over rows: for lane l component c0 + l % 32 of the rows
-// r0 + 4 (l / 32) + {0..3, 8..11}: the rows whose products a lane holds in
-// registers 0..7 of an MFMA result, so that a result is the other operand as it
-// stands.  r0 is a multiple of 16, c0 of 32.
-template <int D> __device__ __forceinline__ uint4 tile_columns(const unsigned char *tile, int r0, int c0) {
-  const int l = lane_id(), r = l & 15;
-  const int row = r0 + 4 * (l >> 5) + (r >> 2), c = c0 + ((l >> 4) & 1) * 16 + 4 * (r & 3);
-  const auto read = [&](int at) __attribute__((always_inline)) {
-    const unsigned char *p = tile + tile_offset<D>(at, c >> 3) + (c & 7) * 2;
-    return bit_cast<uint2>(
-        __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 __attribute__((address_space(3))) *)(p)));
-  };
-  const uint2 lo = read(row), hi = read(row + 8);
-  return uint4{lo.x, lo.y, hi.x, hi.y};
-}
+// How a lane reads a tile for the 32 x 32 x 16 products; places are kept, so that
+// a read is an instruction with a constant offset.
+template <int D> struct TileReads {
+  int row[D / 16], column[D / 32][2];
+  __device__ __forceinline__ TileReads() {
+    const int l = lane_id(), r = l & 15;
+#pragma unroll
+    for (int s = 0; s < D / 16; s++) row[s] = tile_offset<D>(l & 31, 2 * s + (l >> 5));
+#pragma unroll
+    for (int t = 0; t < D / 32; t++)
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        const int c = t * 32 + ((l >> 4) & 1) * 16 + 4 * (r & 3);
+        column[t][h] = tile_offset<D>(8 * h + 4 * (l >> 5) + (r >> 2), c >> 3) + (c & 7) * 2;
+      }
+  }
+  // Operand of a product over components: row r0 + l % 32 (r0 a multiple of 32),
+  // components 16 s + 8 (l / 32) ...
+  __device__ __forceinline__ uint4 rows(const unsigned char *tile, int r0, int s) const {
+    return *reinterpret_cast<const uint4 *>(tile + r0 * (D * 2) + row[s]);
+  }
+  // Operand of a product over rows: for lane l component 32 t + l % 32 of the rows
+  // r0 + 4 (l / 32) + {0..3, 8..11} (r0 a multiple of 16): the rows whose products a
+  // lane holds in registers 0..7 of an MFMA result, so that a result is the other
+  // operand as it stands.
+  __device__ __forceinline__ uint4 columns(const unsigned char *tile, int r0, int t) const {
+    const auto read = [&](int h) __attribute__((always_inline)) {
+      const unsigned char *p = tile + r0 * (D * 2) + column[t][h];
+      return bit_cast<uint2>(
+          __builtin_amdgcn_ds_read_tr16_b64_v4i16((i16x4 __attribute__((address_space(3))) *)(p)));
+    };
+    const uint2 lo = read(0), hi = read(1);
+    return uint4{lo.x, lo.y, hi.x, hi.y};
+  }
+};
 
 static __device__ uint4 g_zeros;  // what is loaded in place of rows and units that are not there
 
@@ -257,6 +273,15 @@ template <int D, int THREADS> struct TileLoads {
     unit = (threadIdx.x % (D / 8)) ^ tile_swizzle<D>(row);
     live = unit * 8 < dim;
     lds = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE) * 1024;
+  }
+  // Bytes from one of this lane's rows to its next, 0 for a lane that loads zeros.
+  __device__ __forceinline__ int64_t step(int64_t row_stride) const { return live ? row_stride * (2 * STEP) : 0; }
+  // Where this lane starts in rows beginning at `first`.
+  __device__ __forceinline__ const char *start(const uint16_t *first, int64_t row_stride) const {
+    return live ? (const char *)(first + row * row_stride + unit * 8) : (const char *)&g_zeros;
+  }
+  __device__ __forceinline__ void load(const void *src, uint32_t tile, int i) const {
+    load_to_lds(src, tile + lds + i * (THREADS * 16));
   }
   __device__ __forceinline__ void load(const uint16_t *row_data, bool there, uint32_t tile, int i) const {
     const void *src = there && live ? (const void *)(row_data + unit * 8) : (const void *)&g_zeros;

@@ -87,6 +87,7 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, 2) void atten
   const int keys = last_key(tokens - 1) + 1;
 
   const TileLoads<D, AG_THREADS> loads(a.dim);
+  const TileReads<D> reads;
   const uint32_t lds_base = lds_address(lds);
   const auto fetch = [&](int key0, int stage) __attribute__((always_inline)) {
 #pragma unroll
@@ -125,8 +126,8 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, 2) void atten
     for (int i = 0; i < 16; i++) p[i] = dp[i] = 0.0f;
 #pragma unroll
     for (int s = 0; s < D / 16; s++) {
-      p = E::mfma(tile_rows<D>(kt, b + (lane & 31), s), q[s], p);
-      dp = E::mfma(tile_rows<D>(kt + TILE, b + (lane & 31), s), g[s], dp);
+      p = E::mfma(reads.rows(kt, b, s), q[s], p);
+      dp = E::mfma(reads.rows(kt + TILE, b, s), g[s], dp);
     }
 #pragma unroll
     for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(fmaf(p[i], scale_log2, -shift));
@@ -174,7 +175,7 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, 2) void atten
         const uint4 ds = E::pack(w);
 #pragma unroll
         for (int dt = 0; dt < D / 32; dt++)
-          dq[dt] = E::mfma(tile_columns<D>(kt, b + c * 16, dt * 32), ds, dq[dt]);
+          dq[dt] = E::mfma(reads.columns(kt, b + c * 16, dt), ds, dq[dt]);
       }
     }
   });
@@ -251,6 +252,7 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 
   }
 
   const TileLoads<D, AG_THREADS> loads(a.dim);
+  const TileReads<D> reads;
   const uint32_t lds_base = lds_address(lds);
   // Row r of a step is token r / heads, head r % heads of the step's tokens and chunk.
   const auto place = [&](int r, int64_t step, int &token, int &head) __attribute__((always_inline)) {
@@ -320,7 +322,7 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 
         for (int i = 0; i < 16; i++) p[x][i] = dp[x][i] = 0.0f;
 #pragma unroll
       for (int s = 0; s < D / 16; s++) {
-        const uint4 qr = tile_rows<D>(qt, b + (lane & 31), s), gr = tile_rows<D>(gt, b + (lane & 31), s);
+        const uint4 qr = reads.rows(qt, b, s), gr = reads.rows(gt, b, s);
 #pragma unroll
         for (int x = 0; x < KT; x++) p[x] = E::mfma(qr, k[x][s], p[x]);
 #pragma unroll
@@ -368,7 +370,7 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 
         }
 #pragma unroll
         for (int dt = 0; dt < D / 32; dt++) {
-          const uint4 gc = tile_columns<D>(gt, b + 16 * c, dt * 32), qc = tile_columns<D>(qt, b + 16 * c, dt * 32);
+          const uint4 gc = reads.columns(gt, b + 16 * c, dt), qc = reads.columns(qt, b + 16 * c, dt);
 #pragma unroll
           for (int x = 0; x < KT; x++) dv[x][dt] = E::mfma(gc, pw[x], dv[x][dt]);
 #pragma unroll
