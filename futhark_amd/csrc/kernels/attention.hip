@@ -98,70 +98,65 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
   const TileLoads<D, AT_THREADS> loads(a.dim);
   const TileReads<D> reads;
   const uint32_t lds_base = lds_address(lds);
-  int32_t page[LOADS];
+  clear_unloaded<D>(lds, 4 * TILE, a.dim);
+  // Paged: this lane's one of the page numbers of the next tile of keys, and of
+  // the next of values.
+  int k_page = 0, v_page = 0;
   const auto fetch_pages = [&](int key0) __attribute__((always_inline)) {
     if constexpr (PAGED) {
-#pragma unroll
-      for (int i = 0; i < LOADS; i++) {
-        const int key = key0 + loads.row + i * loads.STEP;
-        page[i] = key < to ? a.pages.table[u.seg * a.pages.cols + (key >> a.pages.page_shift)] : 0;
-      }
+      v_page = k_page;
+      const int key = key0 + lane < to ? key0 + lane : to - 1;
+      k_page = a.pages.table[u.seg * a.pages.cols + (key >> a.pages.page_shift)];
     }
   };
-  // Contiguous keys: this lane's next row of either array.
-  const char *k_next = nullptr, *v_next = nullptr;
-  int64_t k_step = 0, v_step = 0;
-  if constexpr (!PAGED) {
-    k_next = loads.start(a.k.at(u.k_first + from, u.kv_head), a.k.row_stride);
-    v_next = loads.start(a.v.at(u.k_first + from, u.kv_head), a.v.row_stride);
-    k_step = loads.step(a.k.row_stride);
-    v_step = loads.step(a.v.row_stride);
-  }
-  // The tile from key0 on: the next after the one fetched last.
-  const auto fetch = [&](int key0, int stage) __attribute__((always_inline)) {
-    const uint32_t dst = lds_base + stage * (2 * TILE);
+  const int64_t k_stride = PAGED ? a.dim : a.k.row_stride, v_stride = PAGED ? a.dim : a.v.row_stride;
+  const uint32_t k_offset = loads.offset(k_stride), v_offset = loads.offset(v_stride);
+  const int slot_mask = PAGED ? (1 << a.pages.page_shift) - 1 : 0;
+  // The keys (values) from key0 on to the tile at LDS address `tile`.
+  const auto fetch_one = [&](int key0, uint32_t tile, int page, const uint16_t *pages, const Heads &x, int64_t stride,
+                             uint32_t offset) __attribute__((always_inline)) {
     if constexpr (PAGED) {
+      const bool there = key0 + lane < to, named = page >= 0 && page < a.pages.n_pages;
+      // Rows of a load in one page: its address is the same for all lanes.
+      if (slot_mask >= loads.ROWS - 1 && __all(there && named)) {
+        if (loads.live) {
 #pragma unroll
-      for (int i = 0; i < LOADS; i++) {
-        const int key = key0 + loads.row + i * loads.STEP;
-        bool there = key < to;
-        if (there && (page[i] < 0 || page[i] >= a.pages.n_pages)) {
-          there = false;
-          if (a.failure != nullptr) *a.failure = a.code;
+          for (int i = 0; i < LOADS; i++) {
+            const int r = loads.first_row + i * loads.STEP;
+            const int64_t id = __builtin_amdgcn_readlane(page, r);
+            load_to_lds(pages + (a.pages.row_of(id, u.kv_head, a.kv_heads) + ((key0 + r) & slot_mask)) * a.dim, offset,
+                        loads.place(tile, i));
+          }
         }
-        const int64_t at = (a.pages.row_of(page[i], u.kv_head, a.kv_heads) +
-                            (key & ((1 << a.pages.page_shift) - 1))) * a.dim;
-        loads.load(a.pages.k + at, there, dst, i);
-        loads.load(a.pages.v + at, there, dst + TILE, i);
+        return;
       }
-    } else if (key0 + AT_KEYS <= to) {
+      if (there && !named && a.failure != nullptr) *a.failure = a.code;
+      const int safe = there && named ? page : -1;
 #pragma unroll
       for (int i = 0; i < LOADS; i++) {
-        loads.load(k_next, dst, i);
-        loads.load(v_next, dst + TILE, i);
-        k_next += k_step;
-        v_next += v_step;
+        const int id = __shfl(safe, loads.row(i));
+        if (loads.live)
+          loads.load(pages + (a.pages.row_of(id, u.kv_head, a.kv_heads) + ((key0 + loads.row(i)) & slot_mask)) * a.dim,
+                     id >= 0, tile, i);
       }
-    } else {  // the last: rows past the end are zeros
-#pragma unroll
-      for (int i = 0; i < LOADS; i++) {
-        const bool there = key0 + loads.row + i * loads.STEP < to;
-        loads.load(there ? (const void *)k_next : (const void *)&g_zeros, dst, i);
-        loads.load(there ? (const void *)v_next : (const void *)&g_zeros, dst + TILE, i);
-        k_next += k_step;
-        v_next += v_step;
-      }
+    } else {
+      const uint16_t *first = x.at(u.k_first + key0, u.kv_head);
+      if (key0 + AT_KEYS <= to) loads.load(first, stride, offset, tile);
+      else loads.load(first, stride, to - key0, tile);
     }
+  };
+  const auto fetch_k = [&](int key0, int stage) __attribute__((always_inline)) {
+    fetch_one(key0, lds_base + stage * (2 * TILE), k_page, a.pages.k, a.k, k_stride, k_offset);
+  };
+  const auto fetch_v = [&](int key0, int stage, int page) __attribute__((always_inline)) {
+    fetch_one(key0, lds_base + stage * (2 * TILE) + TILE, page, a.pages.v, a.v, v_stride, v_offset);
   };
 
   uint4 q[D / 16];
   {
     const uint16_t *src = a.q.at(u.q_first + u.t0 + token, head);
 #pragma unroll
-    for (int ks = 0; ks < D / 16; ks++) {
-      const int c = ks * 16 + half * 8;
-      q[ks] = c < a.dim ? *reinterpret_cast<const uint4 *>(src + c) : uint4{0, 0, 0, 0};
-    }
+    for (int ks = 0; ks < D / 16; ks++) q[ks] = load_unit(src, ks * 16 + half * 8, a.dim);
   }
   f32x16 o[D / 32];
 #pragma unroll
@@ -170,23 +165,67 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
     for (int i = 0; i < 16; i++) o[dt][i] = 0.0f;
   float top = -INFINITY, sum = 0.0f;  // top: of scores times log2(e); sum: this lane's half
 
-  fetch_pages(from);
-  if (from < to) fetch(from, 0);
-  fetch_pages(from + AT_KEYS);
+  // Scores of 32 keys, their maximum, their weights, and the weights' products
+  // with the values.
+  const auto scores = [&](const unsigned char *kt, int b) __attribute__((always_inline)) {
+    f32x16 s;
+#pragma unroll
+    for (int i = 0; i < 16; i++) s[i] = 0.0f;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ks++) s = E::mfma(reads.rows(kt, b * 32, ks), q[ks], s);
+    return s;
+  };
+  const auto maximum = [&](const f32x16 &s) __attribute__((always_inline)) {
+    float high = s[0];
+#pragma unroll
+    for (int i = 1; i < 16; i++) high = fmaxf(high, s[i]);
+    return fold_halves(high, FMax()) * a.scale_log2;
+  };
+  const auto raise = [&](float high) __attribute__((always_inline)) {
+    if (__any(high > top + AT_RESCALE)) {
+      const float now = fmaxf(top, high);
+      const float factor = now == -INFINITY ? 1.0f : exp2f(top - now);
+      top = now;
+      sum *= factor;
+#pragma unroll
+      for (int dt = 0; dt < D / 32; dt++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[dt][i] *= factor;
+    }
+  };
+  const auto weigh = [&](const f32x16 &s, uint4 (&p)[2]) __attribute__((always_inline)) {
+    const float shift = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+    for (int c = 0; c < 2; c++) {
+      f32x8 w;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        w[i] = __builtin_amdgcn_exp2f(fmaf(s[c * 8 + i], a.scale_log2, -shift));
+        sum += w[i];
+      }
+      p[c] = E::pack(w);
+    }
+  };
+  const auto values = [&](const unsigned char *vt, int b, const uint4 (&p)[2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int c = 0; c < 2; c++)
+#pragma unroll
+      for (int dt = 0; dt < D / 32; dt++) o[dt] = E::mfma(reads.columns(vt, b * 32 + c * 16, dt), p[c], o[dt]);
+  };
 
-  // One tile.  At the BORDER rows of the block see different keys of it, or not all.
-  const auto attend = [&](int key0, int stage, auto border) __attribute__((always_inline)) {
-    constexpr bool BORDER = decltype(border)::value;
+  // A tile of which rows of the block see different keys, or that is not full.
+  const auto border = [&](int key0, int stage) __attribute__((always_inline)) {
     wait_loads();
     __syncthreads();
     if (key0 + AT_KEYS < to) {
-      fetch(key0 + AT_KEYS, stage ^ 1);
+      fetch_k(key0 + AT_KEYS, stage ^ 1);
+      fetch_v(key0 + AT_KEYS, stage ^ 1, k_page);
       fetch_pages(key0 + 2 * AT_KEYS);
     }
     unsigned char *kt = lds + stage * (2 * TILE), *vt = kt + TILE;
     // A value that a row does not see must not reach it, and 0 * NaN would.
     bool unsafe = false;
-    if (BORDER && block_first < block_last) {
+    if (block_first < block_last) {
       bool found = false;
 #pragma unroll
       for (int i = 0; i < LOADS; i++) {
@@ -196,51 +235,24 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
       }
       unsafe = __syncthreads_or(found);
     }
-    const bool active = wave_works && (!BORDER || key0 <= wave_last);
-    uint4 p[4];
+    const bool active = wave_works && key0 <= wave_last;
+    uint4 p[2][2];
     if (active) {
       f32x16 s[2];
 #pragma unroll
-      for (int b = 0; b < 2; b++) {
-#pragma unroll
-        for (int i = 0; i < 16; i++) s[b][i] = 0.0f;
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ks++) s[b] = E::mfma(reads.rows(kt, b * 32, ks), q[ks], s[b]);
-      }
-      if (BORDER && key0 + AT_KEYS - 1 > wave_first) {
+      for (int b = 0; b < 2; b++) s[b] = scores(kt, b);
+      if (key0 + AT_KEYS - 1 > wave_first) {
 #pragma unroll
         for (int b = 0; b < 2; b++)
 #pragma unroll
           for (int i = 0; i < 16; i++)
             if (key0 + b * 32 + 8 * (i >> 2) + 4 * half + (i & 3) > limit) s[b][i] = -INFINITY;
       }
-      float high = s[0][0];
+      raise(fmaxf(maximum(s[0]), maximum(s[1])));
 #pragma unroll
-      for (int i = 1; i < 32; i++) high = fmaxf(high, s[i >> 4][i & 15]);
-      high = fold_halves(high, FMax()) * a.scale_log2;
-      if (__any(high > top + AT_RESCALE)) {
-        const float now = fmaxf(top, high);
-        const float factor = now == -INFINITY ? 1.0f : exp2f(top - now);
-        top = now;
-        sum *= factor;
-#pragma unroll
-        for (int dt = 0; dt < D / 32; dt++)
-#pragma unroll
-          for (int i = 0; i < 16; i++) o[dt][i] *= factor;
-      }
-      const float shift = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-      for (int c = 0; c < 4; c++) {
-        f32x8 w;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-          w[i] = __builtin_amdgcn_exp2f(fmaf(s[c >> 1][(c & 1) * 8 + i], a.scale_log2, -shift));
-          sum += w[i];
-        }
-        p[c] = E::pack(w);
-      }
+      for (int b = 0; b < 2; b++) weigh(s[b], p[b]);
     }
-    if (BORDER && unsafe) {
+    if (unsafe) {
       // Add what the rows see of the values that are not finite, one by one, and
       // take them out of the tile.
       if (active) {
@@ -265,24 +277,116 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
     }
     if (active) {
 #pragma unroll
-      for (int c = 0; c < 4; c++)
-#pragma unroll
-        for (int dt = 0; dt < D / 32; dt++) o[dt] = E::mfma(reads.columns(vt, c * 16, dt), p[c], o[dt]);
+      for (int b = 0; b < 2; b++) values(vt, b, p[b]);
     }
   };
+
+  // Tiles all rows see.  The scores of the next 32 keys are computed while the
+  // weights of the last are: both kinds of instructions of one wave in turn.  Keys
+  // and values are fetched apart, each as soon as its half of a stage is free, two
+  // tiles (keys) and one tile (values) ahead.
   const int full = block_first + 1 < to ? block_first + 1 : to;  // keys before it are seen by all rows
-  int key0 = from, stage = 0;
-  for (;;) {  // a stage is a constant here
-    if (key0 + AT_KEYS > full) break;
-    attend(key0, 0, std::false_type());
-    key0 += AT_KEYS;
-    stage = 1;
-    if (key0 + AT_KEYS > full) break;
-    attend(key0, 1, std::false_type());
-    key0 += AT_KEYS;
-    stage = 0;
+  const int tiles = full > from ? (full - from) / AT_KEYS : 0;
+  const auto key_of = [&](int tile) { return from + tile * AT_KEYS; };
+  f32x16 s0, s1;
+  // Scores s1 of 32 keys of `kt` (from b * 32 on) while the weights of s0 are
+  // computed, then the products of those with 32 values of `vt` (from c * 32 on)
+  // while the maximum of the new scores is taken.  The order is
+  // fixed by hand: an LDS read for the next product, a product, a share of the
+  // other work.
+  const auto half_step = [&](const f32x16 &s0, f32x16 &s1, const unsigned char *kt, int b, const unsigned char *vt, int c)
+      __attribute__((always_inline)) {
+    constexpr int PRODUCTS = D / 16, SHARE = 16 / PRODUCTS;  // in each half; scores a product
+    const float shift = top == -INFINITY ? 0.0f : top;
+    uint32_t p[8];
+#pragma unroll
+    for (int i = 0; i < 16; i++) s1[i] = 0.0f;
+    uint4 x = reads.rows(kt, b * 32, 0);
+    static_for<PRODUCTS>([&](auto i) __attribute__((always_inline)) {
+      uint4 next;
+      if constexpr (i + 1 < PRODUCTS) next = reads.rows(kt, b * 32, i + 1);
+      else next = reads.columns(vt, c * 32, 0);
+      s1 = E::mfma(x, q[i], s1);
+#pragma unroll
+      for (int j = 0; j < SHARE; j += 2) {
+        const int e = i * SHARE + j;
+        const float w0 = __builtin_amdgcn_exp2f(fmaf(s0[e], a.scale_log2, -shift));
+        const float w1 = __builtin_amdgcn_exp2f(fmaf(s0[e + 1], a.scale_log2, -shift));
+        sum += w0;
+        sum += w1;
+        p[e / 2] = E::pack(w0, w1);
+      }
+      x = next;
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    float high = -INFINITY;
+    static_for<PRODUCTS>([&](auto i) __attribute__((always_inline)) {
+      constexpr int half_keys = i / (D / 32), dt = i % (D / 32), n = i + 1;
+      uint4 next = x;
+      if constexpr (n < PRODUCTS) next = reads.columns(vt, c * 32 + n / (D / 32) * 16, n % (D / 32));
+      o[dt] = E::mfma(x, uint4{p[4 * half_keys], p[4 * half_keys + 1], p[4 * half_keys + 2], p[4 * half_keys + 3]}, o[dt]);
+#pragma unroll
+      for (int j = 0; j < SHARE; j += 2) high = fmaxf(high, fmaxf(s1[i * SHARE + j], s1[i * SHARE + j + 1]));
+      x = next;
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    raise(fold_halves(high, FMax()) * a.scale_log2);
+  };
+  const auto attend = [&](int t, int stage, auto is_last) __attribute__((always_inline)) {
+    constexpr bool LAST = decltype(is_last)::value;
+    const unsigned char *kt = lds + stage * (2 * TILE), *vt = kt + TILE;
+    if constexpr (LAST) wait_loads();
+    else wait_but<LOADS>();
+    block_barrier();
+    if (!LAST || key_of(t + 1) < to) fetch_v(key_of(t + 1), stage ^ 1, v_page);
+    if (wave_works) half_step(s0, s1, kt, 1, vt, 0);
+    if constexpr (LAST) {
+      if (wave_works) {
+        uint4 p[2];
+        weigh(s1, p);
+        values(vt, 1, p);
+      }
+    } else {
+      wait_but<LOADS>();
+      block_barrier();
+      if (key_of(t + 2) < to && t + 2 <= tiles) {
+        fetch_k(key_of(t + 2), stage);
+        fetch_pages(key_of(t + 3));
+      }
+      if (wave_works) half_step(s1, s0, lds + (stage ^ 1) * (2 * TILE), 0, vt, 1);
+    }
+  };
+  arrived(q);
+  fetch_pages(from);
+  if (from < to) {
+    fetch_k(from, 0);
+    fetch_v(from, 0, k_page);
   }
-  for (; key0 < to; key0 += AT_KEYS, stage ^= 1) attend(key0, stage, std::true_type());
+  fetch_pages(from + AT_KEYS);
+  int t = 0;
+  const auto simple = [&](int t, int stage) __attribute__((always_inline)) {
+    wait_loads();
+    block_barrier();
+    if (key_of(t + 1) < to) {
+      fetch_k(key_of(t + 1), stage ^ 1);
+      fetch_v(key_of(t + 1), stage ^ 1, k_page);
+      fetch_pages(key_of(t + 2));
+    }
+    const unsigned char *kt = lds + stage * (2 * TILE), *vt = kt + TILE;
+    if (wave_works) {
+      f32x16 s[2];
+#pragma unroll
+      for (int b = 0; b < 2; b++) s[b] = scores(kt, b);
+      raise(fmaxf(maximum(s[0]), maximum(s[1])));
+      uint4 p[2][2];
+#pragma unroll
+      for (int b = 0; b < 2; b++) weigh(s[b], p[b]);
+#pragma unroll
+      for (int b = 0; b < 2; b++) values(vt, b, p[b]);
+    }
+  };
+  for (; t < tiles; t++) simple(t, t & 1);
+  for (; key_of(t) < to; t++) border(key_of(t), t & 1);
 
   sum = fold_halves(sum, FAdd());
   if (row >= rows) return;

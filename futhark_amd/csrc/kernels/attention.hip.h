@@ -13,6 +13,17 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 
 typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+// f(integral_constant<int, 0>) ... f(integral_constant<int, N - 1>), in order.
+template <int N, class F> __device__ __forceinline__ void static_for(F &&f) {
+  if constexpr (N > 0) {
+    static_for<N - 1>(f);
+    f(std::integral_constant<int, N - 1>());
+  }
+}
 
 // 16-bit element types.  `store` and `pack` round to nearest even; `mfma` is
 // C += A B with A 32 x 16, B 16 x 32: lane l holds row (column) l % 32 of A (B)
@@ -24,6 +35,9 @@ struct ElemF16 {
   static __device__ __forceinline__ uint16_t store(float f) { return bit_cast<uint16_t>((_Float16)f); }
   static __device__ __forceinline__ uint4 pack(f32x8 x) {
     return bit_cast<uint4>(__builtin_convertvector(x, f16x8));
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    return bit_cast<uint32_t>(__builtin_convertvector(f32x2{lo, hi}, f16x2));
   }
   static __device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(bit_cast<f16x8>(a), bit_cast<f16x8>(b), c, 0, 0, 0);
@@ -39,6 +53,9 @@ struct ElemBF16 {
   static __device__ __forceinline__ uint16_t store(float f) { return bit_cast<uint16_t>((__bf16)f); }
   static __device__ __forceinline__ uint4 pack(f32x8 x) {
     return bit_cast<uint4>(__builtin_convertvector(x, bf16x8));
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    return bit_cast<uint32_t>(__builtin_convertvector(f32x2{lo, hi}, bf16x2));
   }
   static __device__ __forceinline__ f32x16 mfma(uint4 a, uint4 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(bit_cast<bf16x8>(a), bit_cast<bf16x8>(b), c, 0, 0, 0);
@@ -204,18 +221,38 @@ __device__ __forceinline__ void load_to_lds(const void *src, uint32_t lds) {
                "v"(src)
                : "memory", "m0");
 }
-// The same from base + off (wave uniform) + lane_off, for data that is read once:
-// the non-temporal policy (decoding 64 sequences 98.8 -> 87.3 us, 5.9 TB/s).
-__device__ __forceinline__ void stream_to_lds(const void *base, int64_t off, uint32_t lane_off, uint32_t lds) {
-  const uint64_t at = (uint64_t)base + off;
-  const uint64_t sat = ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32)) << 32) |
-                       (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at);
+// The same from base + offset, base the same for the wave.
+__device__ __forceinline__ uint64_t wave_address(const void *base) {
+  const uint64_t at = (uint64_t)base;
+  return ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(at >> 32)) << 32) |
+         (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)at);
+}
+__device__ __forceinline__ void load_to_lds(const void *base, uint32_t offset, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(
+                   __builtin_amdgcn_readfirstlane(lds)),
+               "v"(offset), "s"(wave_address(base))
+               : "memory", "m0");
+}
+// And for data that is read once: the non-temporal policy (decoding 64 sequences
+// 98.8 -> 87.3 us, 5.9 TB/s).
+__device__ __forceinline__ void stream_to_lds(const void *base, uint32_t offset, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"s"(
                    __builtin_amdgcn_readfirstlane(lds)),
-               "v"(lane_off), "s"(sat)
+               "v"(offset), "s"(wave_address(base))
                : "memory", "m0");
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+
+// All but the N youngest loads have arrived.
+template <int N> __device__ __forceinline__ void wait_but() {
+  static_assert(N == 2 || N == 4 || N == 8 || N == 16, "loads of a tile");
+  if constexpr (N == 2) asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
+  if constexpr (N == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
+  if constexpr (N == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+  if constexpr (N == 16) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+}
+// A barrier that leaves younger loads in flight; what was read of LDS has arrived.
+__device__ __forceinline__ void block_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
 __device__ __forceinline__ uint32_t lds_address(const void *p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) unsigned char *)p;
@@ -259,35 +296,70 @@ template <int D> struct TileReads {
 
 static __device__ uint4 g_zeros;  // what is loaded in place of rows and units that are not there
 
-// A block's loads of a tile of 64 rows: load i of a thread brings 16-byte unit
-// `unit` of row `row` + i * STEP to its place (a thread's slot and, with it, its
-// unit are the same in all its rows).
+// A block's loads of a tile of 64 rows.  Load i of a wave brings ROWS rows from
+// first_row + i * STEP on; a lane brings 16-byte unit `unit` of row `lane_row` of
+// them (its slot and, with it, its unit are the same in all its rows).  Lanes
+// whose unit lies past dim load nothing: those places are cleared beforehand.
 template <int D, int THREADS> struct TileLoads {
-  static constexpr int BYTES = 64 * D * 2, COUNT = BYTES / (THREADS * 16), STEP = 64 / COUNT;
+  static constexpr int BYTES = 64 * D * 2, COUNT = BYTES / (THREADS * 16), STEP = 64 / COUNT, ROWS = WAVE / (D / 8);
   static_assert(COUNT > 0 && STEP % 16 == 0, "the swizzle repeats every 16 rows");
-  int row, unit;
-  bool live;  // the unit has components below dim; the others are zeros
+  int first_row, lane_row, unit;
+  bool live;
   uint32_t lds;  // where the wave's first load goes in the tile at LDS address 0
   __device__ __forceinline__ explicit TileLoads(int dim) {
-    row = threadIdx.x / (D / 8);
-    unit = (threadIdx.x % (D / 8)) ^ tile_swizzle<D>(row);
+    first_row = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE) * ROWS;
+    lane_row = lane_id() / (D / 8);
+    unit = (threadIdx.x % (D / 8)) ^ tile_swizzle<D>(first_row + lane_row);
     live = unit * 8 < dim;
     lds = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE) * 1024;
   }
-  // Bytes from one of this lane's rows to its next, 0 for a lane that loads zeros.
-  __device__ __forceinline__ int64_t step(int64_t row_stride) const { return live ? row_stride * (2 * STEP) : 0; }
-  // Where this lane starts in rows beginning at `first`.
-  __device__ __forceinline__ const char *start(const uint16_t *first, int64_t row_stride) const {
-    return live ? (const char *)(first + row * row_stride + unit * 8) : (const char *)&g_zeros;
+  // The row load i of this lane brings.
+  __device__ __forceinline__ int row(int i) const { return first_row + lane_row + i * STEP; }
+  // This lane's place from its load's first row on.
+  __device__ __forceinline__ uint32_t offset(int64_t row_stride) const {
+    return (uint32_t)lane_row * (uint32_t)row_stride * 2 + unit * 16;
   }
-  __device__ __forceinline__ void load(const void *src, uint32_t tile, int i) const {
-    load_to_lds(src, tile + lds + i * (THREADS * 16));
+  __device__ __forceinline__ uint32_t place(uint32_t tile, int i) const { return tile + lds + i * (THREADS * 16); }
+  // A whole tile of equally spaced rows.
+  __device__ __forceinline__ void load(const uint16_t *first, int64_t row_stride, uint32_t offset, uint32_t tile) const {
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < COUNT; i++) load_to_lds(first + (int64_t)(first_row + i * STEP) * row_stride, offset, place(tile, i));
+    }
   }
+  // The same where only the first `rows` are there: the rest are zeros.
+  __device__ __forceinline__ void load(const uint16_t *first, int64_t row_stride, int rows, uint32_t tile) const {
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < COUNT; i++) load(first + row(i) * row_stride, row(i) < rows, tile, i);
+    }
+  }
+  // Load i from this lane's row, or zeros.
   __device__ __forceinline__ void load(const uint16_t *row_data, bool there, uint32_t tile, int i) const {
-    const void *src = there && live ? (const void *)(row_data + unit * 8) : (const void *)&g_zeros;
-    load_to_lds(src, tile + lds + i * (THREADS * 16));
+    load_to_lds(there ? (const void *)(row_data + unit * 8) : (const void *)&g_zeros, place(tile, i));
   }
 };
+// Clears `bytes` of LDS (a multiple of 16) where units past dim would stay as they
+// are; a barrier comes before the first loads.
+template <int D> __device__ __forceinline__ void clear_unloaded(unsigned char *lds, int bytes, int dim) {
+  if (dim == D) return;
+  for (int i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16) *reinterpret_cast<uint4 *>(lds + i) = uint4{0, 0, 0, 0};
+  __syncthreads();
+}
+
+// Eight components of a row from c on, zeros past dim.  (A load under a condition
+// would be waited for before the next is issued.)
+__device__ __forceinline__ uint4 load_unit(const uint16_t *row, int c, int dim) {
+  const uint4 x = *reinterpret_cast<const uint4 *>(row + (c < dim ? c : 0));
+  return c < dim ? x : uint4{0, 0, 0, 0};
+}
+
+// The compiler's own loads into x have arrived here.  Left to itself it waits for
+// them where x is first used, and inside a loop with every load in flight.
+template <int N> __device__ __forceinline__ void arrived(uint4 (&x)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; i++) asm volatile("" : "+v"(x[i].x), "+v"(x[i].y), "+v"(x[i].z), "+v"(x[i].w));
+}
 
 // Maximum (sum) over the lanes 16 and 32 apart, and over lanes 32 apart alone.
 // A swap of a register with itself leaves the even rows (the lower half) in one
@@ -324,11 +396,15 @@ inline bool heads_span_ok(int64_t rows, int64_t heads, int64_t dim, const fa_hea
   return last < ((__int128)1 << 61);
 }
 
+// Lanes reach the rows of a load by 32-bit offsets.
+constexpr int64_t AT_MOST_STRIDE = (int64_t)1 << 27;
+
 inline int check_heads(const fa_heads *x, int64_t rows, int64_t heads, int64_t dim, bool written) {
   if (x == nullptr || (x->data == nullptr && rows > 0)) return FA_EINVAL;
   if (x->row_stride < 0 || x->head_stride < 0) return FA_EINVAL;
   if (!is_aligned(x->data, 16) || x->row_stride % 8 != 0 || x->head_stride % 8 != 0) return FA_EALIGN;
   if (!heads_span_ok(rows, heads, dim, x)) return FA_EINVAL;
+  if (rows > 1 && x->row_stride >= AT_MOST_STRIDE) return FA_ENOTSUP;
   if (written) {
     // One of the two dimensions lies inside a step of the other.
     const __int128 r = x->row_stride, h = x->head_stride;

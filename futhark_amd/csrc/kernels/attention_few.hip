@@ -179,13 +179,6 @@ __device__ __forceinline__ FewUnit *few_unit(const AttentionArgs &a, int rows, i
   return (FewUnit *)(few_units(a, rows, d) + 2);
 }
 
-template <int N> __device__ __forceinline__ void wait_older_than() {
-  // all but the N youngest loads have arrived
-  if constexpr (N == 16) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-  else asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-  static_assert(N == 16 || N == 8, "loads of a tile");
-}
-
 // A wave's work on a unit: tiles from .. to - 1 of a sequence's keys for some of
 // its tokens and one key head.
 struct FewRun {
@@ -270,12 +263,9 @@ __device__ __forceinline__ void few_attend(const AttentionArgs &a, unsigned char
     limit[ct] = u.first_limit + row / a.group;
     const uint16_t *src = a.q.at(u.row + row / a.group, u.head * a.group + row % a.group);
 #pragma unroll
-    for (int k = 0; k < D / 32; k++) {
-      const int c = 32 * k + 8 * quarter;
-      q[ct][k] = c < a.dim ? *reinterpret_cast<const uint4 *>(src + c) : uint4{0, 0, 0, 0};
-    }
+    for (int k = 0; k < D / 32; k++) q[ct][k] = load_unit(src, 32 * k + 8 * quarter, a.dim);
   }
-  #pragma unroll
+#pragma unroll
   for (int ct = 0; ct < CT; ct++) {
     r.top[ct] = -INFINITY;
     r.sum[ct] = 0.0f;
@@ -294,8 +284,8 @@ __device__ __forceinline__ void few_attend(const AttentionArgs &a, unsigned char
       for (int i = 0; i < LOADS; i++) {
         const int64_t off = ((int64_t)__builtin_amdgcn_readlane(id, i * LOAD_ROWS) * a.kv_heads + u.head) * head_bytes +
                             ((key0 + i * LOAD_ROWS) & slot_mask) * row_bytes;
-        stream_to_lds(a.pages.k, off, lane_at[i % 4], dst + i * (WAVE * 16));
-        stream_to_lds(a.pages.v, off, lane_at[i % 4], dst + L::HALF + i * (WAVE * 16));
+        stream_to_lds((const char *)a.pages.k + off, lane_at[i % 4], dst + i * (WAVE * 16));
+        stream_to_lds((const char *)a.pages.v + off, lane_at[i % 4], dst + L::HALF + i * (WAVE * 16));
       }
       return;
     }
@@ -314,19 +304,14 @@ __device__ __forceinline__ void few_attend(const AttentionArgs &a, unsigned char
 
   // In flight while tile t is multiplied: the page numbers of t + 2 (older),
   // then the 2 LOADS loads of tile t + 1.
-  // The queries have arrived before the loop: inside it the compiler would wait for
-  // them, and with them for the tiles in flight, in every round.
 #pragma unroll
-  for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-    for (int k = 0; k < D / 32; k++)
-      asm volatile("" : "+v"(q[ct][k].x), "+v"(q[ct][k].y), "+v"(q[ct][k].z), "+v"(q[ct][k].w));
+  for (int ct = 0; ct < CT; ct++) arrived(q[ct]);
   wait_loads();
   fetch(u.from);
   fetch_ids(u.from + 2);
   if (u.from + 1 < u.to) fetch(u.from + 1);
   for (int t = u.from; t < u.to; t++) {
-    if (t + 1 < u.to) wait_older_than<2 * LOADS>();
+    if (t + 1 < u.to) wait_but<2 * LOADS>();
     else wait_loads();
     unsigned char *kt = mine + (t & 1) * L::STAGE;
     const int key0 = t * FEW_KEYS;

@@ -29,10 +29,7 @@ struct GradArgs {
 
 template <int D> __device__ __forceinline__ void load_operand(uint4 (&x)[D / 16], const uint16_t *src, int dim) {
 #pragma unroll
-  for (int s = 0; s < D / 16; s++) {
-    const int c = s * 16 + (lane_id() >> 5) * 8;
-    x[s] = c < dim ? *reinterpret_cast<const uint4 *>(src + c) : uint4{0, 0, 0, 0};
-  }
+  for (int s = 0; s < D / 16; s++) x[s] = load_unit(src, s * 16 + (lane_id() >> 5) * 8, dim);
 }
 template <int D> __device__ __forceinline__ void clear(f32x16 (&x)[D / 32]) {
 #pragma unroll
@@ -89,12 +86,17 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, 2) void atten
   const TileLoads<D, AG_THREADS> loads(a.dim);
   const TileReads<D> reads;
   const uint32_t lds_base = lds_address(lds);
+  clear_unloaded<D>(lds, 4 * TILE, a.dim);
+  const uint32_t k_offset = loads.offset(a.k.row_stride), v_offset = loads.offset(a.v.row_stride);
   const auto fetch = [&](int key0, int stage) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < loads.COUNT; i++) {
-      const int key = key0 + loads.row + i * loads.STEP;
-      loads.load(a.k.at(t.first2 + key, kv_head), key < keys, lds_base + stage * (2 * TILE), i);
-      loads.load(a.v.at(t.first2 + key, kv_head), key < keys, lds_base + stage * (2 * TILE) + TILE, i);
+    const uint16_t *k = a.k.at(t.first2 + key0, kv_head), *v = a.v.at(t.first2 + key0, kv_head);
+    const uint32_t k_tile = lds_base + stage * (2 * TILE), v_tile = k_tile + TILE;
+    if (key0 + AG_STEP <= keys) {
+      loads.load(k, a.k.row_stride, k_offset, k_tile);
+      loads.load(v, a.v.row_stride, v_offset, v_tile);
+    } else {
+      loads.load(k, a.k.row_stride, keys - key0, k_tile);
+      loads.load(v, a.v.row_stride, keys - key0, v_tile);
     }
   };
 
@@ -117,6 +119,8 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, 2) void atten
   // A row that sees nothing has lse = -inf; its weights must come out as zero.
   const float lse = a.lse[at * a.heads + head];
   const float shift = lse == -INFINITY ? INFINITY : lse * LOG2E, scale_log2 = a.scale * LOG2E;
+  arrived(q);
+  arrived(g);
   f32x16 dq[D / 32];
   clear<D>(dq);
 
@@ -247,6 +251,8 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 
     const int64_t at = t.first + (key + 32 * x < k_len ? key + 32 * x : k_len - 1);
     load_operand<D>(k[x], a.k.at(at, kv_head), a.dim);
     load_operand<D>(v[x], a.v.at(at, kv_head), a.dim);
+    arrived(k[x]);
+    arrived(v[x]);
     clear<D>(dk[x]);
     clear<D>(dv[x]);
   }
@@ -254,6 +260,7 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 
   const TileLoads<D, AG_THREADS> loads(a.dim);
   const TileReads<D> reads;
   const uint32_t lds_base = lds_address(lds);
+  clear_unloaded<D>(lds, 2 * STAGE, a.dim);
   // Row r of a step is token r / heads, head r % heads of the step's tokens and chunk.
   const auto place = [&](int r, int64_t step, int &token, int &head) __attribute__((always_inline)) {
     const int chunk = (int)(step / steps.per_chunk);
@@ -266,9 +273,11 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 
 #pragma unroll
     for (int i = 0; i < loads.COUNT; i++) {
       int token, head;
-      const bool there = place(loads.row + i * loads.STEP, step, token, head);
-      loads.load(a.q.at(t.first2 + token, head), there, lds_base + stage * STAGE, i);
-      loads.load(a.dout.at(t.first2 + token, head), there, lds_base + stage * STAGE + TILE, i);
+      const bool there = place(loads.row(i), step, token, head);
+      if (loads.live) {
+        loads.load(a.q.at(t.first2 + token, head), there, lds_base + stage * STAGE, i);
+        loads.load(a.dout.at(t.first2 + token, head), there, lds_base + stage * STAGE + TILE, i);
+      }
     }
   };
   // Of every row: log2 of the sum (infinite where there is no row or it sees
