@@ -200,6 +200,22 @@ struct RowSteps {
   }
   __device__ __forceinline__ int64_t count() const { return (int64_t)chunks * per_chunk; }
 };
+// A step: its first token and the first of its heads in the group.
+struct StepAt {
+  int token, head;
+  __device__ __forceinline__ StepAt(const RowSteps &r, int64_t step) {
+    const int chunk = r.chunks == 1 ? 0 : (int)(step / r.per_chunk);
+    token = r.first + (int)(step - (int64_t)chunk * r.per_chunk) * r.tokens;
+    head = chunk * r.heads;
+  }
+  __device__ __forceinline__ void advance(const RowSteps &r, int q_len) {
+    token += r.tokens;
+    if (token >= q_len) {
+      token = r.first;
+      head += r.heads;
+    }
+  }
+};
 __device__ __forceinline__ int parts_of(int64_t steps, int most) {
   const int64_t worth = (steps + AG_PART_STEPS - 1) / AG_PART_STEPS;
   return worth < 1 ? 1 : (worth < most ? (int)worth : most);
@@ -209,209 +225,252 @@ __device__ __forceinline__ int first_token(const GradArgs &a, int key0, int q_le
   const int from = a.causal ? key0 - (k_len - q_len) : 0;
   return from > 0 ? from : 0;
 }
-// Keys a block of the second kernel owns, PER_WAVE times 32 a wave (twice 32 for
-// D = 128 does not fit the registers: 1.6 ms instead of 0.66 ms on 7201 rows).
-template <int D> struct KeyTile {
-  static constexpr int PER_WAVE = 1, KEYS = 32 * PER_WAVE * AG_WAVES;
-};
-// Where part `part` of a key tile leaves its sums: dk then dv, [KEYS][D] each.
+constexpr int AG_KEYS = 32 * AG_WAVES;  // keys a block of the second kernel owns
+// Where part `part` of a key tile leaves its sums: dk then dv, [AG_KEYS][D] each.
 template <int D> __device__ __forceinline__ float *part_sums(const GradArgs &a, int64_t tile, int part) {
-  return a.part + (tile * a.parts + part) * (2 * KeyTile<D>::KEYS * D);
+  return a.part + (tile * a.parts + part) * (2 * AG_KEYS * D);
 }
+// Stages of 64 query rows in LDS: Q, dO, and of every row three numbers.  D = 128
+// runs one wave a SIMD and takes three stages, so that rows have a whole step to
+// arrive.
+template <int D> struct GradStage {
+  static constexpr int TILE = TileLoads<D, AG_THREADS>::BYTES, BYTES = 2 * TILE + 3 * AG_STEP * 4, COUNT = 3;
+};
 
 // dk and dv.  A block owns 128 keys of a key head, a wave 32 of them with K and V
 // as right operands in registers, and walks the query rows that see them, all
-// heads of the group, 64 a step:
+// heads of the group, 64 a step and 32 at a time:
 //   S = Q K^T, dP = dO V^T, dS = P (dP - D), dV^T += dO^T P, dK^T += Q^T dS,
-// with Q and dO read from one tile each by rows and by columns.  The keys at the
-// start of a long sequence are seen by all its rows: their rows are split over
-// `parts` blocks, whose sums a second kernel adds in order.
+// with Q and dO read from one tile each by rows and by columns.  The products S
+// and dP of the next 32 rows are issued in turn with the weights of the last, as
+// the order in the source fixes.  The keys at the start of a long sequence are
+// seen by all its rows: their rows are split over `parts` blocks, whose sums a
+// second kernel adds in order.
 template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 : 2) void attention_dkv_kernel(GradArgs a) {
-  constexpr int TILE = TileLoads<D, AG_THREADS>::BYTES, STAGE = 2 * TILE + 3 * AG_STEP * 4;
-  constexpr int KT = KeyTile<D>::PER_WAVE, KEYS = KeyTile<D>::KEYS;
+  using L = GradStage<D>;
+  constexpr int TILE = L::TILE, PRODUCTS = D / 8;  // of S and dP together, and of dV and dK
+  constexpr int AHEAD = 3;                         // operands read before their product
   extern __shared__ __align__(16) unsigned char lds[];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), half = lane >> 5;
   const int kv_head = blockIdx.x % a.kv_heads, part = blockIdx.y;
   SegTile t;
-  if (!find_tile(a.k_offsets, a.k_lens, a.k_rows, a.q_offsets, a.q_lens, a.q_rows, a.m, KEYS,
+  if (!find_tile(a.k_offsets, a.k_lens, a.k_rows, a.q_offsets, a.q_lens, a.q_rows, a.m, AG_KEYS,
                  blockIdx.x / a.kv_heads, t))
     return;
-  const int k_len = (int)t.len, q_len = (int)t.len2, key0 = (int)t.tile * KEYS, behind = k_len - q_len;
+  const int k_len = (int)t.len, q_len = (int)t.len2, key0 = (int)t.tile * AG_KEYS, behind = k_len - q_len;
   const RowSteps steps(a.group, q_len, first_token(a, key0, q_len, k_len));
   const int parts = parts_of(steps.count(), a.parts);
   if (part >= parts) return;
   const int64_t from = steps.count() * part / parts, to = steps.count() * (part + 1) / parts;
 
-  const int key = key0 + wave * (32 * KT) + (lane & 31);  // and 32 further on
-  const int wave_last = key0 + (wave + 1) * (32 * KT) - 1;
-  uint4 k[KT][D / 16], v[KT][D / 16];
-  f32x16 dk[KT][D / 32], dv[KT][D / 32];
-#pragma unroll
-  for (int x = 0; x < KT; x++) {
-    const int64_t at = t.first + (key + 32 * x < k_len ? key + 32 * x : k_len - 1);
-    load_operand<D>(k[x], a.k.at(at, kv_head), a.dim);
-    load_operand<D>(v[x], a.v.at(at, kv_head), a.dim);
-    arrived(k[x]);
-    arrived(v[x]);
-    clear<D>(dk[x]);
-    clear<D>(dv[x]);
+  const int key = key0 + wave * 32 + (lane & 31);
+  uint4 k[D / 16], v[D / 16];
+  {
+    const int64_t at = t.first + (key < k_len ? key : k_len - 1);
+    load_operand<D>(k, a.k.at(at, kv_head), a.dim);
+    load_operand<D>(v, a.v.at(at, kv_head), a.dim);
   }
+  arrived(k);
+  arrived(v);
+  f32x16 dk[D / 32], dv[D / 32];
+  clear<D>(dk);
+  clear<D>(dv);
 
   const TileLoads<D, AG_THREADS> loads(a.dim);
   const TileReads<D> reads;
   const uint32_t lds_base = lds_address(lds);
-  clear_unloaded<D>(lds, 2 * STAGE, a.dim);
-  // Row r of a step is token r / heads, head r % heads of the step's tokens and chunk.
-  const auto place = [&](int r, int64_t step, int &token, int &head) __attribute__((always_inline)) {
-    const int chunk = (int)(step / steps.per_chunk);
-    token = steps.first + (int)(step - (int64_t)chunk * steps.per_chunk) * steps.tokens + r / steps.heads;
-    const int h = chunk * steps.heads + r % steps.heads;
-    head = kv_head * a.group + h;
-    return r < steps.tokens * steps.heads && h < a.group && token < q_len;
-  };
-  const auto fetch = [&](int64_t step, int stage) __attribute__((always_inline)) {
+  for (int i = threadIdx.x * 16; i < L::COUNT * L::BYTES; i += AG_THREADS * 16)  // rows and units that are never loaded
+    *reinterpret_cast<uint4 *>(lds + i) = uint4{0, 0, 0, 0};
+  __syncthreads();
+  // Row r of a step is token r / heads, head r % heads of the step's.
+  const bool near = ((int64_t)AG_STEP * (a.q.row_stride + a.dout.row_stride) +
+                     steps.heads * (a.q.head_stride + a.dout.head_stride)) < (1 << 30);
+  uint32_t q_at[loads.COUNT], g_at[loads.COUNT];  // of this lane's rows, from the step's first
+  bool mine[loads.COUNT];
 #pragma unroll
-    for (int i = 0; i < loads.COUNT; i++) {
-      int token, head;
-      const bool there = place(loads.row(i), step, token, head);
-      if (loads.live) {
-        loads.load(a.q.at(t.first2 + token, head), there, lds_base + stage * STAGE, i);
-        loads.load(a.dout.at(t.first2 + token, head), there, lds_base + stage * STAGE + TILE, i);
-      }
+  for (int i = 0; i < loads.COUNT; i++) {
+    const int r = loads.row(i);
+    mine[i] = loads.live && r < steps.tokens * steps.heads;
+    q_at[i] = (uint32_t)(r / steps.heads * a.q.row_stride + r % steps.heads * a.q.head_stride + loads.unit * 8) * 2;
+    g_at[i] = (uint32_t)(r / steps.heads * a.dout.row_stride + r % steps.heads * a.dout.head_stride + loads.unit * 8) * 2;
+  }
+  const auto fetch = [&](const StepAt &s, int stage) __attribute__((always_inline)) {
+    const uint32_t q_tile = lds_base + stage * L::BYTES, g_tile = q_tile + TILE;
+    const int head = kv_head * a.group + s.head;
+    const uint16_t *q0 = a.q.at(t.first2 + s.token, head), *g0 = a.dout.at(t.first2 + s.token, head);
+    if (near && s.token + steps.tokens <= q_len && s.head + steps.heads <= a.group) {
+#pragma unroll
+      for (int i = 0; i < loads.COUNT; i++)
+        if (mine[i]) {
+          load_to_lds(q0, q_at[i], loads.place(q_tile, i));
+          load_to_lds(g0, g_at[i], loads.place(g_tile, i));
+        }
+    } else {
+#pragma unroll
+      for (int i = 0; i < loads.COUNT; i++)
+        if (mine[i]) {
+          const int token = loads.row(i) / steps.heads, h = loads.row(i) % steps.heads;
+          const bool there = s.token + token < q_len && s.head + h < a.group;
+          loads.load(a.q.at(t.first2 + s.token + token, head + h), there, q_tile, i);
+          loads.load(a.dout.at(t.first2 + s.token + token, head + h), there, g_tile, i);
+        }
     }
   };
   // Of every row: log2 of the sum (infinite where there is no row or it sees
   // nothing: weights become zero), D, and the last key it sees.
   float row_shift = 0.0f, row_delta = 0.0f;
   int row_last = 0;
-  const auto fetch_row = [&](int64_t step) __attribute__((always_inline)) {
+  const int my_token = threadIdx.x / steps.heads, my_head = threadIdx.x % steps.heads;
+  const auto fetch_row = [&](const StepAt &s) __attribute__((always_inline)) {
     if (threadIdx.x < AG_STEP) {
-      int token, head;
-      const bool there = place(threadIdx.x, step, token, head);
-      const int64_t at = there ? (t.first2 + token) * a.heads + head : 0;
-      const float lse = there ? a.lse[at] : -INFINITY;
-      row_shift = lse == -INFINITY ? INFINITY : lse * LOG2E;
-      row_delta = there ? a.delta[at] : 0.0f;
-      row_last = a.causal ? token + behind : INT32_MAX;
+      const bool there = my_token < steps.tokens && s.token + my_token < q_len && s.head + my_head < a.group;
+      const int64_t at = there ? (t.first2 + s.token + my_token) * a.heads + kv_head * a.group + s.head + my_head : 0;
+      row_shift = a.lse[at];
+      row_delta = a.delta[at];
+      row_last = !there ? INT32_MIN : a.causal ? s.token + my_token + behind : INT32_MAX;
     }
   };
   const auto put_row = [&](int stage) __attribute__((always_inline)) {
     if (threadIdx.x < AG_STEP) {
-      float *x = reinterpret_cast<float *>(lds + stage * STAGE + 2 * TILE);
-      x[threadIdx.x] = row_shift;
-      x[AG_STEP + threadIdx.x] = row_delta;
+      float *x = reinterpret_cast<float *>(lds + stage * L::BYTES + 2 * TILE);
+      const bool none = row_last == INT32_MIN || row_shift == -INFINITY;
+      x[threadIdx.x] = none ? INFINITY : row_shift * LOG2E;
+      x[AG_STEP + threadIdx.x] = none ? 0.0f : row_delta;
       reinterpret_cast<int *>(x)[2 * AG_STEP + threadIdx.x] = row_last;
     }
   };
   const float scale_log2 = a.scale * LOG2E;
-  if (from < to) {
-    fetch_row(from);
-    fetch(from, 0);
-    put_row(0);
-  }
-  int stage = 0;
-  for (int64_t step = from; step < to; step++, stage ^= 1) {
-    wait_loads();
-    __syncthreads();
-    if (step + 1 < to) {
-      fetch_row(step + 1);
-      fetch(step + 1, stage ^ 1);
-    }
-    const unsigned char *qt = lds + stage * STAGE, *gt = qt + TILE;
-    const float *shifts = reinterpret_cast<const float *>(qt + 2 * TILE), *deltas = shifts + AG_STEP;
+
+  // Operand `i` of the products S and dP (in turn) of 32 rows, and of dV and dK.
+  const auto by_rows = [&](const unsigned char *tile, int b, auto i) __attribute__((always_inline)) {
+    return reads.rows(tile + (i % 2 ? TILE : 0), b, i / 2);
+  };
+  const auto by_columns = [&](const unsigned char *tile, int b, auto i) __attribute__((always_inline)) {
+    constexpr int c = i / (D / 16), dt = i % (D / 16) / 2;
+    return reads.columns(tile + (i % 2 ? 0 : TILE), b + 16 * c, dt);
+  };
+  const auto products = [&](const unsigned char *tile, int b, f32x16 &s, f32x16 &dp) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 16; i++) s[i] = dp[i] = 0.0f;
+    static_for<PRODUCTS>([&](auto i) __attribute__((always_inline)) {
+      if constexpr (i % 2 == 0) s = E::mfma(by_rows(tile, b, i), k[i / 2], s);
+      else dp = E::mfma(by_rows(tile, b, i), v[i / 2], dp);
+    });
+  };
+  // 32 rows (`tile`, from b on) whose products are s and dp; and the products of
+  // the next 32 (`next_tile`, from next_b on).
+  const auto half_step = [&](const unsigned char *tile, int b, f32x16 &s, f32x16 &dp, const unsigned char *next_tile,
+                             int next_b, f32x16 &next_s, f32x16 &next_dp, auto masked) __attribute__((always_inline)) {
+    const float *shifts = reinterpret_cast<const float *>(tile + 2 * TILE) + b + 4 * half, *deltas = shifts + AG_STEP;
     const int *lasts = reinterpret_cast<const int *>(deltas + AG_STEP);
-    // the step's first row sees least
-    const bool masked = a.causal && lasts[0] < wave_last;
+    uint4 x[AHEAD];
+    uint32_t pw[8], pds[8];
+    f32x4 shift[4], delta[4];
+    int4 last[4];
 #pragma unroll
-    for (int b = 0; b < AG_STEP; b += 32) {
-      f32x16 p[KT], dp[KT];
-#pragma unroll
-      for (int x = 0; x < KT; x++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) p[x][i] = dp[x][i] = 0.0f;
-#pragma unroll
-      for (int s = 0; s < D / 16; s++) {
-        const uint4 qr = reads.rows(qt, b, s), gr = reads.rows(gt, b, s);
-#pragma unroll
-        for (int x = 0; x < KT; x++) p[x] = E::mfma(qr, k[x][s], p[x]);
-#pragma unroll
-        for (int x = 0; x < KT; x++) dp[x] = E::mfma(gr, v[x][s], dp[x]);
-      }
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const f32x4 shift = *reinterpret_cast<const f32x4 *>(shifts + b + 8 * j + 4 * half);
-#pragma unroll
-        for (int x = 0; x < KT; x++)
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            p[x][4 * j + i] = __builtin_amdgcn_exp2f(fmaf(p[x][4 * j + i], scale_log2, -shift[i]));
-      }
-      if (masked) {
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const int4 last = *reinterpret_cast<const int4 *>(lasts + b + 8 * j + 4 * half);
-#pragma unroll
-          for (int x = 0; x < KT; x++) {
-            if (key + 32 * x > last.x) p[x][4 * j] = 0.0f;
-            if (key + 32 * x > last.y) p[x][4 * j + 1] = 0.0f;
-            if (key + 32 * x > last.z) p[x][4 * j + 2] = 0.0f;
-            if (key + 32 * x > last.w) p[x][4 * j + 3] = 0.0f;
-          }
-        }
-      }
-#pragma unroll
-      for (int c = 0; c < 2; c++) {
-        uint4 pw[KT], pds[KT];
-        f32x4 delta[2];
-#pragma unroll
-        for (int j = 0; j < 2; j++)
-          delta[j] = *reinterpret_cast<const f32x4 *>(deltas + b + 16 * c + 8 * j + 4 * half);
-#pragma unroll
-        for (int x = 0; x < KT; x++) {
-          f32x8 w, ds;
-#pragma unroll
-          for (int i = 0; i < 8; i++) {
-            w[i] = p[x][8 * c + i];
-            ds[i] = w[i] * (dp[x][8 * c + i] - delta[i >> 2][i & 3]);
-          }
-          pw[x] = E::pack(w);
-          pds[x] = E::pack(ds);
-        }
-#pragma unroll
-        for (int dt = 0; dt < D / 32; dt++) {
-          const uint4 gc = reads.columns(gt, b + 16 * c, dt), qc = reads.columns(qt, b + 16 * c, dt);
-#pragma unroll
-          for (int x = 0; x < KT; x++) dv[x][dt] = E::mfma(gc, pw[x], dv[x][dt]);
-#pragma unroll
-          for (int x = 0; x < KT; x++) dk[x][dt] = E::mfma(qc, pds[x], dk[x][dt]);
-        }
-      }
+    for (int j = 0; j < 4; j++) {
+      shift[j] = *reinterpret_cast<const f32x4 *>(shifts + 8 * j);
+      delta[j] = *reinterpret_cast<const f32x4 *>(deltas + 8 * j);
+      if constexpr (decltype(masked)::value) last[j] = *reinterpret_cast<const int4 *>(lasts + 8 * j);
     }
-    if (step + 1 < to) put_row(stage ^ 1);
+    static_for<AHEAD>([&](auto i) __attribute__((always_inline)) { x[i] = by_rows(next_tile, next_b, i); });
+#pragma unroll
+    for (int i = 0; i < 16; i++) next_s[i] = next_dp[i] = 0.0f;
+    __builtin_amdgcn_sched_barrier(0);
+    static_for<PRODUCTS>([&](auto i) __attribute__((always_inline)) {
+      const uint4 now = x[i % AHEAD];
+      if constexpr (i + AHEAD < PRODUCTS) x[i % AHEAD] = by_rows(next_tile, next_b, std::integral_constant<int, i + AHEAD>());
+      else x[i % AHEAD] = by_columns(tile, b, std::integral_constant<int, i + AHEAD - PRODUCTS>());
+      if constexpr (i % 2 == 0) next_s = E::mfma(now, k[i / 2], next_s);
+      else next_dp = E::mfma(now, v[i / 2], next_dp);
+      constexpr int SHARE = 16 / PRODUCTS;
+      static_for<SHARE>([&](auto j) __attribute__((always_inline)) {
+        constexpr int e = i * SHARE + j;
+        float p = __builtin_amdgcn_exp2f(fmaf(s[e], scale_log2, -shift[e / 4][e % 4]));
+        if constexpr (decltype(masked)::value) {
+          const int l = e % 4 == 0 ? last[e / 4].x : e % 4 == 1 ? last[e / 4].y : e % 4 == 2 ? last[e / 4].z : last[e / 4].w;
+          p = key > l ? 0.0f : p;
+        }
+        s[e] = p;
+        dp[e] = p * (dp[e] - delta[e / 4][e % 4]);
+        if constexpr (e % 2 == 1) {
+          pw[e / 2] = E::pack(s[e - 1], s[e]);
+          pds[e / 2] = E::pack(dp[e - 1], dp[e]);
+        }
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    static_for<PRODUCTS>([&](auto i) __attribute__((always_inline)) {
+      constexpr int c = i / (D / 16), dt = i % (D / 16) / 2, at = (i + PRODUCTS) % AHEAD;
+      const uint4 now = x[at];
+      if constexpr (i + AHEAD < PRODUCTS) x[at] = by_columns(tile, b, std::integral_constant<int, i + AHEAD>());
+      if constexpr (i % 2 == 0) dv[dt] = E::mfma(now, uint4{pw[4 * c], pw[4 * c + 1], pw[4 * c + 2], pw[4 * c + 3]}, dv[dt]);
+      else dk[dt] = E::mfma(now, uint4{pds[4 * c], pds[4 * c + 1], pds[4 * c + 2], pds[4 * c + 3]}, dk[dt]);
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+
+  // While step i is worked on its successor's rows are in LDS (from the middle of
+  // the step on) and those of the next but one on their way.
+  StepAt ahead(steps, from);
+  int stage = 0;  // of the step
+  const auto stage_after = [&](int n) { return stage + n < L::COUNT ? stage + n : stage + n - L::COUNT; };
+  if (from < to) {
+    fetch_row(ahead);
+    fetch(ahead, 0);
+    put_row(0);
+    ahead.advance(steps, q_len);
+    if (from + 1 < to) {
+      fetch_row(ahead);
+      fetch(ahead, 1);
+      ahead.advance(steps, q_len);
+    }
+    wait_loads();
+    block_barrier();
+    f32x16 s0, dp0, s1, dp1;
+    products(lds, 0, s0, dp0);
+    const auto whole_step = [&](int64_t step, auto masked) __attribute__((always_inline)) {
+      const unsigned char *tile = lds + stage * L::BYTES, *next = lds + stage_after(1) * L::BYTES;
+      half_step(tile, 0, s0, dp0, tile, 32, s1, dp1, masked);
+      put_row(stage_after(1));
+      wait_loads();
+      block_barrier();
+      if (step + 2 < to) {
+        fetch_row(ahead);
+        fetch(ahead, stage_after(2));
+        ahead.advance(steps, q_len);
+      }
+      // (after the last step these products are of what the stage holds, unused)
+      half_step(tile, 32, s1, dp1, next, 0, s0, dp0, masked);
+      stage = stage_after(1);
+    };
+    // The first steps of a causal tile see only some of its keys.
+    const int64_t border =
+        !a.causal ? 0 : steps.chunks > 1 ? steps.count() : (key0 + AG_KEYS - 1 - behind - steps.first + steps.tokens - 1) / steps.tokens;
+    int64_t step = from;
+    for (; step < to && step < border; step++) whole_step(step, std::true_type());
+    for (; step < to; step++) whole_step(step, std::false_type());
   }
+  if (parts > 1) {
+    float *dst = part_sums<D>(a, blockIdx.x, part) + (key - key0) * D;
 #pragma unroll
-  for (int x = 0; x < KT; x++) {
-    if (parts > 1) {
-      float *dst = part_sums<D>(a, blockIdx.x, part) + (key - key0 + 32 * x) * D;
+    for (int dt = 0; dt < D / 32; dt++)
 #pragma unroll
-      for (int dt = 0; dt < D / 32; dt++)
-#pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-          const int d = dt * 32 + 2 * i + 4 * half;
-          const f32x16 &y = dk[x][dt], &z = dv[x][dt];
-          *reinterpret_cast<f32x4 *>(dst + d) = f32x4{y[i], y[i + 1], y[i + 2], y[i + 3]};
-          *reinterpret_cast<f32x4 *>(dst + KEYS * D + d) = f32x4{z[i], z[i + 1], z[i + 2], z[i + 3]};
-        }
-    } else if (key + 32 * x < k_len) {
-      store_column<E, D>(dk[x], a.scale, a.dk.at(t.first + key + 32 * x, kv_head), a.dim);
-      store_column<E, D>(dv[x], 1.0f, a.dv.at(t.first + key + 32 * x, kv_head), a.dim);
-    }
+      for (int i = 0; i < 16; i += 4) {
+        const int d = dt * 32 + 2 * i + 4 * half;
+        *reinterpret_cast<f32x4 *>(dst + d) = f32x4{dk[dt][i], dk[dt][i + 1], dk[dt][i + 2], dk[dt][i + 3]};
+        *reinterpret_cast<f32x4 *>(dst + AG_KEYS * D + d) =
+            f32x4{dv[dt][i], dv[dt][i + 1], dv[dt][i + 2], dv[dt][i + 3]};
+      }
+  } else if (key < k_len) {
+    store_column<E, D>(dk, a.scale, a.dk.at(t.first + key, kv_head), a.dim);
+    store_column<E, D>(dv, 1.0f, a.dv.at(t.first + key, kv_head), a.dim);
   }
 }
 
 // Adds the parts of the split key tiles: a block an eighth of a tile, four components a thread.
 template <class E, int D> __global__ __launch_bounds__(AG_THREADS) void attention_dkv_join_kernel(GradArgs a) {
-  constexpr int KEYS = KeyTile<D>::KEYS;
+  constexpr int KEYS = AG_KEYS;
   const int kv_head = blockIdx.x % a.kv_heads;
   SegTile t;
   if (!find_tile(a.k_offsets, a.k_lens, a.k_rows, a.q_offsets, a.q_lens, a.q_rows, a.m, KEYS,
@@ -451,8 +510,7 @@ struct GradPlan {
 };
 static GradPlan grad_plan(int64_t q_rows, int64_t k_rows, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t m) {
   GradPlan p;
-  const int keys = head_dim <= 64 ? KeyTile<64>::KEYS : KeyTile<128>::KEYS;
-  p.tiles = most_tiles(k_rows, m, keys) * kv_heads;
+  p.tiles = most_tiles(k_rows, m, AG_KEYS) * kv_heads;
   const int64_t wanted = p.tiles > 0 ? ceil_div(8 * NUM_CUS_HINT, p.tiles) : 1;
   p.parts = (int)(wanted < 8 ? wanted : 8);
   // no tile has more steps than the rows of one head group make
@@ -461,15 +519,15 @@ static GradPlan grad_plan(int64_t q_rows, int64_t k_rows, int64_t heads, int64_t
   if (p.parts > ceil_div(steps, AG_PART_STEPS)) p.parts = (int)ceil_div(steps, AG_PART_STEPS);
   if (p.parts < 1) p.parts = 1;
   p.delta_bytes = (size_t)ceil_div(q_rows * heads, 4) * 16;
-  p.part_bytes = p.parts > 1 ? (size_t)p.tiles * p.parts * 2 * keys * (head_dim <= 64 ? 64 : 128) * sizeof(float) : 0;
+  p.part_bytes = p.parts > 1 ? (size_t)p.tiles * p.parts * 2 * AG_KEYS * (head_dim <= 64 ? 64 : 128) * sizeof(float) : 0;
   return p;
 }
 
 template <class E, int D> static int launch_grad(hipStream_t stream, const GradArgs &a, const GradPlan &p) {
-  constexpr int TILE = TileLoads<D, AG_THREADS>::BYTES, STAGE = 2 * TILE + 3 * AG_STEP * 4;
+  constexpr int TILE = TileLoads<D, AG_THREADS>::BYTES, LDS = GradStage<D>::BYTES * GradStage<D>::COUNT;
   const auto dkv = attention_dkv_kernel<E, D>;
   static const hipError_t raised =
-      hipFuncSetAttribute((const void *)dkv, hipFuncAttributeMaxDynamicSharedMemorySize, 2 * STAGE);
+      hipFuncSetAttribute((const void *)dkv, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   if (raised != hipSuccess) return (int)raised;
   const int64_t units = most_tiles(a.q_rows, a.m, AG_ROWS / a.group) * a.kv_heads;
   if (units > INT32_MAX || p.tiles > INT32_MAX) return FA_ENOTSUP;
@@ -479,7 +537,7 @@ template <class E, int D> static int launch_grad(hipStream_t stream, const GradA
     if (rc != 0) return rc;
   }
   if (p.tiles == 0) return 0;
-  dkv<<<dim3((unsigned)p.tiles, (unsigned)p.parts), AG_THREADS, 2 * STAGE, stream>>>(a);
+  dkv<<<dim3((unsigned)p.tiles, (unsigned)p.parts), AG_THREADS, LDS, stream>>>(a);
   const int rc = launch_status();
   if (rc != 0 || p.parts == 1) return rc;
   attention_dkv_join_kernel<E, D><<<dim3((unsigned)p.tiles, 8), AG_THREADS, 0, stream>>>(a);
