@@ -233,6 +233,13 @@ __device__ __forceinline__ void load_to_lds(const void *base, uint32_t offset, u
                "v"(offset), "s"(wave_address(base))
                : "memory", "m0");
 }
+// Four bytes a lane.
+__device__ __forceinline__ void load_word_to_lds(const void *src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(
+                   __builtin_amdgcn_readfirstlane(lds)),
+               "v"(src)
+               : "memory", "m0");
+}
 // And for data that is read once: the non-temporal policy (decoding 64 sequences
 // 98.8 -> 87.3 us, 5.9 TB/s).
 __device__ __forceinline__ void stream_to_lds(const void *base, uint32_t offset, uint32_t lds) {
@@ -244,13 +251,7 @@ __device__ __forceinline__ void stream_to_lds(const void *base, uint32_t offset,
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 
 // All but the N youngest loads have arrived.
-template <int N> __device__ __forceinline__ void wait_but() {
-  static_assert(N == 2 || N == 4 || N == 8 || N == 16, "loads of a tile");
-  if constexpr (N == 2) asm volatile("s_waitcnt vmcnt(2)" ::: "memory");
-  if constexpr (N == 4) asm volatile("s_waitcnt vmcnt(4)" ::: "memory");
-  if constexpr (N == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-  if constexpr (N == 16) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-}
+template <int N> __device__ __forceinline__ void wait_but() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 // A barrier that leaves younger loads in flight; what was read of LDS has arrived.
 __device__ __forceinline__ void block_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 

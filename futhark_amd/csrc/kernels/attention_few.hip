@@ -248,10 +248,7 @@ __device__ __forceinline__ void few_attend(const AttentionArgs &a, unsigned char
   const auto fetch_ids = [&](int t) __attribute__((always_inline)) {
     const int key = t * FEW_KEYS + lane < u.keys ? t * FEW_KEYS + lane : u.keys - 1;
     const int32_t *src = table + (key >> a.pages.page_shift);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(
-                     __builtin_amdgcn_readfirstlane(lds_base + L::IDS + (t & 3) * (WAVE * 4))),
-                 "v"(src)
-                 : "memory", "m0");
+    load_word_to_lds(src, lds_base + L::IDS + (t & 3) * (WAVE * 4));
   };
   fetch_ids(u.from);
   fetch_ids(u.from + 1);

@@ -16,7 +16,7 @@ constexpr int AG_PART_STEPS = 16;
 struct GradArgs {
   Heads q, k, v, out, dout, dq, dk, dv;
   const float *lse;
-  float *delta;  // [q_rows][heads]: D
+  float *shift, *delta;  // [q_rows][heads]: lse times log2(e), infinite for a row that sees nothing; D
   float *part;   // sums of the parts of split key tiles
   int64_t q_rows, k_rows;
   int heads, kv_heads, group, dim;
@@ -165,7 +165,10 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, 2) void atten
     delta = fold_halves(d, FAdd());
     __syncthreads();  // the tiles are read again from the start
   }
-  if (row < rows && half == 0) a.delta[at * a.heads + head] = delta;
+  if (row < rows && half == 0) {
+    a.shift[at * a.heads + head] = shift;
+    a.delta[at * a.heads + head] = delta;
+  }
   walk([&](const unsigned char *kt, int key0) __attribute__((always_inline)) {
 #pragma unroll
     for (int b = 0; b < AG_STEP; b += 32) {
@@ -230,12 +233,14 @@ constexpr int AG_KEYS = 32 * AG_WAVES;  // keys a block of the second kernel own
 template <int D> __device__ __forceinline__ float *part_sums(const GradArgs &a, int64_t tile, int part) {
   return a.part + (tile * a.parts + part) * (2 * AG_KEYS * D);
 }
-// Stages of 64 query rows in LDS: Q, dO, and of every row three numbers.  D = 128
-// runs one wave a SIMD and takes three stages, so that rows have a whole step to
-// arrive.
+// Stages of 64 query rows in LDS: Q, dO, and of every row its shift and D; so many
+// that rows have two steps to arrive.  Behind them, of every row of a step, which
+// of the step's tokens it belongs to.
 template <int D> struct GradStage {
-  static constexpr int TILE = TileLoads<D, AG_THREADS>::BYTES, BYTES = 2 * TILE + 3 * AG_STEP * 4, COUNT = 3;
+  static constexpr int TILE = TileLoads<D, AG_THREADS>::BYTES, BYTES = 2 * TILE + 2 * AG_STEP * 4, COUNT = 4;
+  static constexpr int TOKENS = COUNT * BYTES, LDS = TOKENS + AG_STEP * 4;
 };
+static __device__ const float g_infinity = INFINITY;  // the shift of a row that is not there (its D is 0)
 
 // dk and dv.  A block owns 128 keys of a key head, a wave 32 of them with K and V
 // as right operands in registers, and walks the query rows that see them, all
@@ -279,65 +284,58 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 
   const TileLoads<D, AG_THREADS> loads(a.dim);
   const TileReads<D> reads;
   const uint32_t lds_base = lds_address(lds);
-  for (int i = threadIdx.x * 16; i < L::COUNT * L::BYTES; i += AG_THREADS * 16)  // rows and units that are never loaded
-    *reinterpret_cast<uint4 *>(lds + i) = uint4{0, 0, 0, 0};
-  __syncthreads();
-  // Row r of a step is token r / heads, head r % heads of the step's.
-  const bool near = ((int64_t)AG_STEP * (a.q.row_stride + a.dout.row_stride) +
+  clear_unloaded<D>(lds, L::TOKENS, a.dim);
+  int *tokens_of = reinterpret_cast<int *>(lds + L::TOKENS);
+  if (threadIdx.x < AG_STEP) tokens_of[threadIdx.x] = threadIdx.x / steps.heads;
+  // Row r of a step is token r / heads, head r % heads of the step's.  The usual
+  // case: all rows of a step used, and within 32-bit offsets of its first.
+  const bool near = steps.tokens * steps.heads == AG_STEP &&
+                    ((int64_t)AG_STEP * (a.q.row_stride + a.dout.row_stride) +
                      steps.heads * (a.q.head_stride + a.dout.head_stride)) < (1 << 30);
-  uint32_t q_at[loads.COUNT], g_at[loads.COUNT];  // of this lane's rows, from the step's first
-  bool mine[loads.COUNT];
+  uint32_t q_at[loads.COUNT], g_at[loads.COUNT];
 #pragma unroll
   for (int i = 0; i < loads.COUNT; i++) {
     const int r = loads.row(i);
-    mine[i] = loads.live && r < steps.tokens * steps.heads;
     q_at[i] = (uint32_t)(r / steps.heads * a.q.row_stride + r % steps.heads * a.q.head_stride + loads.unit * 8) * 2;
     g_at[i] = (uint32_t)(r / steps.heads * a.dout.row_stride + r % steps.heads * a.dout.head_stride + loads.unit * 8) * 2;
   }
+  // Loads of a step: FETCHES of every wave, and one more of the first two.
+  constexpr int FETCHES = 2 * TileLoads<D, AG_THREADS>::COUNT;
+  const int my_token = lane / steps.heads, my_head = lane % steps.heads;
   const auto fetch = [&](const StepAt &s, int stage) __attribute__((always_inline)) {
     const uint32_t q_tile = lds_base + stage * L::BYTES, g_tile = q_tile + TILE;
     const int head = kv_head * a.group + s.head;
-    const uint16_t *q0 = a.q.at(t.first2 + s.token, head), *g0 = a.dout.at(t.first2 + s.token, head);
     if (near && s.token + steps.tokens <= q_len && s.head + steps.heads <= a.group) {
+      const uint16_t *q0 = a.q.at(t.first2 + s.token, head), *g0 = a.dout.at(t.first2 + s.token, head);
+      if (loads.live) {
 #pragma unroll
-      for (int i = 0; i < loads.COUNT; i++)
-        if (mine[i]) {
+        for (int i = 0; i < loads.COUNT; i++) {
           load_to_lds(q0, q_at[i], loads.place(q_tile, i));
           load_to_lds(g0, g_at[i], loads.place(g_tile, i));
         }
+      }
     } else {
 #pragma unroll
-      for (int i = 0; i < loads.COUNT; i++)
-        if (mine[i]) {
-          const int token = loads.row(i) / steps.heads, h = loads.row(i) % steps.heads;
-          const bool there = s.token + token < q_len && s.head + h < a.group;
+      for (int i = 0; i < loads.COUNT; i++) {
+        const int token = loads.row(i) / steps.heads, h = loads.row(i) % steps.heads;
+        const bool there = token < steps.tokens && s.token + token < q_len && s.head + h < a.group;
+        if (loads.live) {
           loads.load(a.q.at(t.first2 + s.token + token, head + h), there, q_tile, i);
           loads.load(a.dout.at(t.first2 + s.token + token, head + h), there, g_tile, i);
         }
+      }
     }
-  };
-  // Of every row: log2 of the sum (infinite where there is no row or it sees
-  // nothing: weights become zero), D, and the last key it sees.
-  float row_shift = 0.0f, row_delta = 0.0f;
-  int row_last = 0;
-  const int my_token = threadIdx.x / steps.heads, my_head = threadIdx.x % steps.heads;
-  const auto fetch_row = [&](const StepAt &s) __attribute__((always_inline)) {
-    if (threadIdx.x < AG_STEP) {
+    if (wave < 2) {
       const bool there = my_token < steps.tokens && s.token + my_token < q_len && s.head + my_head < a.group;
-      const int64_t at = there ? (t.first2 + s.token + my_token) * a.heads + kv_head * a.group + s.head + my_head : 0;
-      row_shift = a.lse[at];
-      row_delta = a.delta[at];
-      row_last = !there ? INT32_MIN : a.causal ? s.token + my_token + behind : INT32_MAX;
+      const float *src = (wave == 0 ? a.shift : a.delta) + (t.first2 + s.token + my_token) * a.heads + head + my_head;
+      const void *none = wave == 0 ? (const void *)&g_infinity : (const void *)&g_zeros;
+      load_word_to_lds(there ? (const void *)src : none, g_tile + TILE + wave * (AG_STEP * 4));
     }
   };
-  const auto put_row = [&](int stage) __attribute__((always_inline)) {
-    if (threadIdx.x < AG_STEP) {
-      float *x = reinterpret_cast<float *>(lds + stage * L::BYTES + 2 * TILE);
-      const bool none = row_last == INT32_MIN || row_shift == -INFINITY;
-      x[threadIdx.x] = none ? INFINITY : row_shift * LOG2E;
-      x[AG_STEP + threadIdx.x] = none ? 0.0f : row_delta;
-      reinterpret_cast<int *>(x)[2 * AG_STEP + threadIdx.x] = row_last;
-    }
+  // All loads but those of the youngest step have arrived.
+  const auto wait_for_older = [&]() {
+    if (wave < 2) wait_but<FETCHES + 1>();
+    else wait_but<FETCHES>();
   };
   const float scale_log2 = a.scale * LOG2E;
 
@@ -358,20 +356,21 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 
     });
   };
   // 32 rows (`tile`, from b on) whose products are s and dp; and the products of
-  // the next 32 (`next_tile`, from next_b on).
+  // the next 32 (`next_tile`, from next_b on).  If masked, the step's tokens from
+  // first_seen on see this lane's key.
   const auto half_step = [&](const unsigned char *tile, int b, f32x16 &s, f32x16 &dp, const unsigned char *next_tile,
-                             int next_b, f32x16 &next_s, f32x16 &next_dp, auto masked) __attribute__((always_inline)) {
+                             int next_b, f32x16 &next_s, f32x16 &next_dp, int first_seen, auto masked)
+      __attribute__((always_inline)) {
     const float *shifts = reinterpret_cast<const float *>(tile + 2 * TILE) + b + 4 * half, *deltas = shifts + AG_STEP;
-    const int *lasts = reinterpret_cast<const int *>(deltas + AG_STEP);
     uint4 x[AHEAD];
     uint32_t pw[8], pds[8];
     f32x4 shift[4], delta[4];
-    int4 last[4];
+    int4 token[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       shift[j] = *reinterpret_cast<const f32x4 *>(shifts + 8 * j);
       delta[j] = *reinterpret_cast<const f32x4 *>(deltas + 8 * j);
-      if constexpr (decltype(masked)::value) last[j] = *reinterpret_cast<const int4 *>(lasts + 8 * j);
+      if constexpr (decltype(masked)::value) token[j] = *reinterpret_cast<const int4 *>(tokens_of + b + 4 * half + 8 * j);
     }
     static_for<AHEAD>([&](auto i) __attribute__((always_inline)) { x[i] = by_rows(next_tile, next_b, i); });
 #pragma unroll
@@ -388,8 +387,8 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 
         constexpr int e = i * SHARE + j;
         float p = __builtin_amdgcn_exp2f(fmaf(s[e], scale_log2, -shift[e / 4][e % 4]));
         if constexpr (decltype(masked)::value) {
-          const int l = e % 4 == 0 ? last[e / 4].x : e % 4 == 1 ? last[e / 4].y : e % 4 == 2 ? last[e / 4].z : last[e / 4].w;
-          p = key > l ? 0.0f : p;
+          const int4 &four = token[e / 4];
+          p = (e % 4 == 0 ? four.x : e % 4 == 1 ? four.y : e % 4 == 2 ? four.z : four.w) < first_seen ? 0.0f : p;
         }
         s[e] = p;
         dp[e] = p * (dp[e] - delta[e / 4][e % 4]);
@@ -410,39 +409,34 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 
     });
   };
 
-  // While step i is worked on its successor's rows are in LDS (from the middle of
-  // the step on) and those of the next but one on their way.
-  StepAt ahead(steps, from);
+  // While a step is worked on, its successor's rows are in LDS from the middle of
+  // the step on, and those of the two behind that on their way.
+  StepAt now(steps, from), ahead = now;
   int stage = 0;  // of the step
-  const auto stage_after = [&](int n) { return stage + n < L::COUNT ? stage + n : stage + n - L::COUNT; };
+  const auto stage_after = [&](int n) { return (stage + n) % L::COUNT; };
   if (from < to) {
-    fetch_row(ahead);
-    fetch(ahead, 0);
-    put_row(0);
-    ahead.advance(steps, q_len);
-    if (from + 1 < to) {
-      fetch_row(ahead);
-      fetch(ahead, 1);
-      ahead.advance(steps, q_len);
+    for (int i = 0; i < 3 && from + i < to; i++, ahead.advance(steps, q_len)) {
+      fetch(ahead, i);
+      if (i == 0) wait_loads();
     }
-    wait_loads();
     block_barrier();
     f32x16 s0, dp0, s1, dp1;
     products(lds, 0, s0, dp0);
     const auto whole_step = [&](int64_t step, auto masked) __attribute__((always_inline)) {
       const unsigned char *tile = lds + stage * L::BYTES, *next = lds + stage_after(1) * L::BYTES;
-      half_step(tile, 0, s0, dp0, tile, 32, s1, dp1, masked);
-      put_row(stage_after(1));
-      wait_loads();
+      const int first_seen = key - behind - now.token;
+      half_step(tile, 0, s0, dp0, tile, 32, s1, dp1, first_seen, masked);
+      if (step + 2 < to) wait_for_older();
+      else wait_loads();
       block_barrier();
-      if (step + 2 < to) {
-        fetch_row(ahead);
-        fetch(ahead, stage_after(2));
+      if (step + 3 < to) {
+        fetch(ahead, stage_after(3));
         ahead.advance(steps, q_len);
       }
       // (after the last step these products are of what the stage holds, unused)
-      half_step(tile, 32, s1, dp1, next, 0, s0, dp0, masked);
+      half_step(tile, 32, s1, dp1, next, 0, s0, dp0, first_seen, masked);
       stage = stage_after(1);
+      now.advance(steps, q_len);
     };
     // The first steps of a causal tile see only some of its keys.
     const int64_t border =
@@ -501,12 +495,12 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS) void attentio
   }
 }
 
-// Workspace: D of every row and head, then the parts.  Key tiles are split so
+// Workspace: the shift and D of every row and head, then the parts.  Key tiles are split so
 // that there are about four blocks for every place on the chip (two a CU).
 struct GradPlan {
   int64_t tiles;
   int parts;
-  size_t delta_bytes, part_bytes;
+  size_t row_bytes, part_bytes;
 };
 static GradPlan grad_plan(int64_t q_rows, int64_t k_rows, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t m) {
   GradPlan p;
@@ -518,13 +512,13 @@ static GradPlan grad_plan(int64_t q_rows, int64_t k_rows, int64_t heads, int64_t
   const int64_t steps = ceil_div(group, lanes) * ceil_div(q_rows, AG_STEP / lanes);
   if (p.parts > ceil_div(steps, AG_PART_STEPS)) p.parts = (int)ceil_div(steps, AG_PART_STEPS);
   if (p.parts < 1) p.parts = 1;
-  p.delta_bytes = (size_t)ceil_div(q_rows * heads, 4) * 16;
+  p.row_bytes = (size_t)ceil_div(q_rows * heads, 4) * 16;
   p.part_bytes = p.parts > 1 ? (size_t)p.tiles * p.parts * 2 * AG_KEYS * (head_dim <= 64 ? 64 : 128) * sizeof(float) : 0;
   return p;
 }
 
 template <class E, int D> static int launch_grad(hipStream_t stream, const GradArgs &a, const GradPlan &p) {
-  constexpr int TILE = TileLoads<D, AG_THREADS>::BYTES, LDS = GradStage<D>::BYTES * GradStage<D>::COUNT;
+  constexpr int TILE = TileLoads<D, AG_THREADS>::BYTES, LDS = GradStage<D>::LDS;
   const auto dkv = attention_dkv_kernel<E, D>;
   static const hipError_t raised =
       hipFuncSetAttribute((const void *)dkv, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
@@ -552,7 +546,7 @@ extern "C" size_t fa_attention_grad_workspace_bytes(int64_t q_rows, int64_t k_ro
       check_shape(FA_F16, heads, kv_heads, head_dim) != 0)
     return 0;
   const GradPlan p = grad_plan(q_rows, k_rows, heads, kv_heads, head_dim, m);
-  return p.delta_bytes + p.part_bytes;
+  return 2 * p.row_bytes + p.part_bytes;
 }
 
 extern "C" int fa_attention_grad(fa_stream_t stream, fa_dtype t, const fa_heads *q, int64_t q_rows,
@@ -585,8 +579,8 @@ extern "C" int fa_attention_grad(fa_stream_t stream, fa_dtype t, const fa_heads 
   if (!is_aligned(workspace, 16)) return FA_EALIGN;
   const GradPlan p = grad_plan(q_rows, k_rows, heads, kv_heads, head_dim, m);
   const GradArgs a = {to_heads(q), to_heads(k), to_heads(v), to_heads(out), to_heads(dout), to_heads(dq),
-                      to_heads(dk), to_heads(dv), lse, (float *)workspace,
-                      (float *)((char *)workspace + p.delta_bytes), q_rows, k_rows, (int)heads, (int)kv_heads,
+                      to_heads(dk), to_heads(dv), lse, (float *)workspace, (float *)((char *)workspace + p.row_bytes),
+                      (float *)((char *)workspace + 2 * p.row_bytes), q_rows, k_rows, (int)heads, (int)kv_heads,
                       (int)(heads / kv_heads), (int)head_dim, q_offsets, q_lens, k_offsets, k_lens, m, scale,
                       causal != 0, p.parts, failure, code};
   const hipStream_t s = (hipStream_t)stream;
