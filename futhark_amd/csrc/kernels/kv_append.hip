@@ -1,69 +1,147 @@
 // Appending new keys and values to a paged cache, with the position rotation of
-// keys and queries applied on the way.  Pure traffic: every row is read once
-// and written once.
+// keys and queries applied on the way.  Pure traffic: every row is read once and
+// written once, 16 bytes a thread.
+//
+// A block takes some heads of one token.  Their rows go through LDS, because a
+// component's partner in the rotation may lie anywhere in its row; the sines and
+// cosines of the token's position are computed once for all of them.  What a
+// block reads is asked for before anything is known of its sequence, so that the
+// chain of dependent loads is segments, page number, store.
 #include "attention.hip.h"
 
 namespace fa {
 
-// A wave per token and slice of its heads; lanes walk the (head, component)
-// pairs.  The angle is position * frequency in f64, reduced there, because a
-// far position times a frequency near 1 leaves few bits of the angle in f32.
-template <class E>
-__global__ __launch_bounds__(256) void kv_append_kernel(Heads q, Heads q_out, Heads k, Heads v, int64_t n,
-                                                        int heads, int kv_heads, int dim,
-                                                        const int64_t *__restrict__ offsets,
-                                                        const int64_t *__restrict__ lens, int64_t m,
-                                                        const float *__restrict__ freqs, int rot,
-                                                        int interleaved, Pages pages, int32_t *failure,
-                                                        int32_t code) {
-  if (blockIdx.x == 0) report_segments(offsets, lens, m, n, failure, code);
-  const int64_t row = (int64_t)blockIdx.x * 4 + threadIdx.x / WAVE;
-  if (row >= n) return;
-  int64_t first, len;
-  const int64_t seg = segment_of_row(offsets, lens, m, n, row, first, len);
+constexpr int KA_THREADS = 256;
+constexpr int KA_MOST_DIM = 128;
+constexpr int KA_UNITS = 3;      // 16-byte units a thread
+constexpr int KA_SEGMENTS = 4;   // segments a lane looks at at a time
+
+// The sequence of a row with its first row and cached tokens; the same for the
+// whole wave.  -1: none, or a broken one.
+__device__ __forceinline__ int64_t sequence_of_row(const int64_t *offsets, const int64_t *lens, const int64_t *past_lens,
+                                                   int64_t m, int64_t n, int64_t row, int64_t &first, int64_t &len,
+                                                   int64_t &past) {
+  for (int64_t base = 0; base < m; base += WAVE * KA_SEGMENTS) {
+    int64_t f[KA_SEGMENTS], l[KA_SEGMENTS], p[KA_SEGMENTS];
+    bool here[KA_SEGMENTS];
+#pragma unroll
+    for (int j = 0; j < KA_SEGMENTS; j++) {
+      const int64_t i = base + j * WAVE + lane_id(), at = i < m ? i : m - 1;
+      p[j] = past_lens[at];
+      here[j] = i < m && segment_ok(offsets, lens, at, n, f[j], l[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < KA_SEGMENTS; j++) {
+      const uint64_t found = __ballot(here[j] && row >= f[j] && row < f[j] + l[j]);
+      if (found != 0) {
+        const int at = __builtin_ctzll(found);
+        first = read_lane(f[j], at);
+        len = read_lane(l[j], at);
+        past = read_lane(p[j], at);
+        return base + j * WAVE + at;
+      }
+    }
+  }
+  return -1;
+}
+
+struct AppendArgs {
+  Heads q, q_out, k, v;
+  int64_t n;
+  int q_heads, kv_heads, dim, block_heads;
+  const int64_t *offsets, *lens;
+  int64_t m;
+  const float *freqs;
+  int rot, interleaved;
+  Pages pages;
+  int32_t *failure, code;
+};
+
+template <class E> __global__ __launch_bounds__(KA_THREADS) void kv_append_kernel(AppendArgs a) {
+  __shared__ uint4 rows[KA_THREADS * KA_UNITS];
+  __shared__ float cosine[KA_MOST_DIM / 2], sine[KA_MOST_DIM / 2];
+  const int64_t row = blockIdx.x;
+  const int per_row = a.dim / 8, heads = a.q_heads + 2 * a.kv_heads;
+  const int head0 = blockIdx.y * a.block_heads;
+  const int units = (heads - head0 < a.block_heads ? heads - head0 : a.block_heads) * per_row;
+  // Heads are numbered: queries, keys, values.
+  uint4 mine[KA_UNITS];
+#pragma unroll
+  for (int j = 0; j < KA_UNITS; j++) {
+    const int i = j * KA_THREADS + threadIdx.x;
+    if (i < units) {
+      const int h = head0 + i / per_row, kh = h - a.q_heads;
+      const uint16_t *src = kh < 0 ? a.q.at(row, h) : kh < a.kv_heads ? a.k.at(row, kh) : a.v.at(row, kh - a.kv_heads);
+      mine[j] = *reinterpret_cast<const uint4 *>(src + i % per_row * 8);
+    }
+  }
+  if (blockIdx.x == 0 && blockIdx.y == 0) report_segments(a.offsets, a.lens, a.m, a.n, a.failure, a.code);
+  int64_t first, len, past;
+  const int64_t seg = sequence_of_row(a.offsets, a.lens, a.pages.past_lens, a.m, a.n, row, first, len, past);
   if (seg < 0) return;
-  const int64_t past = pages.past_lens[seg];
-  if (past < 0 || past > pages.capacity() || len > pages.capacity() - past) {
-    if (failure != nullptr) *failure = code;
+  const int64_t room = a.pages.capacity();
+  if (past < 0 || past > room || len > room - past) {
+    if (a.failure != nullptr) *a.failure = a.code;
     return;
   }
   const int64_t pos = past + (row - first);
-  const int64_t page = pages.table[seg * pages.cols + (pos >> pages.page_shift)];
-  const int64_t slot = pos & (((int64_t)1 << pages.page_shift) - 1);
-  const bool stored = page >= 0 && page < pages.n_pages;
-  if (!stored && failure != nullptr) *failure = code;
-  const int half = rot / 2, units = dim - half;  // a pair or a lone component
-  const int q_heads = q.data != nullptr ? heads : 0;
-  for (int i = lane_id(); i < (q_heads + 2 * kv_heads) * units; i += WAVE) {
-    const int h = i / units, u = i % units;
-    const uint16_t *src;
-    uint16_t *dst;
-    bool turn = true;
-    if (h < q_heads) {
-      src = q.at(row, h);
-      dst = q_out.at(row, h);
-    } else {
-      if (!stored) continue;
-      const bool is_v = h >= q_heads + kv_heads;
-      const int kh = h - q_heads - (is_v ? kv_heads : 0);
-      src = is_v ? v.at(row, kh) : k.at(row, kh);
-      dst = (is_v ? pages.v : pages.k) + (pages.row_of(page, kh, kv_heads) + slot) * dim;
-      turn = !is_v;
-    }
-    if (u < half) {
-      const int a = interleaved ? 2 * u : u, b = interleaved ? 2 * u + 1 : u + half;
-      if (turn) {
-        double s, c;
-        sincos((double)pos * (double)freqs[u], &s, &c);
-        const float x = E::load(src[a]), y = E::load(src[b]), cf = (float)c, sf = (float)s;
-        dst[a] = E::store(x * cf - y * sf);
-        dst[b] = E::store(y * cf + x * sf);
+  const int64_t page = a.pages.table[seg * a.pages.cols + (pos >> a.pages.page_shift)];
+  const int half = a.rot / 2;
+  if ((int)threadIdx.x < half) {
+    // The angle in turns, reduced in f64: a far position times a frequency near 1
+    // leaves few bits of the angle in f32.  What remains is at most half a turn and
+    // is rounded to f32 (an error of at most 2^-25 turns of its size).
+    const double turns = (double)pos * (double)a.freqs[threadIdx.x] * 0.15915494309189533577;
+    const float part = (float)(turns - rint(turns));
+    float s, c;
+    sincospif(2.0f * part, &s, &c);
+    cosine[threadIdx.x] = c;
+    sine[threadIdx.x] = s;
+  }
+#pragma unroll
+  for (int j = 0; j < KA_UNITS; j++) rows[j * KA_THREADS + threadIdx.x] = mine[j];
+  __syncthreads();
+  const int64_t slot = pos & (((int64_t)1 << a.pages.page_shift) - 1);
+  const bool stored = page >= 0 && page < a.pages.n_pages;
+  if (!stored && a.failure != nullptr) *a.failure = a.code;
+#pragma unroll
+  for (int j = 0; j < KA_UNITS; j++) {
+    const int i = j * KA_THREADS + threadIdx.x;
+    if (i >= units) break;
+    const int h = head0 + i / per_row, kh = h - a.q_heads, c0 = i % per_row * 8;
+    uint4 x = mine[j];
+    if (kh < a.kv_heads && c0 < a.rot) {
+      uint16_t in[8], out[8];
+      *reinterpret_cast<uint4 *>(in) = x;
+      if (a.interleaved) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const bool turned = c0 + e < a.rot;
+          const float u = E::load(in[e]), v = E::load(in[e + 1]);
+          const float c = turned ? cosine[(c0 + e) / 2] : 1.0f, s = turned ? sine[(c0 + e) / 2] : 0.0f;
+          out[e] = turned ? E::store(u * c - v * s) : in[e];
+          out[e + 1] = turned ? E::store(v * c + u * s) : in[e + 1];
+        }
       } else {
-        dst[a] = src[a];
-        dst[b] = src[b];
+        const uint16_t *whole = reinterpret_cast<const uint16_t *>(rows + (i - i % per_row));
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const int at = c0 + e;
+          const bool turned = at < a.rot, upper = at >= half;
+          const int pair = turned ? (upper ? at - half : at) : 0;
+          const float u = E::load(in[e]), v = E::load(whole[turned ? (upper ? at - half : at + half) : 0]);
+          out[e] = turned ? E::store(upper ? u * cosine[pair] + v * sine[pair] : u * cosine[pair] - v * sine[pair]) : in[e];
+        }
       }
-    } else {
-      dst[u + half] = src[u + half];
+      x = *reinterpret_cast<const uint4 *>(out);
+    }
+    if (kh < 0) {
+      *reinterpret_cast<uint4 *>(a.q_out.at(row, h) + c0) = x;
+    } else if (stored) {
+      const bool is_v = kh >= a.kv_heads;
+      uint16_t *pages = is_v ? a.pages.v : a.pages.k;
+      *reinterpret_cast<uint4 *>(
+          pages + (a.pages.row_of(page, is_v ? kh - a.kv_heads : kh, a.kv_heads) + slot) * a.dim + c0) = x;
     }
   }
 }
@@ -94,11 +172,19 @@ extern "C" int fa_kv_append(fa_stream_t stream, fa_dtype t, const fa_heads *q, c
   if (rc == 0) rc = check_pages(k_pages, v_pages, n_pages, page_size, page_table, table_cols, past_lens, kv_heads, head_dim);
   if (rc != 0) return rc;
   const fa_heads none = {nullptr, 0, 0};
-  const Heads qh = to_heads(q != nullptr ? q : &none), qo = to_heads(q != nullptr ? q_out : &none);
-  const Pages pages = to_pages(k_pages, v_pages, n_pages, page_size, page_table, table_cols, past_lens);
-  const auto kernel = t == FA_F16 ? kv_append_kernel<ElemF16> : kv_append_kernel<ElemBF16>;
-  kernel<<<dim3((unsigned)ceil_div(n, 4)), dim3(256), 0, (hipStream_t)stream>>>(
-      qh, qo, to_heads(k), to_heads(v), n, (int)heads, (int)kv_heads, (int)head_dim, offsets, lens, m, freqs,
-      (int)rot_dim, interleaved, pages, failure, code);
+  AppendArgs a = {to_heads(q != nullptr ? q : &none), to_heads(q != nullptr ? q_out : &none), to_heads(k),
+                  to_heads(v), n, q != nullptr ? (int)heads : 0, (int)kv_heads, (int)head_dim, 0, offsets, lens, m,
+                  freqs, (int)rot_dim, interleaved, to_pages(k_pages, v_pages, n_pages, page_size, page_table,
+                  table_cols, past_lens), failure, code};
+  // Heads a block takes: as many as its threads hold, fewer while there are few
+  // tokens (two blocks a CU).
+  const int64_t all = a.q_heads + 2 * a.kv_heads, most = KA_THREADS * KA_UNITS / (head_dim / 8);
+  int64_t block_heads = ceil_div(all * n, 2 * NUM_CUS_HINT);
+  if (block_heads < ceil_div(all, 65535)) block_heads = ceil_div(all, 65535);
+  if (block_heads > most) block_heads = most;
+  a.block_heads = (int)block_heads;
+  const dim3 grid((unsigned)n, (unsigned)ceil_div(all, block_heads));
+  if (t == FA_F16) kv_append_kernel<ElemF16><<<grid, KA_THREADS, 0, (hipStream_t)stream>>>(a);
+  else kv_append_kernel<ElemBF16><<<grid, KA_THREADS, 0, (hipStream_t)stream>>>(a);
   return launch_status();
 }
