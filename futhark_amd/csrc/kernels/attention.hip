@@ -454,8 +454,11 @@ template <class E, int D> __global__ __launch_bounds__(AT_THREADS) void attentio
     a.lse[out_row * a.heads + head] = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * LN2;
 }
 
-// How a cache's keys are split over blocks: enough blocks to fill the chip if
-// all sequences are as long as the table allows, at least 256 keys to a block.
+// How a cache's keys are split over blocks: if all sequences are as long as the
+// table allows, as many blocks as run at a time (two a CU), at least 256 keys to a
+// block.  More blocks spread ragged sequences better but cost more in joining than
+// that gives (2334 tokens behind 19762: 331 us; twice as many blocks 315 + 37 us,
+// four times as many 324 + 48 us).
 struct SplitPlan {
   int64_t units;
   int chunk, splits;
@@ -463,7 +466,7 @@ struct SplitPlan {
 static SplitPlan split_plan(int64_t n, int64_t heads, int64_t kv_heads, int64_t m, int64_t capacity) {
   SplitPlan p;
   p.units = most_tiles(n, m, AT_ROWS / (heads / kv_heads)) * kv_heads;
-  const int64_t even = ceil_div(capacity * p.units, 8 * NUM_CUS_HINT);
+  const int64_t even = ceil_div(capacity * p.units, 2 * NUM_CUS_HINT);
   const int64_t chunk = ceil_div(even < 256 ? 256 : even, AT_KEYS) * AT_KEYS;
   p.chunk = (int)(chunk < capacity ? chunk : (capacity > 0 ? capacity : 1));
   p.splits = (int)(capacity > 0 ? ceil_div(capacity, p.chunk) : 1);

@@ -120,36 +120,16 @@ int launch_few(hipStream_t stream, fa_dtype t, int rows, const AttentionArgs &a,
 
 // ------------------------------------------------------------------ segments
 // Segment i as the rules of fa_segred_irregular read it: inside [0, n), not
-// before the end of its predecessor.
+// before the end of its predecessor.  All loads are issued before any is looked at.
 __device__ __forceinline__ bool segment_ok(const int64_t *offsets, const int64_t *lens, int64_t i,
                                            int64_t n, int64_t &first, int64_t &len) {
+  const int64_t j = i > 0 ? i - 1 : 0, before = offsets[j], taken = lens[j];
   first = offsets[i];
   len = lens[i];
-  bool ok = first >= 0 && len >= 0 && first <= n && len <= n - first;
-  if (i > 0) {
-    const int64_t before = offsets[i - 1];
-    ok = ok && before >= 0 && before <= first && lens[i - 1] <= first - before;
-  }
-  return ok;
-}
-
-// The segment that holds `row`, or -1; the same for the whole wave, which looks
-// at 64 segments at a time.
-__device__ __forceinline__ int64_t segment_of_row(const int64_t *offsets, const int64_t *lens, int64_t m,
-                                                  int64_t n, int64_t row, int64_t &first, int64_t &len) {
-  for (int64_t base = 0; base < m; base += WAVE) {
-    const int64_t i = base + lane_id();
-    int64_t f = 0, l = 0;
-    const bool here = i < m && segment_ok(offsets, lens, i, n, f, l) && row >= f && row < f + l;
-    const uint64_t found = __ballot(here);
-    if (found != 0) {
-      const int at = __builtin_ctzll(found);
-      first = read_lane(f, at);
-      len = read_lane(l, at);
-      return base + at;
-    }
-  }
-  return -1;
+  // (unsigned: differences of whatever the arrays hold, and negative lengths are large)
+  const bool inside = (first >= 0) & (first <= n) & ((uint64_t)len <= (uint64_t)n - (uint64_t)first);
+  const bool behind = (i == 0) | ((before >= 0) & (before <= first) & ((uint64_t)taken <= (uint64_t)first - (uint64_t)before));
+  return inside & behind;
 }
 
 // Work on a segment comes in tiles of `per_tile` rows, numbered through the
@@ -166,10 +146,10 @@ __device__ __forceinline__ bool find_tile(const int64_t *offsets, const int64_t 
                                           int per_tile, int64_t number, SegTile &t) {
   int64_t before = 0;
   for (int64_t base = 0; base < m; base += WAVE) {
-    const int64_t i = base + lane_id();
-    int64_t f = 0, l = 0, f2 = 0, l2 = 0;
-    bool ok = i < m && segment_ok(offsets, lens, i, n, f, l);
-    if (offsets2 != nullptr) ok = ok && segment_ok(offsets2, lens2, i, n2, f2, l2);
+    const int64_t i = base + lane_id(), at = i < m ? i : m - 1;
+    int64_t f, l, f2 = 0, l2 = 0;
+    bool ok = segment_ok(offsets, lens, at, n, f, l) & (i < m);
+    if (offsets2 != nullptr) ok = ok & segment_ok(offsets2, lens2, at, n2, f2, l2);
     // lengths are below 2^31
     const int64_t tiles = ok ? ((uint32_t)l + (uint32_t)per_tile - 1) / (uint32_t)per_tile : 0;
     const int64_t upto = before + wave_incl_scan<int64_t, OpAdd<int64_t>>(tiles);

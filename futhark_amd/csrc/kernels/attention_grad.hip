@@ -11,7 +11,7 @@ constexpr int AG_STEP = 64;             // keys (query rows) a step
 // rows with fewer keys than this take D from the weights instead.
 constexpr int AG_EXACT_KEYS = 64;
 // Steps that are worth a part of their own when the rows of a key tile are split.
-constexpr int AG_PART_STEPS = 16;
+constexpr int AG_PART_STEPS = 16, AG_MOST_PARTS = 8;
 
 struct GradArgs {
   Heads q, k, v, out, dout, dq, dk, dv;
@@ -254,7 +254,7 @@ static __device__ const float g_infinity = INFINITY;  // the shift of a row that
 template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 : 2) void attention_dkv_kernel(GradArgs a) {
   using L = GradStage<D>;
   constexpr int TILE = L::TILE, PRODUCTS = D / 8;  // of S and dP together, and of dV and dK
-  constexpr int AHEAD = 3;                         // operands read before their product
+  constexpr int AHEAD = D == 128 ? 3 : 2;          // operands read before their product (as registers allow)
   extern __shared__ __align__(16) unsigned char lds[];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), half = lane >> 5;
   const int kv_head = blockIdx.x % a.kv_heads, part = blockIdx.y;
@@ -462,36 +462,40 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 
   }
 }
 
-// Adds the parts of the split key tiles: a block an eighth of a tile, four components a thread.
+// Adds the parts of the split key tiles, four components a thread, gridDim.y
+// blocks a tile.  (The last block of a tile to finish could add them instead, but
+// making its sums visible to the other XCDs costs more: 490 + 41 us became 735 us.)
 template <class E, int D> __global__ __launch_bounds__(AG_THREADS) void attention_dkv_join_kernel(GradArgs a) {
-  constexpr int KEYS = AG_KEYS;
   const int kv_head = blockIdx.x % a.kv_heads;
   SegTile t;
-  if (!find_tile(a.k_offsets, a.k_lens, a.k_rows, a.q_offsets, a.q_lens, a.q_rows, a.m, KEYS,
+  if (!find_tile(a.k_offsets, a.k_lens, a.k_rows, a.q_offsets, a.q_lens, a.q_rows, a.m, AG_KEYS,
                  blockIdx.x / a.kv_heads, t))
     return;
-  const int k_len = (int)t.len, q_len = (int)t.len2, key0 = (int)t.tile * KEYS;
+  const int k_len = (int)t.len, q_len = (int)t.len2, key0 = (int)t.tile * AG_KEYS;
   const int parts = parts_of(RowSteps(a.group, q_len, first_token(a, key0, q_len, k_len)).count(), a.parts);
   if (parts == 1) return;
-  constexpr int ROWS = KEYS / 8, FOURS = D / 4;
-  for (int i = threadIdx.x; i < ROWS * FOURS; i += AG_THREADS) {
-    const int row = blockIdx.y * ROWS + i / FOURS, d = i % FOURS * 4;
+  constexpr int FOURS = D / 4;
+  for (int i = blockIdx.y * AG_THREADS + threadIdx.x; i < AG_KEYS * FOURS; i += gridDim.y * AG_THREADS) {
+    const int row = i / FOURS, d = i % FOURS * 4;
     if (key0 + row >= k_len || d >= a.dim) continue;
-    f32x4 dk = {0.0f, 0.0f, 0.0f, 0.0f}, dv = dk;
-    for (int p = 0; p < parts; p++) {
-      const float *src = part_sums<D>(a, blockIdx.x, p) + row * D + d;
-      dk += *reinterpret_cast<const f32x4 *>(src);
-      dv += *reinterpret_cast<const f32x4 *>(src + KEYS * D);
-    }
-    uint32_t x[4], y[4];
+    f32x4 x[AG_MOST_PARTS], y[AG_MOST_PARTS];
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      x[j] = E::store(dk[j] * a.scale);
-      y[j] = E::store(dv[j]);
+    for (int p = 0; p < AG_MOST_PARTS; p++) {
+      const float *src = part_sums<D>(a, blockIdx.x, p < parts ? p : 0) + row * D + d;
+      x[p] = *reinterpret_cast<const f32x4 *>(src);
+      y[p] = *reinterpret_cast<const f32x4 *>(src + AG_KEYS * D);
+    }
+#pragma unroll
+    for (int p = 1; p < AG_MOST_PARTS; p++) {
+      if (p < parts) {
+        x[0] += x[p];
+        y[0] += y[p];
+      }
     }
     const int64_t at = t.first + key0 + row;
-    *reinterpret_cast<uint2 *>(a.dk.at(at, kv_head) + d) = uint2{x[0] | x[1] << 16, x[2] | x[3] << 16};
-    *reinterpret_cast<uint2 *>(a.dv.at(at, kv_head) + d) = uint2{y[0] | y[1] << 16, y[2] | y[3] << 16};
+    *reinterpret_cast<uint2 *>(a.dk.at(at, kv_head) + d) =
+        uint2{E::pack(x[0][0] * a.scale, x[0][1] * a.scale), E::pack(x[0][2] * a.scale, x[0][3] * a.scale)};
+    *reinterpret_cast<uint2 *>(a.dv.at(at, kv_head) + d) = uint2{E::pack(y[0][0], y[0][1]), E::pack(y[0][2], y[0][3])};
   }
 }
 
@@ -506,7 +510,7 @@ static GradPlan grad_plan(int64_t q_rows, int64_t k_rows, int64_t heads, int64_t
   GradPlan p;
   p.tiles = most_tiles(k_rows, m, AG_KEYS) * kv_heads;
   const int64_t wanted = p.tiles > 0 ? ceil_div(8 * NUM_CUS_HINT, p.tiles) : 1;
-  p.parts = (int)(wanted < 8 ? wanted : 8);
+  p.parts = (int)(wanted < AG_MOST_PARTS ? wanted : AG_MOST_PARTS);
   // no tile has more steps than the rows of one head group make
   const int64_t group = heads / kv_heads, lanes = group < AG_STEP ? group : AG_STEP;
   const int64_t steps = ceil_div(group, lanes) * ceil_div(q_rows, AG_STEP / lanes);
@@ -534,7 +538,10 @@ template <class E, int D> static int launch_grad(hipStream_t stream, const GradA
   dkv<<<dim3((unsigned)p.tiles, (unsigned)p.parts), AG_THREADS, LDS, stream>>>(a);
   const int rc = launch_status();
   if (rc != 0 || p.parts == 1) return rc;
-  attention_dkv_join_kernel<E, D><<<dim3((unsigned)p.tiles, 8), AG_THREADS, 0, stream>>>(a);
+  // About as many blocks as run at a time: tiles that were not split end at once.
+  int64_t blocks = 16 * NUM_CUS_HINT / p.tiles;
+  blocks = blocks < 1 ? 1 : blocks > 8 ? 8 : blocks;
+  attention_dkv_join_kernel<E, D><<<dim3((unsigned)p.tiles, (unsigned)blocks), AG_THREADS, 0, stream>>>(a);
   return launch_status();
 }
 

@@ -30,7 +30,7 @@ __device__ __forceinline__ int64_t sequence_of_row(const int64_t *offsets, const
     for (int j = 0; j < KA_SEGMENTS; j++) {
       const int64_t i = base + j * WAVE + lane_id(), at = i < m ? i : m - 1;
       p[j] = past_lens[at];
-      here[j] = i < m && segment_ok(offsets, lens, at, n, f[j], l[j]);
+      here[j] = segment_ok(offsets, lens, at, n, f[j], l[j]) & (i < m);
     }
 #pragma unroll
     for (int j = 0; j < KA_SEGMENTS; j++) {
