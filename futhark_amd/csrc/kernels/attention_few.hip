@@ -27,9 +27,6 @@ constexpr int FEW_START = 2;
 // On a short line, where a wave need not begin more than one unit, pieces end
 // with their units and have at least FEW_LEAST tiles.  Short: up to FEW_SHORT of them.
 constexpr int FEW_LEAST = 2, FEW_SHORT = 16;
-// Tables of up to this many keys are attended in one launch, if the units fit the
-// chip at once.
-constexpr int FEW_SHORT_KEYS = 1024;
 constexpr int FEW_THREADS = 256, FEW_WAVES = FEW_THREADS / WAVE;
 
 // Waves a launch has: what fits the LDS of the chip (four waves of 33 KiB a CU,
@@ -665,6 +662,16 @@ static int64_t few_most_units(int rows, int64_t n, int64_t group, int64_t kv_hea
   return most_tiles(n, m, rows / group) * kv_heads;
 }
 
+// Whether a block a unit, in one launch, is the faster way: the units fit the chip
+// at once, and a wave's quarter of the longest table, at about 0.7 us a tile, takes
+// no longer than its piece of the line and the second launch, which is about 10
+// tiles.  (Four sequences of up to 500 keys, 16 units: 7.8 us against 14.9; 17 of up
+// to 3000 with up to nine tokens, 184 units: 22.8 against 20.1.)
+static bool few_in_one_launch(int64_t units, int64_t keys, int64_t waves) {
+  const int64_t tiles = ceil_div(keys, FEW_KEYS);
+  return units * FEW_WAVES <= waves && tiles <= 128 && tiles * waves <= 4 * (10 * waves + tiles * units);
+}
+
 size_t few_workspace(int rows, int64_t n, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t m) {
   const int64_t floats = head_dim <= 64 ? few_part_floats(few_waves<64>(), rows, 64)
                                         : few_part_floats(few_waves<128>(), rows, 128);
@@ -684,7 +691,7 @@ static int launch_few_of(hipStream_t stream, AttentionArgs a, void *workspace) {
   if (raised_short != hipSuccess) return (int)raised_short;
   const int64_t units = few_most_units(ROWS, a.q_rows, a.group, a.kv_heads, a.m);
   if (units > INT32_MAX) return FA_ENOTSUP;
-  if (units * FEW_WAVES <= few_waves<D>() && a.pages.cols << a.pages.page_shift <= FEW_SHORT_KEYS) {
+  if (few_in_one_launch(units, a.pages.cols << a.pages.page_shift, few_waves<D>())) {
     short_kernel<<<dim3((unsigned)units), FEW_THREADS, LDS, stream>>>(a);
     return launch_status();
   }

@@ -257,7 +257,8 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 
   constexpr int AHEAD = D == 128 ? 3 : 2;          // operands read before their product (as registers allow)
   extern __shared__ __align__(16) unsigned char lds[];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), half = lane >> 5;
-  const int kv_head = blockIdx.x % a.kv_heads, part = blockIdx.y;
+  const int kv_head = blockIdx.x % a.kv_heads;
+  const int part = gridDim.y - 1 - blockIdx.y;  // tiles of many parts, the long ones, start first
   SegTile t;
   if (!find_tile(a.k_offsets, a.k_lens, a.k_rows, a.q_offsets, a.q_lens, a.q_rows, a.m, AG_KEYS,
                  blockIdx.x / a.kv_heads, t))
