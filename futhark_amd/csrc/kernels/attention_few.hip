@@ -203,6 +203,13 @@ template <int D, int ROWS> struct FewResult {
   float top[ROWS / 16], sum[ROWS / 16];
 };
 
+// Clears a wave's tiles where units past dim stay as they are.
+template <int D> __device__ __forceinline__ void few_clear(unsigned char *mine, int dim) {
+  if (dim == D) return;
+  for (int i = lane_id() * 16; i < 2 * FewLds<D>::STAGE; i += WAVE * 16) *reinterpret_cast<uint4 *>(mine + i) = uint4{0, 0, 0, 0};
+  wait_loads();
+}
+
 template <class E, int D, int ROWS>
 __device__ __forceinline__ void few_attend(const AttentionArgs &a, unsigned char *mine, const FewRun &u,
                                            FewResult<D, ROWS> &r) {
@@ -217,13 +224,18 @@ __device__ __forceinline__ void few_attend(const AttentionArgs &a, unsigned char
   const int load_row = lane / (D / 8), load_slot = lane % (D / 8);
   const int64_t row_bytes = a.dim * 2, head_bytes = row_bytes << a.pages.page_shift;
   const int slot_mask = (1 << a.pages.page_shift) - 1;
-  // The usual case: whole rows, and pages of at least the rows a load covers.
-  // lane_at: this lane's place among them (the swizzle repeats every 16 rows).
-  const bool plain = a.dim == D && (LOAD_ROWS - 1 & ~slot_mask) == 0;
+  // The usual case: pages of at least the rows a load covers.  lane_at: this lane's
+  // place among them (the swizzle repeats every 16 rows), and whether its unit lies
+  // below dim; those that do not were cleared beforehand.
+  const bool plain = ((LOAD_ROWS - 1) & ~slot_mask) == 0;
   uint32_t lane_at[4];
+  bool lane_live[4];
 #pragma unroll
-  for (int i = 0; i < 4; i++)
-    lane_at[i] = load_row * (D * 2) + (load_slot ^ tile_swizzle<D>(load_row + i * LOAD_ROWS)) * 16;
+  for (int i = 0; i < 4; i++) {
+    const int unit = load_slot ^ tile_swizzle<D>(load_row + i * LOAD_ROWS);
+    lane_at[i] = load_row * (uint32_t)row_bytes + unit * 16;
+    lane_live[i] = unit * 8 < a.dim;
+  }
 
   // Operand places inside a tile.  Row m of a product's 16 keys is key
   // 4 s(m / 4) + m % 4 of them, s = 0 2 1 3: with that order the rows that two
@@ -278,8 +290,10 @@ __device__ __forceinline__ void few_attend(const AttentionArgs &a, unsigned char
       for (int i = 0; i < LOADS; i++) {
         const int64_t off = ((int64_t)__builtin_amdgcn_readlane(id, i * LOAD_ROWS) * a.kv_heads + u.head) * head_bytes +
                             ((key0 + i * LOAD_ROWS) & slot_mask) * row_bytes;
-        stream_to_lds((const char *)a.pages.k + off, lane_at[i % 4], dst + i * (WAVE * 16));
-        stream_to_lds((const char *)a.pages.v + off, lane_at[i % 4], dst + L::HALF + i * (WAVE * 16));
+        if (lane_live[i % 4]) {
+          stream_to_lds((const char *)a.pages.k + off, lane_at[i % 4], dst + i * (WAVE * 16));
+          stream_to_lds((const char *)a.pages.v + off, lane_at[i % 4], dst + L::HALF + i * (WAVE * 16));
+        }
       }
       return;
     }
@@ -464,6 +478,7 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 ? 1 : 2) void attention_few_k
   int64_t at = number * line.piece;
   const int64_t end = at + line.piece < line.total ? at + line.piece : line.total;
   if (at >= end) return;
+  few_clear<D>(lds + wave * FewLds<D>::BYTES, a.dim);
   // The first of the sequences among which the piece begins (the loop below walks
   // on to the one), and the places and units before it.
   int64_t seq = __builtin_amdgcn_readfirstlane(seqs.thread[wave]) * line.each;
@@ -533,6 +548,7 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 ? 1 : 2) void attention_few_s
     s = FewSeq{read_lane(mine.first, at), read_lane(mine.past, at), read_lane(mine.len, at), read_lane(mine.row_tiles, at)};
   }
   if (seq < 0) return;
+  few_clear<D>(lds + wave * FewLds<D>::BYTES, a.dim);
   const int64_t tiles = s.key_tiles();
   const FewRun u(a, per_tile, s, seq, (uint32_t)(blockIdx.x - before), (int)(tiles * wave / FEW_WAVES),
                  (int)(tiles * (wave + 1) / FEW_WAVES));
