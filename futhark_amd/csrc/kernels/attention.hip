@@ -524,7 +524,7 @@ extern "C" int fa_attention(fa_stream_t stream, fa_dtype t, const fa_heads *q, i
 
 extern "C" size_t fa_attention_paged_workspace_bytes(int64_t n, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                                      int64_t m, int64_t page_size, int64_t table_cols) {
-  if (n <= 0 || m <= 0 || n > AT_MOST_ROWS || m > AT_MOST_ROWS || page_size <= 0 || table_cols <= 0 ||
+  if (n <= 0 || m <= 0 || n > AT_MOST_ROWS || m > AT_MOST_ROWS || page_size <= 0 || table_cols < 0 ||
       (__int128)page_size * table_cols > AT_MOST_ROWS || check_shape(FA_F16, heads, kv_heads, head_dim) != 0)
     return 0;
   const int few = few_rows(n, heads, kv_heads, m);

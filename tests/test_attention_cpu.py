@@ -163,3 +163,11 @@ def test_nothing_to_do_is_no_error(K):
     K.attention_paged(*paged_args(m=0, seg=None))
     K.kv_append(*append_args(n=0))
     K.kv_append(*append_args(m=0, seg=None))
+
+
+def test_a_table_without_columns_needs_the_same_workspace(K):
+    """Sequences that hold nothing make the launcher's choice between its ways no other: 1000 of them
+    go the way that writes a workspace."""
+    need = K.attention_paged_workspace_bytes(1000, 8, 8, 64, 1000, 16, 0)
+    assert need == K.attention_paged_workspace_bytes(1000, 8, 8, 64, 1000, 16, 4) > 0
+    refused(K.attention_paged, paged_args(n=1000, h=8, hk=8, m=1000, cols=0, table=None, ws=None, wb=0), FA_ESCRATCH)
