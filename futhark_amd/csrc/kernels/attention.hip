@@ -405,7 +405,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
     return;
   }
   const int64_t out_row = u.q_first + u.t0 + token;
-  const bool empty = top == -INFINITY;  // saw nothing, or only scores of -inf
+  const bool empty = sum == 0.0f;  // saw nothing, or only scores of -inf (and no NaN)
   const float inverse = empty ? 0.0f : 1.0f / sum;
   uint16_t *dst = a.out.at(out_row, head);
 #pragma unroll
@@ -433,25 +433,25 @@ template <class E, int D> __global__ __launch_bounds__(AT_THREADS) void attentio
   const int splits = (keys + a.chunk - 1) / a.chunk;
   float top = -INFINITY;
   for (int s = 0; s < splits; s++) top = fmaxf(top, a.part_ml[2 * part_row(a, blockIdx.x, s, row)]);
+  const float shift = top == -INFINITY ? 0.0f : top;
   float sum = 0.0f, o[D / WAVE] = {};
-  if (top != -INFINITY) {
-    for (int s = 0; s < splits; s++) {
-      const int64_t at = part_row(a, blockIdx.x, s, row);
-      const float f = exp2f(a.part_ml[2 * at] - top);
-      sum += f * a.part_ml[2 * at + 1];
+  for (int s = 0; s < splits; s++) {
+    const int64_t at = part_row(a, blockIdx.x, s, row);
+    const float f = exp2f(a.part_ml[2 * at] - shift);
+    sum += f * a.part_ml[2 * at + 1];
 #pragma unroll
-      for (int c = 0; c < D / WAVE; c++) o[c] += f * a.part_o[at * D + c * WAVE + lane_id()];
-    }
+    for (int c = 0; c < D / WAVE; c++) o[c] += f * a.part_o[at * D + c * WAVE + lane_id()];
   }
+  const bool empty = sum == 0.0f;
   const int head = u.kv_head * a.group + row % a.group;
   const int64_t out_row = u.q_first + u.t0 + row / a.group;
 #pragma unroll
   for (int c = 0; c < D / WAVE; c++) {
     const int d = c * WAVE + lane_id();
-    if (d < a.dim) a.out.at(out_row, head)[d] = E::store(top == -INFINITY ? 0.0f : o[c] / sum);
+    if (d < a.dim) a.out.at(out_row, head)[d] = E::store(empty ? 0.0f : o[c] / sum);
   }
   if (a.lse != nullptr && lane_id() == 0)
-    a.lse[out_row * a.heads + head] = top == -INFINITY ? -INFINITY : (top + log2f(sum)) * LN2;
+    a.lse[out_row * a.heads + head] = empty ? -INFINITY : (top + log2f(sum)) * LN2;
 }
 
 // How a cache's keys are split over blocks: if all sequences are as long as the

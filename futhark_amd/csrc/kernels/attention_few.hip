@@ -433,7 +433,7 @@ __device__ __forceinline__ void few_store(const AttentionArgs &a, const FewRun &
     if (row >= u.rows) continue;
     const int64_t out_row = u.row + row / a.group;
     const int q_head = u.head * a.group + row % a.group;
-    const bool empty = r.top[ct] == -INFINITY;  // only scores of -inf
+    const bool empty = all == 0.0f;  // only scores of -inf (and no NaN)
     const float inverse = empty ? 0.0f : 1.0f / all;
     uint16_t *dst = a.out.at(out_row, q_head);
 #pragma unroll
@@ -564,15 +564,16 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 ? 1 : 2) void attention_few_s
     float top = -INFINITY;
 #pragma unroll
     for (int w = 0; w < FEW_WAVES; w++) top = fmaxf(top, ml[2 * (w * ROWS + row)]);
-    const bool empty = top == -INFINITY;
+    const float shift = top == -INFINITY ? 0.0f : top;
     f32x4 x = {0.0f, 0.0f, 0.0f, 0.0f};
     float sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < FEW_WAVES; w++) {
-      const float f = empty ? 0.0f : exp2f(ml[2 * (w * ROWS + row)] - top);
+      const float f = exp2f(ml[2 * (w * ROWS + row)] - shift);
       sum += f * ml[2 * (w * ROWS + row) + 1];
       x += f * *reinterpret_cast<const f32x4 *>(o + (w * ROWS + row) * D + d);
     }
+    const bool empty = sum == 0.0f;
     const float inverse = empty ? 0.0f : 1.0f / sum;
     const int64_t out_row = u.row + row / a.group;
     const int q_head = u.head * a.group + row % a.group;
@@ -620,7 +621,7 @@ __global__ __launch_bounds__(FEW_THREADS) void attention_few_join_kernel(Attenti
       float f = top;
       for (int step = 1; step < group; step *= 2) top = fmaxf(top, __shfl_xor(top, step));
       top = fmaxf(top, tops[r]);
-      f = top == -INFINITY ? 0.0f : exp2f(f - top);
+      f = exp2f(f - (top == -INFINITY ? 0.0f : top));
       weights[r][j] = f;
       sum *= f;
       for (int step = 1; step < group; step *= 2) sum += __shfl_xor(sum, step);
@@ -654,7 +655,7 @@ __global__ __launch_bounds__(FEW_THREADS) void attention_few_join_kernel(Attenti
     if (turn < step) o += shared[threadIdx.x + step];
   }
   if (row >= rows || turn != 0) return;
-  const bool empty = tops[row] == -INFINITY;
+  const bool empty = sums[row] == 0.0f;
   const float inverse = empty ? 0.0f : 1.0f / sums[row];
   const int64_t out_row = u.row + (row0 + row) / a.group;
   const int q_head = u.head * a.group + (row0 + row) % a.group;

@@ -653,3 +653,39 @@ def test_with_the_arrays_of_a_context(ctx, K):
     assert np.all(np.abs(prod - a @ b.T) <= 1e-5 * (np.abs(a) @ np.abs(b).T))
     for y in (q, k, v, out, offsets, lens):
         y.free()
+
+
+def test_rows_of_nothing_but_nan(K):
+    """A query row of NaN, and a row whose only key is NaN, come out as NaN, not as a row that
+    sees nothing; the others are what they are."""
+    p = Problem("bf16", 4, 2, 64, [100, 70, 1], seed=90)
+    bounds = ref.forward(p.t, p.q, p.k, p.v, p.segs_q, p.segs_k, p.scale, True)
+    p.q[40, 1] = float("nan")
+    p.k[170, 0] = float("nan")  # the one key of the last sequence, of query heads 0 and 1
+    p.forward(K)
+    only_these_are_nan([(40, 1), (170, 0), (170, 1)], p.out[:171], p.lse[:171], *(x[:171] for x in bounds))
+
+
+@pytest.mark.parametrize("t,h,hk,dim,page,new,past", [
+    ("f16", 4, 2, 64, 16, [1, 1], [300, 40]),         # a block a unit
+    ("bf16", 8, 2, 128, 16, [1, 2], [20000, 70]),     # keys split over waves
+    ("f16", 4, 4, 64, 64, [200, 40], [30, 0]),        # many rows
+    ("bf16", 4, 1, 128, 64, [70, 40], [9000, 500]),   # many rows, keys split
+])
+def test_paged_rows_of_nothing_but_nan(K, t, h, hk, dim, page, new, past):
+    c = Cache(t, h, hk, dim, page, new, past, seed=91)
+    k, v, segs = c.gathered()
+    n = sum(new)
+    bounds = ref.forward(t, c.q, k, v, c.segs, segs, c.scale, True)
+    c.q[0, 1] = float("nan")
+    c.attend(K)
+    only_these_are_nan([(0, 1)], c.out[:n], c.lse[:n], *(x[:n] for x in bounds))
+
+
+def only_these_are_nan(rows, out, lse, want, want_lse, tol_o, tol_l):
+    bad = torch.zeros(lse.shape, dtype=torch.bool, device=DEV)
+    for r, h in rows:
+        bad[r, h] = True
+    assert bool(out[bad].isnan().all()) and bool(lse[bad].isnan().all())
+    ref.within(out[~bad], want[~bad], tol_o[~bad])
+    ref.within(lse[~bad], want_lse[~bad], tol_l[~bad])
