@@ -9,7 +9,7 @@
 //                    the wave the rest, and maximum, sum and weights need no
 //                    exchange but one with that partner;
 //   O^T += V^T P^T   the weights are the right operand as they stand in their
-//                    registers (tile_columns reads V in the matching key order),
+//                    registers (TileReads::columns reads V in the matching key order),
 //                    and a lane's column of O^T is its query row again, so that
 //                    rescaling is a multiplication by the lane's own factor.
 // Keys and values go from memory straight into LDS, double buffered, one
@@ -99,21 +99,18 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
   const TileReads<D> reads;
   const uint32_t lds_base = lds_address(lds);
   clear_unloaded<D>(lds, 4 * TILE, a.dim);
-  // Paged: this lane's one of the page numbers of the next tile of keys, and of
-  // the next of values.
-  int k_page = 0, v_page = 0;
+  int page = 0;  // paged: this lane's one of the page numbers of the tile fetched next
   const auto fetch_pages = [&](int key0) __attribute__((always_inline)) {
     if constexpr (PAGED) {
-      v_page = k_page;
       const int key = key0 + lane < to ? key0 + lane : to - 1;
-      k_page = a.pages.table[u.seg * a.pages.cols + (key >> a.pages.page_shift)];
+      page = a.pages.table[u.seg * a.pages.cols + (key >> a.pages.page_shift)];
     }
   };
   const int64_t k_stride = PAGED ? a.dim : a.k.row_stride, v_stride = PAGED ? a.dim : a.v.row_stride;
   const uint32_t k_offset = loads.offset(k_stride), v_offset = loads.offset(v_stride);
   const int slot_mask = PAGED ? (1 << a.pages.page_shift) - 1 : 0;
   // The keys (values) from key0 on to the tile at LDS address `tile`.
-  const auto fetch_one = [&](int key0, uint32_t tile, int page, const uint16_t *pages, const Heads &x, int64_t stride,
+  const auto fetch_one = [&](int key0, uint32_t tile, const uint16_t *pages, const Heads &x, int64_t stride,
                              uint32_t offset) __attribute__((always_inline)) {
     if constexpr (PAGED) {
       const bool there = key0 + lane < to, named = page >= 0 && page < a.pages.n_pages;
@@ -145,11 +142,19 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
       else loads.load(first, stride, to - key0, tile);
     }
   };
-  const auto fetch_k = [&](int key0, int stage) __attribute__((always_inline)) {
-    fetch_one(key0, lds_base + stage * (2 * TILE), k_page, a.pages.k, a.k, k_stride, k_offset);
+  const auto fetch = [&](int key0, int stage) __attribute__((always_inline)) {
+    const uint32_t tile = lds_base + stage * (2 * TILE);
+    fetch_one(key0, tile, a.pages.k, a.k, k_stride, k_offset);
+    fetch_one(key0, tile + TILE, a.pages.v, a.v, v_stride, v_offset);
   };
-  const auto fetch_v = [&](int key0, int stage, int page) __attribute__((always_inline)) {
-    fetch_one(key0, lds_base + stage * (2 * TILE) + TILE, page, a.pages.v, a.v, v_stride, v_offset);
+  // The tile at key0 has arrived in `stage`, the one behind it is on its way.
+  const auto arrive_and_fetch = [&](int key0, int stage) __attribute__((always_inline)) {
+    wait_loads();
+    block_barrier();
+    if (key0 + AT_KEYS < to) {
+      fetch(key0 + AT_KEYS, stage ^ 1);
+      fetch_pages(key0 + 2 * AT_KEYS);
+    }
   };
 
   uint4 q[D / 16];
@@ -183,8 +188,9 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
   };
   const auto raise = [&](float high) __attribute__((always_inline)) {
     if (__any(high > top + AT_RESCALE)) {
-      const float now = fmaxf(top, high);
-      const float factor = now == -INFINITY ? 1.0f : exp2f(top - now);
+      // (each row by its own scores alone: what other rows see changes no bit of it)
+      const float now = high > top + AT_RESCALE ? high : top;
+      const float factor = now == top ? 1.0f : exp2f(top - now);
       top = now;
       sum *= factor;
 #pragma unroll
@@ -215,13 +221,7 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
 
   // A tile of which rows of the block see different keys, or that is not full.
   const auto border = [&](int key0, int stage) __attribute__((always_inline)) {
-    wait_loads();
-    __syncthreads();
-    if (key0 + AT_KEYS < to) {
-      fetch_k(key0 + AT_KEYS, stage ^ 1);
-      fetch_v(key0 + AT_KEYS, stage ^ 1, k_page);
-      fetch_pages(key0 + 2 * AT_KEYS);
-    }
+    arrive_and_fetch(key0, stage);
     unsigned char *kt = lds + stage * (2 * TILE), *vt = kt + TILE;
     // A value that a row does not see must not reach it, and 0 * NaN would.
     bool unsafe = false;
@@ -281,97 +281,9 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
     }
   };
 
-  // Tiles all rows see.  The scores of the next 32 keys are computed while the
-  // weights of the last are: both kinds of instructions of one wave in turn.  Keys
-  // and values are fetched apart, each as soon as its half of a stage is free, two
-  // tiles (keys) and one tile (values) ahead.
-  const int full = block_first + 1 < to ? block_first + 1 : to;  // keys before it are seen by all rows
-  const int tiles = full > from ? (full - from) / AT_KEYS : 0;
-  const auto key_of = [&](int tile) { return from + tile * AT_KEYS; };
-  f32x16 s0, s1;
-  // Scores s1 of 32 keys of `kt` (from b * 32 on) while the weights of s0 are
-  // computed, then the products of those with 32 values of `vt` (from c * 32 on)
-  // while the maximum of the new scores is taken.  The order is
-  // fixed by hand: an LDS read for the next product, a product, a share of the
-  // other work.
-  const auto half_step = [&](const f32x16 &s0, f32x16 &s1, const unsigned char *kt, int b, const unsigned char *vt, int c)
-      __attribute__((always_inline)) {
-    constexpr int PRODUCTS = D / 16, SHARE = 16 / PRODUCTS;  // in each half; scores a product
-    const float shift = top == -INFINITY ? 0.0f : top;
-    uint32_t p[8];
-#pragma unroll
-    for (int i = 0; i < 16; i++) s1[i] = 0.0f;
-    uint4 x = reads.rows(kt, b * 32, 0);
-    static_for<PRODUCTS>([&](auto i) __attribute__((always_inline)) {
-      uint4 next;
-      if constexpr (i + 1 < PRODUCTS) next = reads.rows(kt, b * 32, i + 1);
-      else next = reads.columns(vt, c * 32, 0);
-      s1 = E::mfma(x, q[i], s1);
-#pragma unroll
-      for (int j = 0; j < SHARE; j += 2) {
-        const int e = i * SHARE + j;
-        const float w0 = __builtin_amdgcn_exp2f(fmaf(s0[e], a.scale_log2, -shift));
-        const float w1 = __builtin_amdgcn_exp2f(fmaf(s0[e + 1], a.scale_log2, -shift));
-        sum += w0;
-        sum += w1;
-        p[e / 2] = E::pack(w0, w1);
-      }
-      x = next;
-      __builtin_amdgcn_sched_barrier(0);
-    });
-    float high = -INFINITY;
-    static_for<PRODUCTS>([&](auto i) __attribute__((always_inline)) {
-      constexpr int half_keys = i / (D / 32), dt = i % (D / 32), n = i + 1;
-      uint4 next = x;
-      if constexpr (n < PRODUCTS) next = reads.columns(vt, c * 32 + n / (D / 32) * 16, n % (D / 32));
-      o[dt] = E::mfma(x, uint4{p[4 * half_keys], p[4 * half_keys + 1], p[4 * half_keys + 2], p[4 * half_keys + 3]}, o[dt]);
-#pragma unroll
-      for (int j = 0; j < SHARE; j += 2) high = fmaxf(high, fmaxf(s1[i * SHARE + j], s1[i * SHARE + j + 1]));
-      x = next;
-      __builtin_amdgcn_sched_barrier(0);
-    });
-    raise(fold_halves(high, FMax()) * a.scale_log2);
-  };
-  const auto attend = [&](int t, int stage, auto is_last) __attribute__((always_inline)) {
-    constexpr bool LAST = decltype(is_last)::value;
-    const unsigned char *kt = lds + stage * (2 * TILE), *vt = kt + TILE;
-    if constexpr (LAST) wait_loads();
-    else wait_but<LOADS>();
-    block_barrier();
-    if (!LAST || key_of(t + 1) < to) fetch_v(key_of(t + 1), stage ^ 1, v_page);
-    if (wave_works) half_step(s0, s1, kt, 1, vt, 0);
-    if constexpr (LAST) {
-      if (wave_works) {
-        uint4 p[2];
-        weigh(s1, p);
-        values(vt, 1, p);
-      }
-    } else {
-      wait_but<LOADS>();
-      block_barrier();
-      if (key_of(t + 2) < to && t + 2 <= tiles) {
-        fetch_k(key_of(t + 2), stage);
-        fetch_pages(key_of(t + 3));
-      }
-      if (wave_works) half_step(s1, s0, lds + (stage ^ 1) * (2 * TILE), 0, vt, 1);
-    }
-  };
-  arrived(q);
-  fetch_pages(from);
-  if (from < to) {
-    fetch_k(from, 0);
-    fetch_v(from, 0, k_page);
-  }
-  fetch_pages(from + AT_KEYS);
-  int t = 0;
-  const auto simple = [&](int t, int stage) __attribute__((always_inline)) {
-    wait_loads();
-    block_barrier();
-    if (key_of(t + 1) < to) {
-      fetch_k(key_of(t + 1), stage ^ 1);
-      fetch_v(key_of(t + 1), stage ^ 1, k_page);
-      fetch_pages(key_of(t + 2));
-    }
+  // A tile that is full and that all rows of the block see.
+  const auto inner = [&](int key0, int stage) __attribute__((always_inline)) {
+    arrive_and_fetch(key0, stage);
     const unsigned char *kt = lds + stage * (2 * TILE), *vt = kt + TILE;
     if (wave_works) {
       f32x16 s[2];
@@ -385,8 +297,15 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
       for (int b = 0; b < 2; b++) values(vt, b, p[b]);
     }
   };
-  for (; t < tiles; t++) simple(t, t & 1);
-  for (; key_of(t) < to; t++) border(key_of(t), t & 1);
+  const int full = block_first + 1 < to ? block_first + 1 : to;  // keys before it are seen by all rows
+  const int tiles = full > from ? (full - from) / AT_KEYS : 0;
+  arrived(q);
+  fetch_pages(from);
+  if (from < to) fetch(from, 0);
+  fetch_pages(from + AT_KEYS);
+  int t = 0;
+  for (; t < tiles; t++) inner(from + t * AT_KEYS, t & 1);
+  for (; from + t * AT_KEYS < to; t++) border(from + t * AT_KEYS, t & 1);
 
   sum = fold_halves(sum, FAdd());
   if (row >= rows) return;
@@ -466,7 +385,7 @@ struct SplitPlan {
 static SplitPlan split_plan(int64_t n, int64_t heads, int64_t kv_heads, int64_t m, int64_t capacity) {
   SplitPlan p;
   p.units = most_tiles(n, m, AT_ROWS / (heads / kv_heads)) * kv_heads;
-  const int64_t even = ceil_div(capacity * p.units, 2 * NUM_CUS_HINT);
+  const int64_t even = p.units < 2 * NUM_CUS_HINT ? ceil_div(capacity * p.units, 2 * NUM_CUS_HINT) : capacity;
   const int64_t chunk = ceil_div(even < 256 ? 256 : even, AT_KEYS) * AT_KEYS;
   p.chunk = (int)(chunk < capacity ? chunk : (capacity > 0 ? capacity : 1));
   p.splits = (int)(capacity > 0 ? ceil_div(capacity, p.chunk) : 1);
@@ -474,7 +393,7 @@ static SplitPlan split_plan(int64_t n, int64_t heads, int64_t kv_heads, int64_t 
 }
 
 template <bool PAGED> static int launch_attention(hipStream_t stream, fa_dtype t, const AttentionArgs &a, int64_t units) {
-  if (units > INT32_MAX) return FA_ENOTSUP;
+  if (units > AT_MOST_BLOCKS) return FA_ENOTSUP;
   const dim3 grid((unsigned)units, (unsigned)a.splits);
   const bool narrow = a.dim <= 64;
   const size_t lds = 4 * AT_KEYS * (narrow ? 64 : 128) * 2;
@@ -530,7 +449,7 @@ extern "C" size_t fa_attention_paged_workspace_bytes(int64_t n, int64_t heads, i
   const int few = few_rows(n, heads, kv_heads, m);
   if (few > 0) return few_workspace(few, n, heads, kv_heads, head_dim, m);
   const SplitPlan p = split_plan(n, heads, kv_heads, m, page_size * table_cols);
-  if (p.splits == 1) return 0;
+  if (p.splits == 1 || p.units > AT_MOST_BLOCKS) return 0;  // (more is refused)
   return (size_t)p.units * p.splits * AT_ROWS * ((head_dim <= 64 ? 64 : 128) + 2) * sizeof(float);
 }
 

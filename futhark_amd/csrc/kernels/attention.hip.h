@@ -403,6 +403,8 @@ inline int check_shape(fa_dtype t, int64_t heads, int64_t kv_heads, int64_t head
   return 0;
 }
 
+// Most blocks of 256 threads along one dimension of a launch (2^32 threads).
+constexpr int64_t AT_MOST_BLOCKS = ((int64_t)1 << 24) - 1;
 // Most rows and positions: 32-bit numbers that may run a few tiles past them.
 constexpr int64_t AT_MOST_ROWS = INT32_MAX - 4095;
 

@@ -353,8 +353,9 @@ __device__ __forceinline__ void few_attend(const AttentionArgs &a, unsigned char
       for (int i = 1; i < 8; i++) high = fmaxf(high, w[ct][i >> 2][i & 3]);
       high = fold_quarters(high, FMax()) * a.scale_log2;
       if (__any(high > r.top[ct] + AT_RESCALE)) {
-        const float now = fmaxf(r.top[ct], high);
-        const float factor = now == -INFINITY ? 1.0f : exp2f(r.top[ct] - now);
+        // (each row by its own scores alone: what other rows see changes no bit of it)
+        const float now = high > r.top[ct] + AT_RESCALE ? high : r.top[ct];
+        const float factor = now == r.top[ct] ? 1.0f : exp2f(r.top[ct] - now);
         r.top[ct] = now;
         r.sum[ct] *= factor;
 #pragma unroll
@@ -698,6 +699,8 @@ size_t few_workspace(int rows, int64_t n, int64_t heads, int64_t kv_heads, int64
 
 template <class E, int D, int ROWS>
 static int launch_few_of(hipStream_t stream, AttentionArgs a, void *workspace) {
+  const int64_t units = few_most_units(ROWS, a.q_rows, a.group, a.kv_heads, a.m);
+  if (units > AT_MOST_BLOCKS) return FA_ENOTSUP;
   constexpr int LDS = FewLds<D>::BYTES * FEW_WAVES;
   const auto kernel = attention_few_kernel<E, D, ROWS>, short_kernel = attention_few_short_kernel<E, D, ROWS>;
   static const hipError_t raised =
@@ -706,8 +709,6 @@ static int launch_few_of(hipStream_t stream, AttentionArgs a, void *workspace) {
       hipFuncSetAttribute((const void *)short_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   if (raised != hipSuccess) return (int)raised;
   if (raised_short != hipSuccess) return (int)raised_short;
-  const int64_t units = few_most_units(ROWS, a.q_rows, a.group, a.kv_heads, a.m);
-  if (units > INT32_MAX) return FA_ENOTSUP;
   if (few_in_one_launch(units, a.pages.cols << a.pages.page_shift, few_waves<D>())) {
     short_kernel<<<dim3((unsigned)units), FEW_THREADS, LDS, stream>>>(a);
     return launch_status();

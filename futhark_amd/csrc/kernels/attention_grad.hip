@@ -523,13 +523,13 @@ static GradPlan grad_plan(int64_t q_rows, int64_t k_rows, int64_t heads, int64_t
 }
 
 template <class E, int D> static int launch_grad(hipStream_t stream, const GradArgs &a, const GradPlan &p) {
+  const int64_t units = most_tiles(a.q_rows, a.m, AG_ROWS / a.group) * a.kv_heads;
+  if (units > AT_MOST_BLOCKS || p.tiles > AT_MOST_BLOCKS) return FA_ENOTSUP;
   constexpr int TILE = TileLoads<D, AG_THREADS>::BYTES, LDS = GradStage<D>::LDS;
   const auto dkv = attention_dkv_kernel<E, D>;
   static const hipError_t raised =
       hipFuncSetAttribute((const void *)dkv, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   if (raised != hipSuccess) return (int)raised;
-  const int64_t units = most_tiles(a.q_rows, a.m, AG_ROWS / a.group) * a.kv_heads;
-  if (units > INT32_MAX || p.tiles > INT32_MAX) return FA_ENOTSUP;
   if (units > 0) {
     attention_dq_kernel<E, D><<<dim3((unsigned)units), AG_THREADS, 4 * TILE, stream>>>(a);
     const int rc = launch_status();

@@ -164,6 +164,7 @@ extern "C" int fa_kv_append(fa_stream_t stream, fa_dtype t, const fa_heads *q, c
   if (rc != 0) return rc;
   if (rot_dim < 0 || rot_dim > head_dim || rot_dim % 2 != 0) return FA_EINVAL;
   if (n == 0 || m == 0) return 0;
+  if (n > AT_MOST_BLOCKS) return FA_ENOTSUP;  // a row of blocks a token
   if (rot_dim > 0 && freqs == nullptr) return FA_EINVAL;
   if (!is_aligned(freqs, 4)) return FA_EALIGN;
   if (q != nullptr) {

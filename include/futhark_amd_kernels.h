@@ -335,25 +335,36 @@ int fa_matmul_ws(fa_stream_t stream, fa_dtype in_t,
  * (FA_EALIGN); strides are not negative, and in an array that is written no two
  * elements share a place (FA_EINVAL).  A read array may repeat rows or heads
  * with a stride of 0; the gradient then has one entry per row and head and is
- * the caller's to sum.
+ * the caller's to sum.  Row strides are below 2^27 elements (FA_ENOTSUP) unless
+ * there is one row.
  *
  * Element types: FA_F16 and FA_BF16.  head_dim is a multiple of 8, 8 to 128;
  * heads is a multiple of kv_heads, and query head h reads key and value head
- * h / (heads / kv_heads), at most 128 query heads to one.  Other types, sizes
- * and groups return FA_ENOTSUP.  Products are summed and softmax statistics
- * kept in f32.
+ * h / (heads / kv_heads), at most 128 query heads to one and 65535 in all.
+ * Other types, sizes and groups return FA_ENOTSUP.  Products are summed and
+ * softmax statistics kept in f32; weights and derivatives of scores are rounded
+ * to the element type once, for the products they enter.  (In f16 a derivative
+ * below 2^-14 loses bits and below 2^-25 it is zero: scale the loss, and dout
+ * with it, as for other f16 gradients.)
  *
  * Sequences are segments of the rows, offsets[i] and lens[i] for i < m, on the
  * device, under the rules of fa_segred_irregular (in order, disjoint, inside
- * the n rows; n and m at most 2^31 - 4096).  Rows in no segment are neither read nor
- * written.  A segment that breaks the rules (or has a length or page number out
- * of range, below) is detected on the device: `code` is stored into *failure
+ * the n rows; n and m at most 2^31 - 4096).  Rows in no segment are not written
+ * and what they hold has no effect; fa_kv_append may read them.  A launch that
+ * would need 2^24 blocks (about 2^31 query rows of all heads, or new tokens of a
+ * cache beyond 2^24) returns FA_ENOTSUP.  Finding a block's segment costs it a
+ * read of all segments before it, 64 at a time.
+ *
+ * A segment that breaks the rules (or has a length or page number out of range,
+ * below) is detected on the device: `code` is stored into *failure
  * (device-visible memory; NULL: not reported), the segment is left out, and
  * nothing outside the arrays is touched.
  *
  * Nothing is allocated and no state is kept between calls: launches may be
- * captured into a graph, and calls on several streams may overlap as long as
- * they do not share outputs or workspace.
+ * captured into a graph, and calls on several streams (captured ones too) may
+ * overlap as long as they do not share outputs or workspace: a workspace serves
+ * one call at a time, and calls in order on one stream may use the same.
+ * Outputs overlap no input, except where it is said that they may.
  * Results do not depend on timing (no floating-point atomics). */
 typedef struct fa_heads {
   void *data;
@@ -367,8 +378,9 @@ typedef struct fa_heads {
  * (i, j counted from the start of their segments: the last query sees every
  * key).  A row that sees no key, or only keys of score -inf, gives out = 0 and
  * lse = -inf.  Keys that a row does not see have no effect on it, whatever
- * values they hold; a NaN among the scores it sees makes its out and lse NaN.  scale is positive and finite.  lse: [q_rows][heads] f32,
- * or NULL.  A pair of q and k segments where either is invalid is left out. */
+ * values they hold; a NaN among the scores it sees makes its out and lse NaN.
+ * scale is positive and finite.  lse: [q_rows][heads] f32, or NULL.  A pair of q
+ * and k segments where either is invalid is left out. */
 int fa_attention(fa_stream_t stream, fa_dtype t, const fa_heads *q, int64_t q_rows,
                  const fa_heads *k, const fa_heads *v, int64_t k_rows,
                  int64_t heads, int64_t kv_heads, int64_t head_dim,

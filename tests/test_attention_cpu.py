@@ -171,3 +171,24 @@ def test_a_table_without_columns_needs_the_same_workspace(K):
     need = K.attention_paged_workspace_bytes(1000, 8, 8, 64, 1000, 16, 0)
     assert need == K.attention_paged_workspace_bytes(1000, 8, 8, 64, 1000, 16, 4) > 0
     refused(K.attention_paged, paged_args(n=1000, h=8, hk=8, m=1000, cols=0, table=None, ws=None, wb=0), FA_ESCRATCH)
+
+
+def test_limits_of_strides_and_launches(K):
+    """A row stride of 2^27 elements, more heads than a launch numbers, more blocks than it has."""
+    for row, code in ((1 << 27, FA_ENOTSUP), ((1 << 27) + 4, FA_EALIGN)):
+        x = H(4, 64, row=row)
+        for which in ("q", "k", "v", "out"):
+            refused(K.attention, attention_args(hk=4, **{which: x})[1] + [None, 0], code)
+            refused(K.attention_grad, grad_args(hk=4, **{which: x}), code)
+        for which in ("q", "out"):
+            refused(K.attention_paged, paged_args(**{which: x}), code)
+        for which in ("q", "qo", "k", "v"):
+            refused(K.kv_append, append_args(hk=4, **{which: x}), code)
+    most = (1 << 31) - 4096
+    many = dict(n=most, kn=most, h=64, hk=64)
+    refused(K.attention, attention_args(**many)[1] + [None, 0], FA_ENOTSUP)
+    refused(K.attention_grad, grad_args(wb=1 << 62, **many), FA_ENOTSUP)
+    many.pop("kn")
+    refused(K.attention_paged, paged_args(wb=1 << 62, **many), FA_ENOTSUP)       # many rows a sequence
+    refused(K.attention_paged, paged_args(wb=1 << 62, m=most, **many), FA_ENOTSUP)  # one row a sequence
+    refused(K.kv_append, append_args(n=1 << 24), FA_ENOTSUP)

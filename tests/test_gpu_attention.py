@@ -689,3 +689,114 @@ def only_these_are_nan(rows, out, lse, want, want_lse, tol_o, tol_l):
     assert bool(out[bad].isnan().all()) and bool(lse[bad].isnan().all())
     ref.within(out[~bad], want[~bad], tol_o[~bad])
     ref.within(lse[~bad], want_lse[~bad], tol_l[~bad])
+
+
+@pytest.mark.parametrize("h,new,past", [(16, [1, 1], [100, 1]), (4, [200, 3], [70, 9])])
+def test_pages_past_32_bit_offsets(K, h, new, past):
+    """A cache of 2^31 elements and more, its last pages in use."""
+    hk, dim, page = 4, 128, 64
+    c = Cache("bf16", h, hk, dim, page, new, past, seed=92)
+    n_pages = (1 << 31) // (hk * page * dim) + c.pages
+    kp, vp = (torch.empty(n_pages, hk, page, dim, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    kp[-c.pages:], vp[-c.pages:] = c.kp, c.vp
+    c.table = torch.where(c.table >= 0, c.table + (n_pages - c.pages), c.table)
+    c.kp, c.vp, c.pages = kp, vp, n_pages
+    freqs = torch.tensor([10000.0 ** (-j / 64) for j in range(64)], dtype=torch.float32, device=DEV)
+    q_rot = torch.empty_like(c.q)
+    c.append(K, freqs, dim, False, q_out=q_rot)
+    pos = c.positions()
+    live = pos >= 0
+    want = ref.rotate(c.k, pos.clamp(min=0), freqs, dim, False)
+    at = [(c.table[s].long()[(past[s] + i) // page], (past[s] + i) % page, f + i)
+          for s, (f, n) in enumerate(c.segs) for i in range(n)]
+    got = torch.stack([c.kp[p, :, slot] for p, slot, _ in at])
+    rows = want[[r for _, _, r in at]]
+    ref.within(got, rows, ref.U["bf16"] * rows.abs() + 4 * 2.0 ** -24 * 16 + ref.tiny("bf16"))
+    assert int(live.sum()) == len(at)
+    q_rot[~live] = 0
+    c.attend(K, q=q_rot)
+    c.check(q=q_rot)
+
+
+def test_rows_past_32_bit_offsets(K):
+    """Parts of rows 2^26 elements apart: the last row begins past 2^31 elements."""
+    h, hk, dim, n, stride = 4, 2, 64, 40, 1 << 26
+    p = Problem("f16", h, hk, dim, [30, 10], seed=93)
+    whole = torch.empty((n - 1) * stride + 4096, dtype=torch.float16, device=DEV)
+
+    def far(x, at):
+        y = whole.as_strided((n, x.shape[1], dim), (stride, dim, 1), at)
+        y.copy_(x[:n])
+        return y
+
+    at = 0
+    for name in ("q", "k", "v", "out", "dout", "dq", "dk", "dv"):
+        x = getattr(p, name)
+        setattr(p, name, far(x, at))
+        at += x.shape[1] * dim
+    p.nq = p.nk = n
+    p.lse = p.lse[:n].contiguous()
+    p.forward(K)
+    p.backward(K)
+    p.check_forward()
+    p.check_backward()
+
+
+@pytest.mark.parametrize("h,hk,dim", [(4, 2, 64), (8, 1, 128)])
+def test_key_tiles_whose_rows_are_split(K, h, hk, dim):
+    """Few key tiles and many rows: the sums of a tile come from several blocks."""
+    p = Problem("bf16", h, hk, dim, [2100, 40], seed=94)
+    p.forward(K)
+    p.backward(K)
+    p.check_backward()
+
+
+@pytest.mark.parametrize("t,h,hk,dim,page,new,past", [
+    ("f16", 4, 2, 80, 1, [3, 7], [90, 11]),
+    ("bf16", 4, 2, 96, 2, [3, 7, 1], [900, 11, 31]),
+    ("f16", 40, 1, 64, 8, [1, 1, 1], [33, 900, 0]),
+    ("bf16", 6, 2, 128, 16, [70, 130], [9, 600]),
+])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_values_of_later_tokens_have_no_effect(K, t, h, hk, dim, page, new, past, bad):
+    """What the last new token of a sequence has in the cache does not reach the tokens before it."""
+    a, b = (Cache(t, h, hk, dim, page, new, past, seed=95) for _ in range(2))
+    for s, (n, p) in enumerate(zip(new, past)):
+        pos = p + n - 1
+        for x in (b.kp, b.vp):
+            x[b.table[s, pos // page].long(), :, pos % page] = bad
+    a.attend(K)
+    a.check()
+    b.attend(K)
+    for f, n in a.segs:
+        assert torch.equal(a.out[f:f + n - 1], b.out[f:f + n - 1])
+        assert torch.equal(a.lse[f:f + n - 1], b.lse[f:f + n - 1])
+        assert not bool(b.out[f + n - 1].isfinite().any())
+
+
+def test_two_graphs_and_two_streams(K):
+    """Captured calls of two sequences of steps, each with its own workspace, replayed on two
+    streams at once."""
+    caches = [Cache("bf16", 8, 2, 128, 16, [1, 1, 1], [5000, 40, 900], seed=96 + i) for i in range(2)]
+    graphs = []
+    for c in caches:
+        c.attend(K)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            c.attend(K)
+        graphs.append(g)
+    sides = [torch.cuda.Stream() for _ in caches]
+    for _ in range(3):
+        for c in caches:
+            c.q.copy_(-c.q)
+            c.out.fill_(MARK)
+            c.lse.fill_(MARK)
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, sides):
+            with torch.cuda.stream(s):
+                g.replay()
+                g.replay()
+        torch.cuda.synchronize()
+        for c in caches:
+            c.check()
