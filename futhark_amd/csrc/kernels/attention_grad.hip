@@ -11,7 +11,7 @@ constexpr int AG_STEP = 64;             // keys (query rows) a step
 // rows with fewer keys than this take D from the weights instead.
 constexpr int AG_EXACT_KEYS = 64;
 // Steps that are worth a part of their own when the rows of a key tile are split.
-constexpr int AG_PART_STEPS = 16, AG_MOST_PARTS = 8;
+constexpr int AG_PART_STEPS = 32, AG_MOST_PARTS = 8;
 
 struct GradArgs {
   Heads q, k, v, out, dout, dq, dk, dv;
@@ -500,8 +500,14 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS) void attentio
   }
 }
 
-// Workspace: the shift and D of every row and head, then the parts.  Key tiles are split so
-// that there are about four blocks for every place on the chip (two a CU).
+// Workspace: the shift and D of every row and head, then the parts.  Key tiles are
+// split so that there are about three blocks for every place on the chip (one a
+// CU, two for D = 64); lengths are not known here, and a sequence is expected to be
+// at most eight times as long as the average (a longer one has fewer parts).  What
+// that balances against is the parts' traffic and the second launch: five sequences
+// of up to 4096 tokens, 32 + 8 heads of 128, all kernels 947 us with eight blocks a
+// place and 16 steps a part, 895 with three and 32; thirty of up to 512, 16 heads of
+// 64, 71 us with parts and 62 without.
 struct GradPlan {
   int64_t tiles;
   int parts;
@@ -510,11 +516,13 @@ struct GradPlan {
 static GradPlan grad_plan(int64_t q_rows, int64_t k_rows, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t m) {
   GradPlan p;
   p.tiles = most_tiles(k_rows, m, AG_KEYS) * kv_heads;
-  const int64_t wanted = p.tiles > 0 ? ceil_div(8 * NUM_CUS_HINT, p.tiles) : 1;
+  const int64_t places = NUM_CUS_HINT * (head_dim <= 64 ? 2 : 1);
+  const int64_t wanted = p.tiles > 0 ? ceil_div(3 * places, p.tiles) : 1;
   p.parts = (int)(wanted < AG_MOST_PARTS ? wanted : AG_MOST_PARTS);
   // no tile has more steps than the rows of one head group make
   const int64_t group = heads / kv_heads, lanes = group < AG_STEP ? group : AG_STEP;
-  const int64_t steps = ceil_div(group, lanes) * ceil_div(q_rows, AG_STEP / lanes);
+  const int64_t longest = m > 0 && q_rows / m < q_rows / 8 ? 8 * (q_rows / m + 1) : q_rows;
+  const int64_t steps = ceil_div(group, lanes) * ceil_div(longest, AG_STEP / lanes);
   if (p.parts > ceil_div(steps, AG_PART_STEPS)) p.parts = (int)ceil_div(steps, AG_PART_STEPS);
   if (p.parts < 1) p.parts = 1;
   p.row_bytes = (size_t)ceil_div(q_rows * heads, 4) * 16;
