@@ -308,8 +308,9 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
   for (; from + t * AT_KEYS < to; t++) border(from + t * AT_KEYS, t & 1);
 
   sum = fold_halves(sum, FAdd());
-  if (row >= rows) return;
+  const bool there = row < rows;
   if (PAGED && keys > a.chunk) {
+    if (!there) return;
     const int64_t at = part_row(a, blockIdx.x, blockIdx.y, row);
 #pragma unroll
     for (int dt = 0; dt < D / 32; dt++)
@@ -326,18 +327,8 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
   const int64_t out_row = u.q_first + u.t0 + token;
   const bool empty = sum == 0.0f;  // saw nothing, or only scores of -inf (and no NaN)
   const float inverse = empty ? 0.0f : 1.0f / sum;
-  uint16_t *dst = a.out.at(out_row, head);
-#pragma unroll
-  for (int dt = 0; dt < D / 32; dt++)
-#pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const int d = dt * 32 + 2 * i + 4 * half;
-      uint16_t x[4];
-#pragma unroll
-      for (int j = 0; j < 4; j++) x[j] = E::store(empty ? 0.0f : o[dt][i + j] * inverse);
-      if (d < a.dim) *reinterpret_cast<uint2 *>(dst + d) = uint2{x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16};
-    }
-  if (a.lse != nullptr && half == 0)
+  store_column<E, D>(o, inverse, a.out.at(out_row, head), a.dim, there, empty);
+  if (a.lse != nullptr && half == 0 && there)
     a.lse[out_row * a.heads + head] = empty ? -INFINITY : (top + log2f(sum)) * LN2;
 }
 

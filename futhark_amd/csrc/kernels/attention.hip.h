@@ -360,6 +360,29 @@ struct FAdd {
   __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
 };
 
+// A lane's column of a transposed result (C of E::mfma, D / 32 of them), times
+// factor, as a row of 16-bit components; zeros if `zero`, nothing unless `there`.
+// Two lanes of the wave's halves hold four of every eight components each; they
+// trade so that each stores 16 bytes.  All lanes of the wave take part.
+template <class E, int D>
+__device__ __forceinline__ void store_column(const f32x16 (&x)[D / 32], float factor, uint16_t *dst, int dim, bool there,
+                                             bool zero = false) {
+#pragma unroll
+  for (int t = 0; t < D / 32; t++)
+#pragma unroll
+    for (int i = 0; i < 16; i += 8) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        w[j] = zero ? 0 : E::pack(x[t][i + 2 * j] * factor, x[t][i + 2 * j + 1] * factor);
+      const auto lo = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+      const auto hi = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+      const int d = t * 32 + 2 * i + 8 * (lane_id() >> 5);
+      if (there && d < dim)
+        *reinterpret_cast<uint4 *>(dst + d) = uint4{(uint32_t)lo[0], (uint32_t)hi[0], (uint32_t)lo[1], (uint32_t)hi[1]};
+    }
+}
+
 // Reports broken segments; every thread of the calling block takes part.
 __device__ __forceinline__ void report_segments(const int64_t *offsets, const int64_t *lens, int64_t m,
                                                 int64_t n, int32_t *failure, int32_t code) {

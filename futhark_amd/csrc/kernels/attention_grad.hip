@@ -37,20 +37,6 @@ template <int D> __device__ __forceinline__ void clear(f32x16 (&x)[D / 32]) {
 #pragma unroll
     for (int i = 0; i < 16; i++) x[t][i] = 0.0f;
 }
-// A lane's column of a transposed result, as a row of the output.
-template <class E, int D>
-__device__ __forceinline__ void store_column(const f32x16 (&x)[D / 32], float factor, uint16_t *dst, int dim) {
-#pragma unroll
-  for (int t = 0; t < D / 32; t++)
-#pragma unroll
-    for (int i = 0; i < 16; i += 4) {
-      const int d = t * 32 + 2 * i + 4 * (lane_id() >> 5);
-      uint32_t w[4];
-#pragma unroll
-      for (int j = 0; j < 4; j++) w[j] = E::store(x[t][i + j] * factor);
-      if (d < dim) *reinterpret_cast<uint2 *>(dst + d) = uint2{w[0] | w[1] << 16, w[2] | w[3] << 16};
-    }
-}
 // dq and D.  Laid out as the forward kernel: 128 query rows of a key head, a wave
 // owns 32 of them, 64 keys a step;
 //   S^T = K Q^T, dP^T = V dO^T, dS^T = P^T (dP^T - D), dQ^T += K^T dS^T,
@@ -186,7 +172,7 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, 2) void atten
       }
     }
   });
-  if (row < rows) store_column<E, D>(dq, a.scale, a.dq.at(at, head), a.dim);
+  store_column<E, D>(dq, a.scale, a.dq.at(at, head), a.dim, row < rows);
 }
 
 // The query rows of a key tile, in steps of AG_STEP: `heads` query heads side by
@@ -229,7 +215,8 @@ __device__ __forceinline__ int first_token(const GradArgs &a, int key0, int q_le
   return from > 0 ? from : 0;
 }
 constexpr int AG_KEYS = 32 * AG_WAVES;  // keys a block of the second kernel owns
-// Where part `part` of a key tile leaves its sums: dk then dv, [AG_KEYS][D] each.
+// Where part `part` of a key tile leaves its sums: dk then dv, and of each four
+// components of every thread side by side, as they stand in the registers.
 template <int D> __device__ __forceinline__ float *part_sums(const GradArgs &a, int64_t tile, int part) {
   return a.part + (tile * a.parts + part) * (2 * AG_KEYS * D);
 }
@@ -447,19 +434,17 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 
     for (; step < to; step++) whole_step(step, std::false_type());
   }
   if (parts > 1) {
-    float *dst = part_sums<D>(a, blockIdx.x, part) + (key - key0) * D;
+    f32x4 *dst = reinterpret_cast<f32x4 *>(part_sums<D>(a, blockIdx.x, part)) + threadIdx.x;
 #pragma unroll
     for (int dt = 0; dt < D / 32; dt++)
 #pragma unroll
       for (int i = 0; i < 16; i += 4) {
-        const int d = dt * 32 + 2 * i + 4 * half;
-        *reinterpret_cast<f32x4 *>(dst + d) = f32x4{dk[dt][i], dk[dt][i + 1], dk[dt][i + 2], dk[dt][i + 3]};
-        *reinterpret_cast<f32x4 *>(dst + AG_KEYS * D + d) =
-            f32x4{dv[dt][i], dv[dt][i + 1], dv[dt][i + 2], dv[dt][i + 3]};
+        dst[(dt * 4 + i / 4) * AG_THREADS] = f32x4{dk[dt][i], dk[dt][i + 1], dk[dt][i + 2], dk[dt][i + 3]};
+        dst[(D / 8 + dt * 4 + i / 4) * AG_THREADS] = f32x4{dv[dt][i], dv[dt][i + 1], dv[dt][i + 2], dv[dt][i + 3]};
       }
-  } else if (key < k_len) {
-    store_column<E, D>(dk, a.scale, a.dk.at(t.first + key, kv_head), a.dim);
-    store_column<E, D>(dv, 1.0f, a.dv.at(t.first + key, kv_head), a.dim);
+  } else {
+    store_column<E, D>(dk, a.scale, a.dk.at(t.first + key, kv_head), a.dim, key < k_len);
+    store_column<E, D>(dv, 1.0f, a.dv.at(t.first + key, kv_head), a.dim, key < k_len);
   }
 }
 
@@ -475,14 +460,15 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS) void attentio
   const int k_len = (int)t.len, q_len = (int)t.len2, key0 = (int)t.tile * AG_KEYS;
   const int parts = parts_of(RowSteps(a.group, q_len, first_token(a, key0, q_len, k_len)).count(), a.parts);
   if (parts == 1) return;
-  constexpr int FOURS = D / 4;
-  for (int i = blockIdx.y * AG_THREADS + threadIdx.x; i < AG_KEYS * FOURS; i += gridDim.y * AG_THREADS) {
-    const int row = i / FOURS, d = i % FOURS * 4;
-    if (key0 + row >= k_len || d >= a.dim) continue;
+  const int row = threadIdx.x / WAVE * 32 + (lane_id() & 31);
+  if (key0 + row >= k_len) return;
+  for (int i = blockIdx.y; i < D / 8; i += gridDim.y) {
+    const int d = i * 8 + (lane_id() >> 5) * 4;
+    if (d >= a.dim) continue;
     f32x4 x[AG_MOST_PARTS], y[AG_MOST_PARTS];
 #pragma unroll
     for (int p = 0; p < AG_MOST_PARTS; p++) {
-      const float *src = part_sums<D>(a, blockIdx.x, p < parts ? p : 0) + row * D + d;
+      const float *src = part_sums<D>(a, blockIdx.x, p < parts ? p : 0) + (i * AG_THREADS + threadIdx.x) * 4;
       x[p] = *reinterpret_cast<const f32x4 *>(src);
       y[p] = *reinterpret_cast<const f32x4 *>(src + AG_KEYS * D);
     }
