@@ -32,9 +32,25 @@ struct Unit {
 template <bool PAGED>
 __device__ __forceinline__ bool find_unit(const AttentionArgs &a, int64_t number, int per_tile, Unit &u) {
   SegTile t;
-  if (!find_tile(a.q_offsets, a.q_lens, a.q_rows, PAGED ? nullptr : a.k_offsets, a.k_lens, a.k_rows, a.m, per_tile,
-                 number / a.kv_heads, t))
+  if (a.by_keys) {
+    const int64_t i = lane_id() < a.m ? lane_id() : a.m - 1;
+    int64_t first, len, first2 = 0, len2;
+    bool ok = segment_ok(a.q_offsets, a.q_lens, i, a.q_rows, first, len) & (lane_id() < a.m), found;
+    if constexpr (PAGED) {
+      const int64_t past = a.pages.past_lens[i], room = a.pages.capacity();
+      const bool fits = past >= 0 && past <= room && len <= room - past;
+      if (number == 0 && ok && len > 0 && !fits && a.failure != nullptr) *a.failure = a.code;
+      ok = ok & fits;
+      len2 = past + len;
+    } else {
+      ok = ok & segment_ok(a.k_offsets, a.k_lens, i, a.k_rows, first2, len2);
+    }
+    find_tile_by_keys(ok, first, len, first2, len2, per_tile, a.causal, number / a.kv_heads, t, found);
+    if (!found) return false;
+  } else if (!find_tile(a.q_offsets, a.q_lens, a.q_rows, PAGED ? nullptr : a.k_offsets, a.k_lens, a.k_rows, a.m,
+                        per_tile, number / a.kv_heads, t)) {
     return false;
+  }
   u.kv_head = (int)(number % a.kv_heads);
   u.seg = t.seg;
   u.q_first = t.first;
@@ -429,7 +445,9 @@ extern "C" int fa_attention(fa_stream_t stream, fa_dtype t, const fa_heads *q, i
   a.causal = causal != 0;
   a.failure = failure, a.code = code;
   a.splits = 1;
-  return launch_attention<false>((hipStream_t)stream, t, a, most_tiles(q_rows, m, AT_ROWS / a.group) * kv_heads);
+  const int64_t units = most_tiles(q_rows, m, AT_ROWS / a.group) * kv_heads;
+  a.by_keys = takes_by_keys(units, m, head_dim);
+  return launch_attention<false>((hipStream_t)stream, t, a, units);
 }
 
 extern "C" size_t fa_attention_paged_workspace_bytes(int64_t n, int64_t heads, int64_t kv_heads, int64_t head_dim,
@@ -482,6 +500,7 @@ extern "C" int fa_attention_paged(fa_stream_t stream, fa_dtype t, const fa_heads
   if (few > 0) return launch_few((hipStream_t)stream, t, few, a, workspace);
   const SplitPlan p = split_plan(n, heads, kv_heads, m, page_size * table_cols);
   a.chunk = p.chunk, a.splits = p.splits;
+  a.by_keys = takes_by_keys(p.units, m, head_dim);
   if (p.splits > 1) {
     const int64_t parts = p.units * p.splits * AT_ROWS;
     a.part_o = (float *)workspace;

@@ -99,6 +99,7 @@ struct AttentionArgs {
   int64_t m;
   float scale_log2;  // scale * log2(e)
   int causal;
+  bool by_keys;  // the order of tiles (find_tile_by_keys)
   int32_t *failure, code;
   // paged only: the cache; keys of a unit that one block takes, and where parts go
   Pages pages;
@@ -168,6 +169,52 @@ __device__ __forceinline__ bool find_tile(const int64_t *offsets, const int64_t 
     before = read_lane(upto, WAVE - 1);
   }
   return false;
+}
+
+// The same for up to WAVE segments, a segment a lane (`ok` if it has one), with the
+// tiles that see most keys first, whatever segment they are of: started in this
+// order, blocks end together.  A tile's level is the number of keys it sees, in
+// tiles: of tile `tile` from the end of a segment top - tile if causal, else top;
+// the highest level is found that more than `number` tiles reach.
+__device__ __forceinline__ void find_tile_by_keys(bool ok, int64_t first, int64_t len, int64_t first2, int64_t len2,
+                                                  int per_tile, bool causal, int64_t number, SegTile &t, bool &found) {
+  const int tiles = ok ? (int)(((uint32_t)len + (uint32_t)per_tile - 1) / (uint32_t)per_tile) : 0;
+  const int top = tiles > 0 ? (int)(len2 / per_tile) : INT32_MIN / 2;
+  const auto upto_level = [&](int x) {
+    const int n = top - x + 1;
+    return n <= 0 ? 0 : !causal || n > tiles ? tiles : n;
+  };
+  int high = wave_reduce<int, OpMax<int>>(top);
+  int low = wave_reduce<int, OpMin<int>>(tiles > 0 ? causal ? top - tiles + 1 : top : INT32_MAX / 2);
+  const int64_t all = wave_reduce<int64_t, OpAdd<int64_t>>(tiles);
+  found = number < all;
+  if (!found) return;
+  while (low < high) {
+    const int x = low + (high - low + 1) / 2;
+    if (wave_reduce<int, OpAdd<int>>(upto_level(x)) > (int)number) low = x;
+    else high = x - 1;
+  }
+  const int above = upto_level(low + 1), here = upto_level(low) - above;
+  const int rank = (int)number - wave_reduce<int, OpAdd<int>>(above);
+  const int upto = wave_incl_scan<int, OpAdd<int>>(here);
+  const int at = __builtin_ctzll(__ballot(upto > rank));
+  t.seg = at;
+  t.tiles = read_lane(tiles, at);
+  t.tile = read_lane(above, at) + rank - (read_lane(upto, at) - read_lane(here, at));
+  t.first = read_lane(first, at);
+  t.len = read_lane(len, at);
+  t.first2 = read_lane(first2, at);
+  t.len2 = read_lane(len2, at);
+}
+
+// Whether blocks of units (at most `units`, of 128 query rows) take the tiles by
+// keys: where the chip holds half of them or more at a time (two blocks a CU, three
+// for D = 64).  With more the long ones even out, and tiles of one segment next to
+// each other share their keys in L2.  (600 units of six sequences with up to 8192
+// cached tokens 288 -> 267 us, 1100 of forty prompts of up to 333 15.4 -> 13.5; but
+// 1400 of twenty sequences, forward and gradient, 290 -> 306.)
+inline bool takes_by_keys(int64_t units, int64_t m, int64_t dim) {
+  return m <= WAVE && units <= 2 * NUM_CUS_HINT * (dim <= 64 ? 3 : 2);
 }
 
 // Tiles that n rows in m segments make at most (empty segments make none).

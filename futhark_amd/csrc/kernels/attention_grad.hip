@@ -24,6 +24,7 @@ struct GradArgs {
   int64_t m;
   float scale;
   int causal, parts;
+  bool by_keys;  // the order of dq's tiles
   int32_t *failure, code;
 };
 
@@ -51,9 +52,17 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, 2) void atten
   }
   const int per_tile = AG_ROWS / a.group, kv_head = blockIdx.x % a.kv_heads;
   SegTile t;
-  if (!find_tile(a.q_offsets, a.q_lens, a.q_rows, a.k_offsets, a.k_lens, a.k_rows, a.m, per_tile,
-                 blockIdx.x / a.kv_heads, t))
+  if (a.by_keys) {
+    const int64_t i = lane_id() < a.m ? lane_id() : a.m - 1;
+    int64_t first, len, first2, len2;
+    bool ok = segment_ok(a.q_offsets, a.q_lens, i, a.q_rows, first, len) & (lane_id() < a.m), found;
+    ok = ok & segment_ok(a.k_offsets, a.k_lens, i, a.k_rows, first2, len2);
+    find_tile_by_keys(ok, first, len, first2, len2, per_tile, a.causal, blockIdx.x / a.kv_heads, t, found);
+    if (!found) return;
+  } else if (!find_tile(a.q_offsets, a.q_lens, a.q_rows, a.k_offsets, a.k_lens, a.k_rows, a.m, per_tile,
+                        blockIdx.x / a.kv_heads, t)) {
     return;
+  }
   const int q_len = (int)t.len, k_len = (int)t.len2;
   const int t0 = (int)(t.tiles - 1 - t.tile) * per_tile;  // the last tokens see most: they start first
   const int tokens = q_len - t0 < per_tile ? q_len - t0 : per_tile;
@@ -516,7 +525,7 @@ static GradPlan grad_plan(int64_t q_rows, int64_t k_rows, int64_t heads, int64_t
   return p;
 }
 
-template <class E, int D> static int launch_grad(hipStream_t stream, const GradArgs &a, const GradPlan &p) {
+template <class E, int D> static int launch_grad(hipStream_t stream, GradArgs a, const GradPlan &p) {
   const int64_t units = most_tiles(a.q_rows, a.m, AG_ROWS / a.group) * a.kv_heads;
   if (units > AT_MOST_BLOCKS || p.tiles > AT_MOST_BLOCKS) return FA_ENOTSUP;
   constexpr int TILE = TileLoads<D, AG_THREADS>::BYTES, LDS = GradStage<D>::LDS;
@@ -524,6 +533,7 @@ template <class E, int D> static int launch_grad(hipStream_t stream, const GradA
   static const hipError_t raised =
       hipFuncSetAttribute((const void *)dkv, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   if (raised != hipSuccess) return (int)raised;
+  a.by_keys = takes_by_keys(units, a.m, a.dim);
   if (units > 0) {
     attention_dq_kernel<E, D><<<dim3((unsigned)units), AG_THREADS, 4 * TILE, stream>>>(a);
     const int rc = launch_status();
@@ -584,7 +594,7 @@ extern "C" int fa_attention_grad(fa_stream_t stream, fa_dtype t, const fa_heads 
                       to_heads(dk), to_heads(dv), lse, (float *)workspace, (float *)((char *)workspace + p.row_bytes),
                       (float *)((char *)workspace + 2 * p.row_bytes), q_rows, k_rows, (int)heads, (int)kv_heads,
                       (int)(heads / kv_heads), (int)head_dim, q_offsets, q_lens, k_offsets, k_lens, m, scale,
-                      causal != 0, p.parts, failure, code};
+                      causal != 0, p.parts, false, failure, code};
   const hipStream_t s = (hipStream_t)stream;
   if (t == FA_F16) return head_dim <= 64 ? launch_grad<ElemF16, 64>(s, a, p) : launch_grad<ElemF16, 128>(s, a, p);
   return head_dim <= 64 ? launch_grad<ElemBF16, 64>(s, a, p) : launch_grad<ElemBF16, 128>(s, a, p);
