@@ -70,9 +70,14 @@ __device__ __forceinline__ bool find_unit(const AttentionArgs &a, int64_t number
   return true;
 }
 
-// What splits of a unit leave for the kernel that joins them.
-__device__ __forceinline__ int64_t part_row(const AttentionArgs &a, int64_t unit, int split, int row) {
-  return (unit * a.splits + split) * AT_ROWS + row;
+// What splits of a unit leave for the kernel that joins them: maximum and sum of
+// every row, and the output so far, of which four components of every thread stand
+// side by side as they do in the registers.
+__device__ __forceinline__ float *part_ml(const AttentionArgs &a, int64_t unit, int split, int row) {
+  return a.part_ml + 2 * ((unit * a.splits + split) * AT_ROWS + row);
+}
+template <int D> __device__ __forceinline__ f32x4 *part_o(const AttentionArgs &a, int64_t unit, int split, int four) {
+  return reinterpret_cast<f32x4 *>(a.part_o + (unit * a.splits + split) * (AT_ROWS * D)) + four * AT_THREADS + threadIdx.x;
 }
 
 template <class E, int D, bool PAGED>
@@ -327,17 +332,12 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
   const bool there = row < rows;
   if (PAGED && keys > a.chunk) {
     if (!there) return;
-    const int64_t at = part_row(a, blockIdx.x, blockIdx.y, row);
 #pragma unroll
     for (int dt = 0; dt < D / 32; dt++)
 #pragma unroll
       for (int i = 0; i < 16; i += 4)
-        *reinterpret_cast<f32x4 *>(a.part_o + at * D + dt * 32 + 2 * i + 4 * half) =
-            f32x4{o[dt][i], o[dt][i + 1], o[dt][i + 2], o[dt][i + 3]};
-    if (half == 0) {
-      a.part_ml[2 * at] = top;
-      a.part_ml[2 * at + 1] = sum;
-    }
+        *part_o<D>(a, blockIdx.x, blockIdx.y, dt * 4 + i / 4) = f32x4{o[dt][i], o[dt][i + 1], o[dt][i + 2], o[dt][i + 3]};
+    if (half == 0) *reinterpret_cast<f32x2 *>(part_ml(a, blockIdx.x, blockIdx.y, row)) = f32x2{top, sum};
     return;
   }
   const int64_t out_row = u.q_first + u.t0 + token;
@@ -348,43 +348,48 @@ __global__ __launch_bounds__(AT_THREADS, 2) void attention_kernel(AttentionArgs 
     a.lse[out_row * a.heads + head] = empty ? -INFINITY : (top + log2f(sum)) * LN2;
 }
 
-// Joins the parts of the units whose keys were split: a wave per query row.
+// Joins the parts of the units whose keys were split: a block a unit and 32
+// components, laid out as the block that left them.
 template <class E, int D> __global__ __launch_bounds__(AT_THREADS) void attention_join_kernel(AttentionArgs a) {
   const int per_tile = AT_ROWS / a.group;
   Unit u;
   if (!find_unit<true>(a, blockIdx.x, per_tile, u)) return;
-  const int row = blockIdx.y * AT_WAVES + threadIdx.x / WAVE, rows = u.tokens * a.group;
-  const int keys = u.t0 + u.tokens + u.k_len - u.q_len;
-  if (row >= rows || keys <= a.chunk) return;
+  const int keys = u.t0 + u.tokens + u.k_len - u.q_len, dt = blockIdx.y;
+  if (keys <= a.chunk || dt * 32 >= a.dim) return;
+  const int row = threadIdx.x / WAVE * 32 + (lane_id() & 31), rows = u.tokens * a.group;
   const int splits = (keys + a.chunk - 1) / a.chunk;
   float top = -INFINITY;
-  for (int s = 0; s < splits; s++) top = fmaxf(top, a.part_ml[2 * part_row(a, blockIdx.x, s, row)]);
+  for (int s = 0; s < splits; s++) top = fmaxf(top, part_ml(a, blockIdx.x, s, row)[0]);
   const float shift = top == -INFINITY ? 0.0f : top;
-  float sum = 0.0f, o[D / WAVE] = {};
+  float sum = 0.0f;
+  f32x16 o[1];
+#pragma unroll
+  for (int i = 0; i < 16; i++) o[0][i] = 0.0f;
   for (int s = 0; s < splits; s++) {
-    const int64_t at = part_row(a, blockIdx.x, s, row);
-    const float f = exp2f(a.part_ml[2 * at] - shift);
-    sum += f * a.part_ml[2 * at + 1];
+    const f32x2 ml = *reinterpret_cast<const f32x2 *>(part_ml(a, blockIdx.x, s, row));
+    const float f = exp2f(ml[0] - shift);
+    sum += f * ml[1];
 #pragma unroll
-    for (int c = 0; c < D / WAVE; c++) o[c] += f * a.part_o[at * D + c * WAVE + lane_id()];
-  }
-  const bool empty = sum == 0.0f;
-  const int head = u.kv_head * a.group + row % a.group;
-  const int64_t out_row = u.q_first + u.t0 + row / a.group;
+    for (int i = 0; i < 16; i += 4) {
+      const f32x4 x = *part_o<D>(a, blockIdx.x, s, dt * 4 + i / 4);
 #pragma unroll
-  for (int c = 0; c < D / WAVE; c++) {
-    const int d = c * WAVE + lane_id();
-    if (d < a.dim) a.out.at(out_row, head)[d] = E::store(empty ? 0.0f : o[c] / sum);
+      for (int j = 0; j < 4; j++) o[0][i + j] += f * x[j];
+    }
   }
-  if (a.lse != nullptr && lane_id() == 0)
+  const bool there = row < rows, empty = sum == 0.0f;
+  const int my_row = there ? row : 0, head = u.kv_head * a.group + my_row % a.group;
+  const int64_t out_row = u.q_first + u.t0 + my_row / a.group;
+  store_column<E, 32>(o, 1.0f / sum, a.out.at(out_row, head) + dt * 32, a.dim - dt * 32, there, empty);
+  if (a.lse != nullptr && dt == 0 && there && lane_id() < 32)
     a.lse[out_row * a.heads + head] = empty ? -INFINITY : (top + log2f(sum)) * LN2;
 }
 
-// How a cache's keys are split over blocks: if all sequences are as long as the
-// table allows, as many blocks as run at a time (two a CU), at least 256 keys to a
-// block.  More blocks spread ragged sequences better but cost more in joining than
-// that gives (2334 tokens behind 19762: 331 us; twice as many blocks 315 + 37 us,
-// four times as many 324 + 48 us).
+// How a cache's keys are split over blocks.  Lengths are not known here.  One
+// sequence is taken to be as long as the table allows: as many blocks as run at a
+// time (two a CU).  Several are ragged: twice as many, at least 256 keys to a block.
+// (Twenty chunks of up to 300 tokens behind up to 4096 105 -> 74 us, two of 32 heads
+// without groups 184 -> 117; six of up to 1024 behind up to 8192, which fill the chip
+// unsplit, 266 -> 280.  Three times as many: 93, 127, 279.)
 struct SplitPlan {
   int64_t units;
   int chunk, splits;
@@ -392,7 +397,8 @@ struct SplitPlan {
 static SplitPlan split_plan(int64_t n, int64_t heads, int64_t kv_heads, int64_t m, int64_t capacity) {
   SplitPlan p;
   p.units = most_tiles(n, m, AT_ROWS / (heads / kv_heads)) * kv_heads;
-  const int64_t even = p.units < 2 * NUM_CUS_HINT ? ceil_div(capacity * p.units, 2 * NUM_CUS_HINT) : capacity;
+  const int64_t blocks = (m > 1 ? 4 : 2) * NUM_CUS_HINT;
+  const int64_t even = p.units < blocks ? ceil_div(capacity * p.units, blocks) : capacity;
   const int64_t chunk = ceil_div(even < 256 ? 256 : even, AT_KEYS) * AT_KEYS;
   p.chunk = (int)(chunk < capacity ? chunk : (capacity > 0 ? capacity : 1));
   p.splits = (int)(capacity > 0 ? ceil_div(capacity, p.chunk) : 1);
@@ -508,7 +514,7 @@ extern "C" int fa_attention_paged(fa_stream_t stream, fa_dtype t, const fa_heads
   }
   rc = launch_attention<true>((hipStream_t)stream, t, a, p.units);
   if (rc != 0 || p.splits == 1) return rc;
-  const dim3 grid((unsigned)p.units, (unsigned)ceil_div(AT_ROWS, AT_WAVES));
+  const dim3 grid((unsigned)p.units, head_dim <= 64 ? 2 : 4);
   if (t == FA_F16) {
     if (head_dim <= 64) attention_join_kernel<ElemF16, 64><<<grid, AT_THREADS, 0, (hipStream_t)stream>>>(a);
     else attention_join_kernel<ElemF16, 128><<<grid, AT_THREADS, 0, (hipStream_t)stream>>>(a);
