@@ -720,10 +720,11 @@ static int launch_few_of(hipStream_t stream, AttentionArgs a, void *workspace) {
   const int rc = launch_status();
   if (rc != 0) return rc;
   // Rows a block of the second kernel joins: as many as its threads hold, fewer
-  // while there are blocks to spare.
+  // while there are less than two blocks a CU (17 sequences with up to nine tokens
+  // 20.0 -> 18.6 us against one a CU; four a CU the same).
   const int64_t rows = ROWS / a.group * a.group;  // of a unit, at most
   int join_rows = FEW_THREADS / (D / 4);
-  while (join_rows > 1 && units * ceil_div(rows, join_rows) < NUM_CUS_HINT) join_rows /= 2;
+  while (join_rows > 1 && units * ceil_div(rows, join_rows) < 2 * NUM_CUS_HINT) join_rows /= 2;
   const dim3 grid((unsigned)units, (unsigned)ceil_div(rows, join_rows));
   attention_few_join_kernel<E, D, ROWS><<<grid, FEW_THREADS, 0, stream>>>(a, join_rows);
   return launch_status();

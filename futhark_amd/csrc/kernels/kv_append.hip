@@ -4,11 +4,12 @@
 //
 // A block takes some heads of one token.  Their rows go through LDS, because a
 // component's partner in the rotation may lie anywhere in its row; the sines and
-// cosines of the token's position are computed once for all of them.  What a
-// block reads is asked for before anything is known of its sequence, so that the
-// chain of dependent loads is segments, page number, store.  Loads and stores are
-// non-temporal: nothing is used twice (14555 tokens of 32 + 8 heads of 128: 88 ->
-// 78 us, 4.6 TB/s; 32 tokens: 4.6 us, launch and that chain).
+// cosines of the token's position are computed once for all of them.  Loads return
+// in the order they were asked for: the segments come first, the rows behind them,
+// and the page number past both by the scalar cache, so that looking up the place
+// and computing the angles hide behind the rows (14555 tokens of 32 + 8 heads of
+// 128: 79 -> 58 us, 6.1 TB/s).  Loads and stores are non-temporal: nothing is used
+// twice (88 -> 78 us before that).  32 tokens: 4.5 us, launch and the chain.
 #include "attention.hip.h"
 
 namespace fa {
@@ -19,33 +20,35 @@ constexpr int KA_UNITS = 3;      // 16-byte units a thread
 constexpr int KA_SEGMENTS = 4;   // segments a lane looks at at a time
 
 // The sequence of a row with its first row and cached tokens; the same for the
-// whole wave.  -1: none, or a broken one.
-__device__ __forceinline__ int64_t sequence_of_row(const int64_t *offsets, const int64_t *lens, const int64_t *past_lens,
-                                                   int64_t m, int64_t n, int64_t row, int64_t &first, int64_t &len,
-                                                   int64_t &past) {
-  for (int64_t base = 0; base < m; base += WAVE * KA_SEGMENTS) {
-    int64_t f[KA_SEGMENTS], l[KA_SEGMENTS], p[KA_SEGMENTS];
-    bool here[KA_SEGMENTS];
+// whole wave.  A lane looks at N segments from `base` on.
+template <int N> struct Look {
+  int64_t first[N], len[N], past[N];
+  bool ok[N];
+  __device__ __forceinline__ void load(const int64_t *offsets, const int64_t *lens, const int64_t *past_lens, int64_t m,
+                                       int64_t n, int64_t base) {
 #pragma unroll
-    for (int j = 0; j < KA_SEGMENTS; j++) {
+    for (int j = 0; j < N; j++) {
       const int64_t i = base + j * WAVE + lane_id(), at = i < m ? i : m - 1;
-      p[j] = past_lens[at];
-      here[j] = segment_ok(offsets, lens, at, n, f[j], l[j]) & (i < m);
-    }
-#pragma unroll
-    for (int j = 0; j < KA_SEGMENTS; j++) {
-      const uint64_t found = __ballot(here[j] && row >= f[j] && row < f[j] + l[j]);
-      if (found != 0) {
-        const int at = __builtin_ctzll(found);
-        first = read_lane(f[j], at);
-        len = read_lane(l[j], at);
-        past = read_lane(p[j], at);
-        return base + j * WAVE + at;
-      }
+      past[j] = past_lens[at];
+      ok[j] = segment_ok(offsets, lens, at, n, first[j], len[j]) & (i < m);
     }
   }
-  return -1;
-}
+  // The number of the row's segment from `base` on, or -1.
+  __device__ __forceinline__ int find(int64_t row, int64_t &f, int64_t &l, int64_t &p) const {
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+      const uint64_t found = __ballot(ok[j] && row >= first[j] && row < first[j] + len[j]);
+      if (found != 0) {
+        const int at = __builtin_ctzll(found);
+        f = read_lane(first[j], at);
+        l = read_lane(len[j], at);
+        p = read_lane(past[j], at);
+        return j * WAVE + at;
+      }
+    }
+    return -1;
+  }
+};
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
@@ -61,6 +64,11 @@ struct AppendArgs {
   int32_t *failure, code;
 };
 
+// From an address that is the same for the wave, through the scalar cache.
+__device__ __forceinline__ int32_t scalar_load(const int32_t *p) {
+  return *(const int32_t __attribute__((address_space(4))) *)wave_address(p);
+}
+
 template <class E> __global__ __launch_bounds__(KA_THREADS) void kv_append_kernel(AppendArgs a) {
   __shared__ uint4 rows[KA_THREADS * KA_UNITS];
   __shared__ float cosine[KA_MOST_DIM / 2], sine[KA_MOST_DIM / 2];
@@ -68,20 +76,33 @@ template <class E> __global__ __launch_bounds__(KA_THREADS) void kv_append_kerne
   const int per_row = a.dim / 8, heads = a.q_heads + 2 * a.kv_heads;
   const int head0 = blockIdx.y * a.block_heads;
   const int units = (heads - head0 < a.block_heads ? heads - head0 : a.block_heads) * per_row;
+  // The first segments and this thread's frequency before the rows.
+  Look<1> nearest;
+  nearest.load(a.offsets, a.lens, a.pages.past_lens, a.m, a.n, 0);
+  const int half = a.rot / 2;
+  const float *freqs = half > 0 ? a.freqs : reinterpret_cast<const float *>(a.lens);  // (something to load)
+  const float freq = freqs[(int)threadIdx.x < half ? threadIdx.x : 0];
   // Heads are numbered: queries, keys, values.
   uint4 mine[KA_UNITS];
+  const uint16_t *q_row = a.q.at(row, 0), *k_row = a.k.at(row, 0), *v_row = a.v.at(row, 0);
 #pragma unroll
   for (int j = 0; j < KA_UNITS; j++) {
-    const int i = j * KA_THREADS + threadIdx.x;
-    if (i < units) {
-      const int h = head0 + i / per_row, kh = h - a.q_heads;
-      const uint16_t *src = kh < 0 ? a.q.at(row, h) : kh < a.kv_heads ? a.k.at(row, kh) : a.v.at(row, kh - a.kv_heads);
-      mine[j] = bit_cast<uint4>(__builtin_nontemporal_load(reinterpret_cast<const i32x4 *>(src + i % per_row * 8)));
-    }
+    // (no branches: loads under a condition would be waited for one by one)
+    const int i = j * KA_THREADS + threadIdx.x < units ? j * KA_THREADS + threadIdx.x : units - 1;
+    const int h = head0 + i / per_row, kh = h - a.q_heads, vh = kh - a.kv_heads;
+    const uint16_t *q = q_row + h * a.q.head_stride, *k = k_row + kh * a.k.head_stride, *v = v_row + vh * a.v.head_stride;
+    const uint16_t *src = kh < 0 ? q : vh < 0 ? k : v;
+    mine[j] = bit_cast<uint4>(__builtin_nontemporal_load(reinterpret_cast<const i32x4 *>(src + i % per_row * 8)));
+  }
+  int64_t first, len, past;
+  int64_t seg = nearest.find(row, first, len, past);
+  for (int64_t base = WAVE; seg < 0 && base < a.m; base += WAVE * KA_SEGMENTS) {
+    Look<KA_SEGMENTS> more;
+    more.load(a.offsets, a.lens, a.pages.past_lens, a.m, a.n, base);
+    const int at = more.find(row, first, len, past);
+    if (at >= 0) seg = base + at;
   }
   if (blockIdx.x == 0 && blockIdx.y == 0) report_segments(a.offsets, a.lens, a.m, a.n, a.failure, a.code);
-  int64_t first, len, past;
-  const int64_t seg = sequence_of_row(a.offsets, a.lens, a.pages.past_lens, a.m, a.n, row, first, len, past);
   if (seg < 0) return;
   const int64_t room = a.pages.capacity();
   if (past < 0 || past > room || len > room - past) {
@@ -89,13 +110,12 @@ template <class E> __global__ __launch_bounds__(KA_THREADS) void kv_append_kerne
     return;
   }
   const int64_t pos = past + (row - first);
-  const int64_t page = a.pages.table[seg * a.pages.cols + (pos >> a.pages.page_shift)];
-  const int half = a.rot / 2;
+  const int64_t page = scalar_load(a.pages.table + seg * a.pages.cols + (pos >> a.pages.page_shift));
   if ((int)threadIdx.x < half) {
     // The angle in turns, reduced in f64: a far position times a frequency near 1
     // leaves few bits of the angle in f32.  What remains is at most half a turn and
     // is rounded to f32 (an error of at most 2^-25 turns of its size).
-    const double turns = (double)pos * (double)a.freqs[threadIdx.x] * 0.15915494309189533577;
+    const double turns = (double)pos * (double)freq * 0.15915494309189533577;
     const float part = (float)(turns - rint(turns));
     float s, c;
     sincospif(2.0f * part, &s, &c);
