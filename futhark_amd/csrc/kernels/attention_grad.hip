@@ -457,8 +457,8 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 
   }
 }
 
-// Adds the parts of the split key tiles, four components a thread, gridDim.y
-// blocks a tile.  (The last block of a tile to finish could add them instead, but
+// Adds the parts of the split key tiles, gridDim.y blocks a tile, laid out as the
+// blocks that left them.  (The last block of a tile to finish could add them instead, but
 // making its sums visible to the other XCDs costs more: 490 + 41 us became 735 us.)
 template <class E, int D> __global__ __launch_bounds__(AG_THREADS) void attention_dkv_join_kernel(GradArgs a) {
   const int kv_head = blockIdx.x % a.kv_heads;
@@ -470,28 +470,31 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS) void attentio
   const int parts = parts_of(RowSteps(a.group, q_len, first_token(a, key0, q_len, k_len)).count(), a.parts);
   if (parts == 1) return;
   const int row = threadIdx.x / WAVE * 32 + (lane_id() & 31);
-  if (key0 + row >= k_len) return;
-  for (int i = blockIdx.y; i < D / 8; i += gridDim.y) {
-    const int d = i * 8 + (lane_id() >> 5) * 4;
-    if (d >= a.dim) continue;
-    f32x4 x[AG_MOST_PARTS], y[AG_MOST_PARTS];
+  const bool there = key0 + row < k_len;
+  const int64_t at = t.first + key0 + (there ? row : 0);
+  // 32 components of dk or of dv at a time, two parts at a time.
+  for (int c = blockIdx.y; c < D / 16; c += gridDim.y) {
+    const bool is_v = c >= D / 32;
+    const int dt = c % (D / 32);
+    const auto load = [&](int part, f32x4 (&x)[4]) __attribute__((always_inline)) {
+      const f32x4 *src = reinterpret_cast<const f32x4 *>(part_sums<D>(a, blockIdx.x, part)) + 4 * c * AG_THREADS + threadIdx.x;
 #pragma unroll
-    for (int p = 0; p < AG_MOST_PARTS; p++) {
-      const float *src = part_sums<D>(a, blockIdx.x, p < parts ? p : 0) + (i * AG_THREADS + threadIdx.x) * 4;
-      x[p] = *reinterpret_cast<const f32x4 *>(src);
-      y[p] = *reinterpret_cast<const f32x4 *>(src + AG_KEYS * D);
-    }
+      for (int i = 0; i < 4; i++) x[i] = src[i * AG_THREADS];
+    };
+    f32x16 sum[1];
 #pragma unroll
-    for (int p = 1; p < AG_MOST_PARTS; p++) {
-      if (p < parts) {
-        x[0] += x[p];
-        y[0] += y[p];
+    for (int i = 0; i < 16; i++) sum[0][i] = 0.0f;
+    for (int p = 0; p < parts; p += 2) {
+      f32x4 x[4], y[4];
+      load(p, x);
+      load(p + 1 < parts ? p + 1 : p, y);
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        sum[0][i] += x[i / 4][i % 4];
+        if (p + 1 < parts) sum[0][i] += y[i / 4][i % 4];
       }
     }
-    const int64_t at = t.first + key0 + row;
-    *reinterpret_cast<uint2 *>(a.dk.at(at, kv_head) + d) =
-        uint2{E::pack(x[0][0] * a.scale, x[0][1] * a.scale), E::pack(x[0][2] * a.scale, x[0][3] * a.scale)};
-    *reinterpret_cast<uint2 *>(a.dv.at(at, kv_head) + d) = uint2{E::pack(y[0][0], y[0][1]), E::pack(y[0][2], y[0][3])};
+    store_column<E, 32>(sum, is_v ? 1.0f : a.scale, (is_v ? a.dv : a.dk).at(at, kv_head) + dt * 32, a.dim - dt * 32, there);
   }
 }
 
