@@ -364,7 +364,8 @@ int fa_matmul_ws(fa_stream_t stream, fa_dtype in_t,
  * captured into a graph, and calls on several streams (captured ones too) may
  * overlap as long as they do not share outputs or workspace: a workspace serves
  * one call at a time, and calls in order on one stream may use the same.
- * Outputs overlap no input, except where it is said that they may.
+ * Outputs overlap no input and not each other, except where it is said that they
+ * may.
  * Results do not depend on timing (no floating-point atomics). */
 typedef struct fa_heads {
   void *data;

@@ -800,3 +800,35 @@ def test_two_graphs_and_two_streams(K):
         torch.cuda.synchronize()
         for c in caches:
             c.check()
+
+
+@pytest.mark.parametrize("dim", [40, 72])
+def test_split_key_tiles_of_odd_heads(K, dim):
+    p = Problem("f16", 12, 2, dim, [1300, 7, 300], [1300, 200, 90], seed=97)
+    p.forward(K)
+    p.check_forward()
+    p.backward(K)
+    p.check_backward()
+
+
+def test_bad_pages_and_lengths_of_many_rows(K):
+    """The same as above for the kernel that takes many rows, its keys split."""
+    for what in ("page high", "past negative", "past high", "past huge", "len"):
+        c, good = (Cache("bf16", 2, 1, 64, 16, [70, 90, 65], [3000, 20, 40], seed=98) for _ in range(2))
+        if what == "page high":
+            c.table[1, 3] = c.pages
+        elif what == "len":
+            c.lens[1] = 1 << 40
+        else:
+            c.past_lens[1] = {"past negative": -1, "past high": c.cols * 16 - 89, "past huge": (1 << 63) - 1}[what]
+        c.attend(K)
+        assert c.failure.item() == 6, what
+        good.attend(K)
+        good.check()
+        kept = [0] if what == "len" else [0, 2]  # a length past the end breaks the segment behind it too
+        for s in kept:
+            f, n = c.segs[s]
+            assert torch.equal(good.out[f:f + n], c.out[f:f + n]), (what, s)
+        f, n = c.segs[1]
+        if what != "page high":
+            assert bool((c.out[f:f + n] == MARK).all()), what
