@@ -54,7 +54,7 @@ __device__ __forceinline__ bool find_unit(const AttentionArgs &a, int64_t number
     } else {
       ok = ok & segment_ok(a.k_offsets, a.k_lens, i, a.k_rows, first2, len2);
     }
-    find_tile_by_keys(ok, first, len, first2, len2, per_tile, a.causal, number / a.kv_heads, t, found);
+    find_tile_by_keys(ok, first, len, first2, len2, len2, per_tile, a.causal, number / a.kv_heads, t, found);
     if (!found) return false;
   } else if (!find_tile(a.q_offsets, a.q_lens, a.q_rows, PAGED ? nullptr : a.k_offsets, a.k_lens, a.k_rows, a.m,
                         per_tile, number / a.kv_heads, t)) {

@@ -174,12 +174,13 @@ __device__ __forceinline__ bool find_tile(const int64_t *offsets, const int64_t 
 // The same for up to WAVE segments, a segment a lane (`ok` if it has one), with the
 // tiles that see most keys first, whatever segment they are of: started in this
 // order, blocks end together.  A tile's level is the number of keys it sees, in
-// tiles: of tile `tile` from the end of a segment top - tile if causal, else top;
+// tiles, `seen` keys for the first one: of the one `tile` behind it top - tile if
+// causal, else top;
 // the highest level is found that more than `number` tiles reach.
-__device__ __forceinline__ void find_tile_by_keys(bool ok, int64_t first, int64_t len, int64_t first2, int64_t len2,
+__device__ __forceinline__ void find_tile_by_keys(bool ok, int64_t first, int64_t len, int64_t first2, int64_t len2, int64_t seen,
                                                   int per_tile, bool causal, int64_t number, SegTile &t, bool &found) {
   const int tiles = ok ? (int)(((uint32_t)len + (uint32_t)per_tile - 1) / (uint32_t)per_tile) : 0;
-  const int top = tiles > 0 ? (int)(len2 / per_tile) : INT32_MIN / 2;
+  const int top = tiles > 0 ? (int)(seen / per_tile) : INT32_MIN / 2;
   const auto upto_level = [&](int x) {
     const int n = top - x + 1;
     return n <= 0 ? 0 : !causal || n > tiles ? tiles : n;

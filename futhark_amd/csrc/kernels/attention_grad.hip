@@ -29,7 +29,7 @@ struct GradArgs {
   int64_t m;
   float scale;
   int causal, parts;
-  bool by_keys;  // the order of dq's tiles
+  bool by_keys, by_rows;  // the order of dq's tiles, and of dk's and dv's
   int32_t *failure, code;
 };
 
@@ -62,7 +62,7 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, 2) void atten
     int64_t first, len, first2, len2;
     bool ok = segment_ok(a.q_offsets, a.q_lens, i, a.q_rows, first, len) & (lane_id() < a.m), found;
     ok = ok & segment_ok(a.k_offsets, a.k_lens, i, a.k_rows, first2, len2);
-    find_tile_by_keys(ok, first, len, first2, len2, per_tile, a.causal, blockIdx.x / a.kv_heads, t, found);
+    find_tile_by_keys(ok, first, len, first2, len2, len2, per_tile, a.causal, blockIdx.x / a.kv_heads, t, found);
     if (!found) return;
   } else if (!find_tile(a.q_offsets, a.q_lens, a.q_rows, a.k_offsets, a.k_lens, a.k_rows, a.m, per_tile,
                         blockIdx.x / a.kv_heads, t)) {
@@ -234,6 +234,19 @@ constexpr int AG_KEYS = 32 * AG_WAVES;  // keys a block of the second kernel own
 template <int D> __device__ __forceinline__ float *part_sums(const GradArgs &a, int64_t tile, int part) {
   return a.part + (tile * a.parts + part) * (2 * AG_KEYS * D);
 }
+// The key tile of this block, the one that most tokens see first if by_rows.
+__device__ __forceinline__ bool find_key_tile(const GradArgs &a, SegTile &t) {
+  const int64_t number = blockIdx.x / a.kv_heads;
+  if (!a.by_rows)
+    return find_tile(a.k_offsets, a.k_lens, a.k_rows, a.q_offsets, a.q_lens, a.q_rows, a.m, AG_KEYS, number, t);
+  const int64_t i = lane_id() < a.m ? lane_id() : a.m - 1;
+  int64_t first, len, first2, len2;
+  bool ok = segment_ok(a.k_offsets, a.k_lens, i, a.k_rows, first, len) & (lane_id() < a.m), found;
+  ok = ok & segment_ok(a.q_offsets, a.q_lens, i, a.q_rows, first2, len2);
+  find_tile_by_keys(ok, first, len, first2, len2, a.causal ? len : len2, AG_KEYS, a.causal, number, t, found);
+  return found;
+}
+
 // Stages of 64 query rows in LDS: Q, dO, and of every row its shift and D; so many
 // that rows have two steps to arrive.  Behind them, of every row of a step, which
 // of the step's tokens it belongs to.
@@ -264,9 +277,7 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 
   const int kv_head = blockIdx.x % a.kv_heads;
   const int part = gridDim.y - 1 - blockIdx.y;  // tiles of many parts, the long ones, start first
   SegTile t;
-  if (!find_tile(a.k_offsets, a.k_lens, a.k_rows, a.q_offsets, a.q_lens, a.q_rows, a.m, AG_KEYS,
-                 blockIdx.x / a.kv_heads, t))
-    return;
+  if (!find_key_tile(a, t)) return;
   const int k_len = (int)t.len, q_len = (int)t.len2, key0 = (int)t.tile * AG_KEYS, behind = k_len - q_len;
   const RowSteps steps(a.group, q_len, first_token(a, key0, q_len, k_len));
   const int parts = parts_of(steps.count(), a.parts);
@@ -471,9 +482,7 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 
 template <class E, int D> __global__ __launch_bounds__(AG_THREADS) void attention_dkv_join_kernel(GradArgs a) {
   const int kv_head = blockIdx.x % a.kv_heads;
   SegTile t;
-  if (!find_tile(a.k_offsets, a.k_lens, a.k_rows, a.q_offsets, a.q_lens, a.q_rows, a.m, AG_KEYS,
-                 blockIdx.x / a.kv_heads, t))
-    return;
+  if (!find_key_tile(a, t)) return;
   const int k_len = (int)t.len, q_len = (int)t.len2, key0 = (int)t.tile * AG_KEYS;
   const int parts = parts_of(RowSteps(a.group, q_len, first_token(a, key0, q_len, k_len)).count(), a.parts);
   if (parts == 1) return;
@@ -545,6 +554,7 @@ template <class E, int D> static int launch_grad(hipStream_t stream, GradArgs a,
       hipFuncSetAttribute((const void *)dkv, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   if (raised != hipSuccess) return (int)raised;
   a.by_keys = takes_by_keys(units, a.m, a.dim);
+  a.by_rows = a.m <= WAVE && p.tiles <= 2 * NUM_CUS_HINT * (a.dim <= 64 ? 2 : 1);
   if (units > 0) {
     attention_dq_kernel<E, D><<<dim3((unsigned)units), AG_THREADS, 4 * TILE, stream>>>(a);
     const int rc = launch_status();
@@ -605,7 +615,7 @@ extern "C" int fa_attention_grad(fa_stream_t stream, fa_dtype t, const fa_heads 
                       to_heads(dk), to_heads(dv), lse, (float *)workspace, (float *)((char *)workspace + p.row_bytes),
                       (float *)((char *)workspace + 2 * p.row_bytes), q_rows, k_rows, (int)heads, (int)kv_heads,
                       (int)(heads / kv_heads), (int)head_dim, q_offsets, q_lens, k_offsets, k_lens, m, scale,
-                      causal != 0, p.parts, false, failure, code};
+                      causal != 0, p.parts, false, false, failure, code};
   const hipStream_t s = (hipStream_t)stream;
   if (t == FA_F16) return head_dim <= 64 ? launch_grad<ElemF16, 64>(s, a, p) : launch_grad<ElemF16, 128>(s, a, p);
   return head_dim <= 64 ? launch_grad<ElemBF16, 64>(s, a, p) : launch_grad<ElemBF16, 128>(s, a, p);
