@@ -15,8 +15,14 @@ constexpr int AG_STEP = 64;             // keys (query rows) a step
 // rounded output is then off by as much as a rounding of the scores' derivative;
 // rows with fewer keys than this take D from the weights instead.
 constexpr int AG_EXACT_KEYS = 64;
-// Steps that are worth a part of their own when the rows of a key tile are split.
-constexpr int AG_PART_STEPS = 32, AG_MOST_PARTS = 8;
+// A key tile's rows are split into up to AG_MOST_PARTS parts.
+constexpr int AG_MOST_PARTS = 8;
+// Steps that are worth a part of their own, by the rounds that AG_MOST_PARTS of every
+// tile would take: the fewer there are, the longer the chip would wait for the
+// longest tile.  (32 steps, against 4: one sequence of 512, 32 + 8 heads of 128,
+// forward and backward 109 and 70 us, four of up to 700, 8 + 2 heads, 114 and 76;
+// against 8: three of up to 700, 32 + 8 heads, 118 and 89, one of 1024 140 and 127.)
+constexpr int part_steps_for(int64_t rounds) { return rounds <= 1 ? 4 : rounds <= 4 ? 8 : 32; }
 
 struct GradArgs {
   Heads q, k, v, out, dout, dq, dk, dv;
@@ -28,7 +34,7 @@ struct GradArgs {
   const int64_t *q_offsets, *q_lens, *k_offsets, *k_lens;
   int64_t m;
   float scale;
-  int causal, parts;
+  int causal, parts, part_steps;
   bool by_keys, by_rows;  // the order of dq's tiles, and of dk's and dv's
   int32_t *failure, code;
 };
@@ -219,8 +225,8 @@ struct StepAt {
     }
   }
 };
-__device__ __forceinline__ int parts_of(int64_t steps, int most) {
-  const int64_t worth = (steps + AG_PART_STEPS - 1) / AG_PART_STEPS;
+__device__ __forceinline__ int parts_of(int64_t steps, int most, int part_steps) {
+  const int64_t worth = (steps + part_steps - 1) / part_steps;
   return worth < 1 ? 1 : (worth < most ? (int)worth : most);
 }
 // First token that sees a key of the tile from key0 on.
@@ -280,7 +286,7 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 
   if (!find_key_tile(a, t)) return;
   const int k_len = (int)t.len, q_len = (int)t.len2, key0 = (int)t.tile * AG_KEYS, behind = k_len - q_len;
   const RowSteps steps(a.group, q_len, first_token(a, key0, q_len, k_len));
-  const int parts = parts_of(steps.count(), a.parts);
+  const int parts = parts_of(steps.count(), a.parts, a.part_steps);
   if (part >= parts) return;
   const int64_t from = steps.count() * part / parts, to = steps.count() * (part + 1) / parts;
 
@@ -484,7 +490,7 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS) void attentio
   SegTile t;
   if (!find_key_tile(a, t)) return;
   const int k_len = (int)t.len, q_len = (int)t.len2, key0 = (int)t.tile * AG_KEYS;
-  const int parts = parts_of(RowSteps(a.group, q_len, first_token(a, key0, q_len, k_len)).count(), a.parts);
+  const int parts = parts_of(RowSteps(a.group, q_len, first_token(a, key0, q_len, k_len)).count(), a.parts, a.part_steps);
   if (parts == 1) return;
   const int row = threadIdx.x / WAVE * 32 + (lane_id() & 31);
   const bool there = key0 + row < k_len;
@@ -525,7 +531,7 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS) void attentio
 // 64, 71 us with parts and 62 without.
 struct GradPlan {
   int64_t tiles;
-  int parts;
+  int parts, part_steps;
   size_t row_bytes, part_bytes;
 };
 static GradPlan grad_plan(int64_t q_rows, int64_t k_rows, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t m) {
@@ -534,11 +540,12 @@ static GradPlan grad_plan(int64_t q_rows, int64_t k_rows, int64_t heads, int64_t
   const int64_t places = NUM_CUS_HINT * (head_dim <= 64 ? 2 : 1);
   const int64_t wanted = p.tiles > 0 ? ceil_div(3 * places, p.tiles) : 1;
   p.parts = (int)(wanted < AG_MOST_PARTS ? wanted : AG_MOST_PARTS);
+  p.part_steps = part_steps_for(ceil_div(p.tiles * AG_MOST_PARTS, places));
   // no tile has more steps than the rows of one head group make
   const int64_t group = heads / kv_heads, lanes = group < AG_STEP ? group : AG_STEP;
   const int64_t longest = m > 0 && q_rows / m < q_rows / 8 ? 8 * (q_rows / m + 1) : q_rows;
   const int64_t steps = ceil_div(group, lanes) * ceil_div(longest, AG_STEP / lanes);
-  if (p.parts > ceil_div(steps, AG_PART_STEPS)) p.parts = (int)ceil_div(steps, AG_PART_STEPS);
+  if (p.parts > ceil_div(steps, p.part_steps)) p.parts = (int)ceil_div(steps, p.part_steps);
   if (p.parts < 1) p.parts = 1;
   p.row_bytes = (size_t)ceil_div(q_rows * heads, 4) * 16;
   p.part_bytes = p.parts > 1 ? (size_t)p.tiles * p.parts * 2 * AG_KEYS * (head_dim <= 64 ? 64 : 128) * sizeof(float) : 0;
@@ -615,7 +622,7 @@ extern "C" int fa_attention_grad(fa_stream_t stream, fa_dtype t, const fa_heads 
                       to_heads(dk), to_heads(dv), lse, (float *)workspace, (float *)((char *)workspace + p.row_bytes),
                       (float *)((char *)workspace + 2 * p.row_bytes), q_rows, k_rows, (int)heads, (int)kv_heads,
                       (int)(heads / kv_heads), (int)head_dim, q_offsets, q_lens, k_offsets, k_lens, m, scale,
-                      causal != 0, p.parts, false, false, failure, code};
+                      causal != 0, p.parts, p.part_steps, false, false, failure, code};
   const hipStream_t s = (hipStream_t)stream;
   if (t == FA_F16) return head_dim <= 64 ? launch_grad<ElemF16, 64>(s, a, p) : launch_grad<ElemF16, 128>(s, a, p);
   return head_dim <= 64 ? launch_grad<ElemBF16, 64>(s, a, p) : launch_grad<ElemBF16, 128>(s, a, p);
