@@ -3,7 +3,8 @@
 // Both are bound by the matrix units at the clock that power allows, on long
 // sequences 1.2 and 1.08 PFLOP/s of the products they compute (one of 8192 tokens,
 // not causal, 32 + 8 heads of 128: 1.36 and 2.04 ms).  On ragged ones (five of up
-// to 4096: 260 and 420 us) about 13 us of a key tile are its beginning and end.
+// to 4096: 255 and 390 us, the units busy 55 and 43 % of the time) about 13 us of a
+// key tile are its beginning and end.
 #include "attention.hip.h"
 
 namespace fa {
@@ -268,10 +269,11 @@ static __device__ const float g_infinity = INFINITY;  // the shift of a row that
 //   S = Q K^T, dP = dO V^T, dS = P (dP - D), dV^T += dO^T P, dK^T += Q^T dS,
 // with Q and dO read from one tile each by rows and by columns.  The products S
 // and dP of the next 32 rows are issued in turn with the weights of the last, as
-// the order in the source fixes.  (LDS reads take as long as the products: all four
-// waves read the same rows.  64 keys a wave would halve them, but its sums, operands
-// and products need more than the 512 registers of a lane, and the spills took 2.4
-// times as long.)  The keys at the start of a long sequence are
+// the order in the source fixes.  (All four waves read the same rows of LDS; 64 keys
+// a wave would halve those reads, but its sums, operands and products need more than
+// the 512 registers of a lane, and the spills took 2.4 times as long.  From the last
+// step to the first, so that blocks side by side read the same rows: the same time,
+// D = 64 3 % more.)  The keys at the start of a long sequence are
 // seen by all its rows: their rows are split over `parts` blocks, whose sums a
 // second kernel adds in order.
 template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 : 2) void attention_dkv_kernel(GradArgs a) {
