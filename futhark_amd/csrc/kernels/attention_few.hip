@@ -29,9 +29,14 @@ constexpr int FEW_KEYS = 32;        // keys of a tile
 // much longer, or waves that meet many short sequences end last (64 ragged
 // sequences: the last wave at 121 us with the mean at 86 us).
 constexpr int FEW_START = 2;
-// On a short line, where a wave need not begin more than one unit, pieces end
-// with their units and have at least FEW_LEAST tiles.  Short: up to FEW_SHORT of them.
-constexpr int FEW_LEAST = 2, FEW_SHORT = 16;
+// On a short line, where a wave need not begin more than one unit, pieces end with
+// their units and have at least few_least() tiles (32 KiB of keys and values: fewer
+// leave more parts to join, 17 sequences of up to nine tokens, heads of 64, with two
+// tiles 18.6 us and with four 15.7).  Short: up to FEW_SHORT of them; with more,
+// waves that end with a unit lose more than beginning another costs (64 sequences of
+// up to 2048 keys, heads of 128: up to 16 of them 41.5 us, four 31.9).
+constexpr int FEW_SHORT = 4;
+template <int D> constexpr int few_least() { return D == 128 ? 2 : 4; }
 constexpr int FEW_THREADS = 256, FEW_WAVES = FEW_THREADS / WAVE;
 
 // Waves a launch has: what fits the LDS of the chip (four waves of 33 KiB a CU,
@@ -101,7 +106,7 @@ __device__ __forceinline__ int64_t few_sum(const int64_t (&x)[FEW_WAVES], int to
 }
 // Lays out the line, and finds for each wave of the block the thread that counts
 // the place where the wave's piece begins, with the places and units before that.
-__device__ __forceinline__ FewLine few_line(const AttentionArgs &a, int per_tile, FewTable &table) {
+template <int D> __device__ __forceinline__ FewLine few_line(const AttentionArgs &a, int per_tile, FewTable &table) {
   const int waves = gridDim.x * FEW_WAVES;
   FewLine line;
   line.each = (a.m + FEW_THREADS - 1) / FEW_THREADS;
@@ -130,7 +135,7 @@ __device__ __forceinline__ FewLine few_line(const AttentionArgs &a, int per_tile
   line.start = FEW_START;
   if (line.is_short) {
     const uint32_t even = ((uint32_t)all_tiles + (uint32_t)spare - 1) / (uint32_t)spare;
-    line.piece = even < FEW_LEAST ? FEW_LEAST : even;
+    line.piece = even < few_least<D>() ? few_least<D>() : even;
     line.start = 0;
     places = 0;
     for (int64_t i = i0; i < i1; i++) {
@@ -479,7 +484,7 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 ? 1 : 2) void attention_few_k
   const int per_tile = ROWS / a.group;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   const int64_t number = (int64_t)blockIdx.x * FEW_WAVES + wave;
-  const FewLine line = few_line(a, per_tile, seqs);
+  const FewLine line = few_line<D>(a, per_tile, seqs);
   if (blockIdx.x == 0 && threadIdx.x == 0) *few_units(a, ROWS, D) = line.units;
   int64_t at = number * line.piece;
   const int64_t end = at + line.piece < line.total ? at + line.piece : line.total;
@@ -686,13 +691,13 @@ static int64_t few_most_units(int rows, int64_t n, int64_t group, int64_t kv_hea
 }
 
 // Whether a block a unit, in one launch, is the faster way: the units fit the chip
-// at once, and a wave's quarter of the longest table, at about 0.7 us a tile, takes
-// no longer than its piece of the line and the second launch, which is about 10
-// tiles.  (Four sequences of up to 500 keys, 16 units: 7.8 us against 14.9; 17 of up
-// to 3000 with up to nine tokens, 184 units: 22.8 against 18.6.)
-static bool few_in_one_launch(int64_t units, int64_t keys, int64_t waves) {
-  const int64_t tiles = ceil_div(keys, FEW_KEYS);
-  return units * FEW_WAVES <= waves && tiles <= 128 && tiles * waves <= 4 * (10 * waves + tiles * units);
+// at once, and a wave's quarter of the longest table takes no longer than its piece
+// of the line and the second launch.  (Heads of 128, 4 to 32 sequences of up to 512
+// keys 12.7 us against 16 to 19 on the line, of 1040 19 against 17, of 2048 31
+// against 21; heads of 64, 500 keys 9.7 against 13.9, 1040 11.4 against 14.5, 2048
+// 20 against 22 where units fill the chip, 4000 30 against 15.5.)
+template <int D> static bool few_in_one_launch(int64_t units, int64_t keys) {
+  return units * FEW_WAVES <= few_waves<D>() && keys <= (D == 128 ? 1024 : 1536);
 }
 
 size_t few_workspace(int rows, int64_t n, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t m) {
@@ -714,7 +719,7 @@ static int launch_few_of(hipStream_t stream, AttentionArgs a, void *workspace) {
       hipFuncSetAttribute((const void *)short_kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   if (raised != hipSuccess) return (int)raised;
   if (raised_short != hipSuccess) return (int)raised_short;
-  if (few_in_one_launch(units, a.pages.cols << a.pages.page_shift, few_waves<D>())) {
+  if (few_in_one_launch<D>(units, a.pages.cols << a.pages.page_shift)) {
     short_kernel<<<dim3((unsigned)units), FEW_THREADS, LDS, stream>>>(a);
     return launch_status();
   }
@@ -726,7 +731,7 @@ static int launch_few_of(hipStream_t stream, AttentionArgs a, void *workspace) {
   if (rc != 0) return rc;
   // Rows a block of the second kernel joins: as many as its threads hold, fewer
   // while there are less than two blocks a CU (17 sequences with up to nine tokens
-  // 20.0 -> 18.6 us against one a CU; four a CU the same).
+  // 20.0 -> 18.6 us, against one a CU; four a CU the same).
   const int64_t rows = ROWS / a.group * a.group;  // of a unit, at most
   int join_rows = FEW_THREADS / (D / 4);
   while (join_rows > 1 && units * ceil_div(rows, join_rows) < 2 * NUM_CUS_HINT) join_rows /= 2;

@@ -832,3 +832,16 @@ def test_bad_pages_and_lengths_of_many_rows(K):
         f, n = c.segs[1]
         if what != "page high":
             assert bool((c.out[f:f + n] == MARK).all()), what
+
+
+@pytest.mark.parametrize("t,h,hk,dim,page,new,past", [
+    ("bf16", 8, 2, 128, 16, [1] * 9, [1500, 3, 900, 0, 31, 1023, 64, 1499, 700]),       # a short line
+    ("f16", 16, 4, 64, 16, [1] * 9, [2500, 3, 900, 0, 31, 1023, 64, 2499, 700]),
+    ("bf16", 32, 8, 128, 16, [1] * 70, [(61 * i) % 1900 for i in range(70)]),            # units fill half of the waves
+    ("f16", 24, 8, 64, 32, [1, 3, 9, 2, 0, 7] * 6, [(331 * i) % 2200 for i in range(36)]),
+    ("bf16", 32, 32, 128, 16, [1] * 40, [(97 * i) % 1200 for i in range(40)]),           # more units than waves
+])
+def test_lines_of_all_lengths(K, t, h, hk, dim, page, new, past):
+    c = Cache(t, h, hk, dim, page, new, past, seed=99)
+    c.attend(K)
+    c.check()
