@@ -1,5 +1,5 @@
-// What the attention kernels (attention.hip, attention_grad.hip, kv_append.hip)
-// share: argument checks on the host, 16-bit element types, arrays of heads and
+// What the attention kernels (attention.hip, attention_few.hip, attention_grad.hip,
+// kv_append.hip) share: argument checks on the host, 16-bit element types, arrays of heads and
 // the walk over segments on the device.
 #pragma once
 #include "dispatch.hip.h"
@@ -175,8 +175,7 @@ __device__ __forceinline__ bool find_tile(const int64_t *offsets, const int64_t 
 // tiles that see most keys first, whatever segment they are of: started in this
 // order, blocks end together.  A tile's level is the number of keys it sees, in
 // tiles, `seen` keys for the first one: of the one `tile` behind it top - tile if
-// causal, else top;
-// the highest level is found that more than `number` tiles reach.
+// causal, else top.  The highest level is found that more than `number` tiles reach.
 __device__ __forceinline__ void find_tile_by_keys(bool ok, int64_t first, int64_t len, int64_t first2, int64_t len2, int64_t seen,
                                                   int per_tile, bool causal, int64_t number, SegTile &t, bool &found) {
   const int tiles = ok ? (int)(((uint32_t)len + (uint32_t)per_tile - 1) / (uint32_t)per_tile) : 0;
