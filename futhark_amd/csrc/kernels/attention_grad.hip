@@ -160,16 +160,19 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, 2) void atten
     }
   };
   if (last_key(0) < AG_EXACT_KEYS) {
-    float d = 0.0f;
+    // A row of one key has the weight 1, whatever lse's rounding makes of it: its D is
+    // dP itself, so that dP - D is zero here and, with the same products, for dk.
+    float d = 0.0f, only = 0.0f;
     walk([&](const unsigned char *kt, int key0) __attribute__((always_inline)) {
       for (int b = 0; b < AG_STEP; b += 32) {
         f32x16 p, dp;
         weights(kt, key0, b, p, dp);
+        if (key0 + b == 0 && half == 0) only = dp[0];
 #pragma unroll
         for (int i = 0; i < 16; i++) d += p[i] * dp[i];
       }
     });
-    delta = fold_halves(d, FAdd());
+    delta = fold_halves(limit == 0 ? only : d, FAdd());
     __syncthreads();  // the tiles are read again from the start
   }
   if (row < rows && half == 0) {

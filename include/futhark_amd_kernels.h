@@ -394,8 +394,9 @@ int fa_attention(fa_stream_t stream, fa_dtype t, const fa_heads *q, int64_t q_ro
  * what fa_attention returned for the same arguments (out and lse):
  *   D_i = dout_i.out_i,  ds_ij = p_ij (dout_i.v_j - D_i),
  *   dq_i = scale sum_j ds_ij k_j,  dk_j = scale sum_i ds_ij q_i,  dv_j = sum_i p_ij dout_i,
- * dk and dv summed over the query heads of a key head as well.  Rows in no
- * segment keep what they held.  Unlike in fa_attention, non-finite values in a
+ * dk and dv summed over the query heads of a key head as well.  A row that sees
+ * one key has p = 1 and adds exactly zero to dq and dk.  Rows in no segment keep
+ * what they held.  Unlike in fa_attention, non-finite values in a
  * segment may spread to other rows of that segment.  workspace:
  * fa_attention_grad_workspace_bytes() bytes, 16-byte aligned, contents
  * irrelevant. */

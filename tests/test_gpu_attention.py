@@ -845,3 +845,39 @@ def test_lines_of_all_lengths(K, t, h, hk, dim, page, new, past):
     c = Cache(t, h, hk, dim, page, new, past, seed=99)
     c.attend(K)
     c.check()
+
+
+@pytest.mark.parametrize("t", ["bf16", "f16"])
+@pytest.mark.parametrize("h,hk,dim,q_lens,k_lens,causal", [
+    (4, 2, 128, [1] * 70, None, True),               # sequences of one token
+    (3, 1, 64, [1, 1, 1], None, False),
+    (16, 2, 72, [1] * 9, [1] * 9, True),
+    (5, 5, 8, [1], None, True),
+    (2, 1, 128, [2100, 3, 130], [1, 1, 1], False),   # many rows on one key, split into parts
+    (12, 4, 40, [700], [1], False),
+    (4, 2, 64, [40, 1, 200], [1, 1, 1], True),       # rows of nothing before the row of one key
+])
+def test_rows_of_one_key_have_no_gradient(K, t, h, hk, dim, q_lens, k_lens, causal):
+    """A row that sees one key has the weight 1 whatever its score is: the derivative of the score is
+    zero, and with it dq and dk, not the difference of two roundings."""
+    p = Problem(t, h, hk, dim, q_lens, k_lens, causal, seed=101, spread=3.0)
+    p.forward(K)
+    p.backward(K)
+    p.check_backward()
+    for x, segs in ((p.dq, p.segs_q), (p.dk, p.segs_k)):
+        for f, n in segs:
+            assert not bool(x[f:f + n].any())
+
+
+@pytest.mark.parametrize("t,h,hk,dim", [("bf16", 8, 2, 128), ("f16", 6, 6, 64), ("f16", 5, 1, 96)])
+def test_first_rows_of_sequences_have_no_gradient(K, t, h, hk, dim):
+    """The same for the first row of a causal sequence, beside rows that see more, and for the row that
+    sees the first key behind rows that see nothing."""
+    q_lens, k_lens = [2, 64, 300, 1, 90, 130], [2, 64, 300, 1, 40, 129]
+    p = Problem(t, h, hk, dim, q_lens, k_lens, seed=102)
+    p.forward(K)
+    p.backward(K)
+    p.check_backward()
+    for (f, n), (_, kn) in zip(p.segs_q, p.segs_k):
+        assert not bool(p.dq[f:f + n - kn + 1].any())
+        assert n == 1 or bool(p.dq[f + n - kn + 1:f + n].any(-1).all())
