@@ -48,11 +48,14 @@ __device__ __forceinline__ bool find_unit(const AttentionArgs &a, int64_t number
     if constexpr (PAGED) {
       const int64_t past = a.pages.past_lens[i], room = a.pages.capacity();
       const bool fits = past >= 0 && past <= room && len <= room - past;
+      ok = SegChain().keep(ok, first, len, a.q_offsets, a.q_lens, a.m, a.q_rows, 0);
       if (number == 0 && ok && len > 0 && !fits && a.failure != nullptr) *a.failure = a.code;
       ok = ok & fits;
       len2 = past + len;
     } else {
-      ok = ok & segment_ok(a.k_offsets, a.k_lens, i, a.k_rows, first2, len2);
+      const bool ok2 = segment_ok(a.k_offsets, a.k_lens, i, a.k_rows, first2, len2);
+      ok = SegChain().keep(ok, first, len, a.q_offsets, a.q_lens, a.m, a.q_rows, 0) &
+           SegChain().keep(ok2, first2, len2, a.k_offsets, a.k_lens, a.m, a.k_rows, 0);
     }
     find_tile_by_keys(ok, first, len, first2, len2, len2, per_tile, a.causal, number / a.kv_heads, t, found);
     if (!found) return false;

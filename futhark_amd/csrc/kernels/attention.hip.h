@@ -133,10 +133,38 @@ __device__ __forceinline__ bool segment_ok(const int64_t *offsets, const int64_t
   return inside & behind;
 }
 
+// Where a segment ends, 0 for one that does not lie inside [0, n).
+__device__ __forceinline__ int segment_end(int64_t first, int64_t len, int64_t n) {
+  return (first >= 0) & (first <= n) & ((uint64_t)len <= (uint64_t)n - (uint64_t)first) ? (int)(first + len) : 0;
+}
+// A segment that lies behind its predecessor lies behind all earlier ones as long as
+// those keep the rules.  Behind a broken one it has to be compared with all of them.
+// A wave looks at its segments in order, WAVE at a time; this is what goes from one
+// batch to the next.
+struct SegChain {
+  bool broken = false;  // a segment so far breaks the rules; `end` is then the end of all so far
+  int end = 0;
+  // Whether segment base + lane, ok by segment_ok, also starts behind all before it.
+  __device__ __forceinline__ bool keep(bool ok, int64_t first, int64_t len, const int64_t *offsets, const int64_t *lens,
+                                       int64_t m, int64_t n, int64_t base) {
+    const bool live = base + lane_id() < m;
+    if (!broken) {
+      if (!__any(live & !ok)) return ok;
+      broken = true;
+      if (base > 0) end = (int)(offsets[base - 1] + lens[base - 1]);
+    }
+    const int upto = wave_incl_scan<int, OpMax<int>>(live ? segment_end(first, len, n) : 0);
+    const int before = OpMax<int>::apply(wave_shift_up1<int, OpMax<int>>(upto), end);
+    end = OpMax<int>::apply(end, read_lane(upto, WAVE - 1));
+    return ok & (first >= before);
+  }
+};
+
 // Work on a segment comes in tiles of `per_tile` rows, numbered through the
 // segments in order; the tile of number `number`, or false if there are fewer.
 // The same for the whole wave, which looks at 64 segments at a time.  A broken
-// segment (also one whose partner in `offsets2` is broken) has no tiles.
+// segment (also one whose partner in `offsets2` is broken, or that overlaps an
+// earlier one) has no tiles.
 struct SegTile {
   int64_t seg, tile, tiles;  // segment, tile in it, tiles it has
   int64_t first, len;
@@ -146,11 +174,17 @@ __device__ __forceinline__ bool find_tile(const int64_t *offsets, const int64_t 
                                           const int64_t *offsets2, const int64_t *lens2, int64_t n2, int64_t m,
                                           int per_tile, int64_t number, SegTile &t) {
   int64_t before = 0;
+  SegChain chain, chain2;
   for (int64_t base = 0; base < m; base += WAVE) {
     const int64_t i = base + lane_id(), at = i < m ? i : m - 1;
     int64_t f, l, f2 = 0, l2 = 0;
     bool ok = segment_ok(offsets, lens, at, n, f, l) & (i < m);
-    if (offsets2 != nullptr) ok = ok & segment_ok(offsets2, lens2, at, n2, f2, l2);
+    if (offsets2 != nullptr) {
+      const bool ok2 = segment_ok(offsets2, lens2, at, n2, f2, l2);
+      ok = chain.keep(ok, f, l, offsets, lens, m, n, base) & chain2.keep(ok2, f2, l2, offsets2, lens2, m, n2, base);
+    } else {
+      ok = chain.keep(ok, f, l, offsets, lens, m, n, base);
+    }
     // lengths are below 2^31
     const int64_t tiles = ok ? ((uint32_t)l + (uint32_t)per_tile - 1) / (uint32_t)per_tile : 0;
     const int64_t upto = before + wave_incl_scan<int64_t, OpAdd<int64_t>>(tiles);

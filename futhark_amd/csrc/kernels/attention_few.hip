@@ -55,30 +55,40 @@ struct FewSeq {
   __device__ __forceinline__ int key_tiles() const { return (int)(((int64_t)past + len + FEW_KEYS - 1) / FEW_KEYS); }
   __device__ __forceinline__ int64_t units(int kv_heads) const { return (int64_t)row_tiles * kv_heads; }
 };
-__device__ __forceinline__ FewSeq few_seq(const AttentionArgs &a, int per_tile, int64_t i, bool report) {
-  FewSeq s = {0, 0, 0, 0};
-  int64_t first, len;
-  const int64_t past = a.pages.past_lens[i], room = a.pages.capacity();
-  bool ok = segment_ok(a.q_offsets, a.q_lens, i, a.q_rows, first, len);
-  ok = ok && (len == 0 || (past >= 0 && past <= room && len <= room - past));
-  if (ok) {
-    s.first = (int)first;
-    s.past = len > 0 ? (int)past : 0;
-    s.len = (int)len;
-    s.row_tiles = (int)(((uint32_t)len + (uint32_t)per_tile - 1) / (uint32_t)per_tile);
-  } else if (report && a.failure != nullptr) {
-    *a.failure = a.code;
+// Segment i as the arrays have it.
+struct FewSegment {
+  int64_t first, len, past;
+  bool ok;  // by segment_ok
+  __device__ __forceinline__ FewSegment(const AttentionArgs &a, int64_t i) {
+    past = a.pages.past_lens[i];
+    ok = segment_ok(a.q_offsets, a.q_lens, i, a.q_rows, first, len);
   }
-  return s;
-}
+  __device__ __forceinline__ int end(const AttentionArgs &a) const { return segment_end(first, len, a.q_rows); }
+  // The sequence, of no tokens unless `kept` and its cached ones fit the table.
+  __device__ __forceinline__ FewSeq seq(const AttentionArgs &a, int per_tile, bool kept, bool report) const {
+    FewSeq s = {0, 0, 0, 0};
+    const int64_t room = a.pages.capacity();
+    if (kept && (len == 0 || (past >= 0 && past <= room && len <= room - past))) {
+      s.first = (int)first;
+      s.past = len > 0 ? (int)past : 0;
+      s.len = (int)len;
+      s.row_tiles = (int)(((uint32_t)len + (uint32_t)per_tile - 1) / (uint32_t)per_tile);
+    } else if (report && a.failure != nullptr) {
+      *a.failure = a.code;
+    }
+    return s;
+  }
+};
 
 // What a block knows of the line.  Thread t counts the sequences t * each ..
 // (t + 1) * each - 1.  Up to FEW_THREADS sequences are kept.
 struct FewTable {
   int64_t tiles[FEW_WAVES], units[FEW_WAVES], places[FEW_WAVES];  // a wave's threads count
+  int ends[FEW_WAVES];  // the largest end of their segments
   // Where the pieces of the block's waves begin: the thread that counts the
-  // place, and the places and units before those it counts.
-  int thread[FEW_WAVES];
+  // place, the places and units before those it counts, and, if any segment is
+  // broken, the largest end of the segments before them (else -1).
+  int thread[FEW_WAVES], reach[FEW_WAVES];
   int64_t before[FEW_WAVES], units_before[FEW_WAVES];
   FewSeq seq[FEW_THREADS];
 };
@@ -89,8 +99,15 @@ struct FewLine {
   int start;             // places of a unit before its tiles
   bool is_short;
   const FewTable *table;
-  __device__ __forceinline__ FewSeq seq(const AttentionArgs &a, int per_tile, int64_t i) const {
-    return each == 1 ? table->seq[i] : few_seq(a, per_tile, i, false);
+  // A sequence, `reach` being that of the segments before it.
+  __device__ __forceinline__ FewSeq seq(const AttentionArgs &a, int per_tile, int64_t i, const int &reach) const {
+    if (each == 1) return table->seq[i];
+    const FewSegment g(a, i);
+    return g.seq(a, per_tile, g.ok && g.first >= reach, false);
+  }
+  // Takes `reach` behind sequence i.
+  __device__ __forceinline__ void pass(const AttentionArgs &a, int64_t i, int &reach) const {
+    if (each > 1 && reach >= 0) reach = OpMax<int>::apply(reach, FewSegment(a, i).end(a));
   }
   // Places of a unit; a short line pads it to whole pieces.
   __device__ __forceinline__ int unit(const FewSeq &s) const {
@@ -114,17 +131,38 @@ template <int D> __device__ __forceinline__ FewLine few_line(const AttentionArgs
   const int64_t i0 = threadIdx.x * line.each, i1 = i0 + line.each < a.m ? i0 + line.each : a.m;
   const int wave = threadIdx.x / WAVE;
   FewSeq s = {0, 0, 0, 0};
-  int64_t tiles = 0, units = 0;
-  for (int64_t i = i0; i < i1; i++) {
-    s = few_seq(a, per_tile, i, blockIdx.x == 0);
-    units += s.units(a.kv_heads);
-    tiles += s.units(a.kv_heads) * s.key_tiles();
+  int64_t tiles, units, units_upto, tiles_upto;
+  int reach = -1;
+  for (;;) {
+    bool whole = true;
+    int end = reach;
+    tiles = units = 0;
+    for (int64_t i = i0; i < i1; i++) {
+      const FewSegment g(a, i);
+      s = g.seq(a, per_tile, g.ok && (reach < 0 || g.first >= end), blockIdx.x == 0);
+      units += s.units(a.kv_heads);
+      tiles += s.units(a.kv_heads) * s.key_tiles();
+      whole = whole && g.ok;
+      end = OpMax<int>::apply(end, g.end(a));
+    }
+    table.seq[threadIdx.x] = s;
+    units_upto = wave_incl_scan<int64_t, OpAdd<int64_t>>(units);
+    tiles_upto = wave_incl_scan<int64_t, OpAdd<int64_t>>(tiles);
+    if (reach < 0 && !__all(whole)) tiles_upto = -1;  // (of segments that do not count)
+    if (lane_id() == WAVE - 1) table.tiles[wave] = tiles_upto, table.units[wave] = units_upto;
+    __syncthreads();
+    int64_t least = 0;
+#pragma unroll
+    for (int w = 0; w < FEW_WAVES; w++) least = OpMin<int64_t>::apply(least, table.tiles[w]);
+    if (least == 0) break;  // (the same for the whole block)
+    // Once more, with where the segments before end.
+    const int ends = wave_incl_scan<int, OpMax<int>>(end);
+    if (lane_id() == WAVE - 1) table.ends[wave] = ends;
+    __syncthreads();
+    reach = OpMax<int>::apply(0, wave_shift_up1<int, OpMax<int>>(ends));
+#pragma unroll
+    for (int w = 0; w < FEW_WAVES; w++) reach = w < wave ? OpMax<int>::apply(reach, table.ends[w]) : reach;
   }
-  table.seq[threadIdx.x] = s;
-  const int64_t units_upto = wave_incl_scan<int64_t, OpAdd<int64_t>>(units);
-  const int64_t tiles_upto = wave_incl_scan<int64_t, OpAdd<int64_t>>(tiles);
-  if (lane_id() == WAVE - 1) table.tiles[wave] = tiles_upto, table.units[wave] = units_upto;
-  __syncthreads();
   const int64_t all_units = few_sum(table.units, FEW_WAVES), all_tiles = few_sum(table.tiles, FEW_WAVES);
   // Pieces of this many tiles are at most as many as there are waves: every unit
   // has at most one that is not full.
@@ -138,8 +176,10 @@ template <int D> __device__ __forceinline__ FewLine few_line(const AttentionArgs
     line.piece = even < few_least<D>() ? few_least<D>() : even;
     line.start = 0;
     places = 0;
+    int before = reach;
     for (int64_t i = i0; i < i1; i++) {
-      if (line.each > 1) s = few_seq(a, per_tile, i, false);
+      if (line.each > 1) s = line.seq(a, per_tile, i, before);
+      line.pass(a, i, before);
       places += s.units(a.kv_heads) * line.unit(s);
     }
   }
@@ -155,6 +195,7 @@ template <int D> __device__ __forceinline__ FewLine few_line(const AttentionArgs
     const int64_t at = ((int64_t)blockIdx.x * FEW_WAVES + w) * line.piece;
     if (at >= before && at < before + places) {
       table.thread[w] = threadIdx.x;
+      table.reach[w] = reach;
       table.before[w] = before;
       table.units_before[w] = units_here;
     }
@@ -495,12 +536,13 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 ? 1 : 2) void attention_few_k
   int64_t seq = __builtin_amdgcn_readfirstlane(seqs.thread[wave]) * line.each;
   int64_t precede = seqs.before[wave], units_before = seqs.units_before[wave];
   while (at < end) {
-    const FewSeq s = line.seq(a, per_tile, seq);
+    const FewSeq s = line.seq(a, per_tile, seq, seqs.reach[wave]);
     const int length = line.unit(s);
     const int64_t places = s.units(a.kv_heads) * length;
     if (at >= precede + places) {
       precede += places;
       units_before += s.units(a.kv_heads);
+      line.pass(a, seq, seqs.reach[wave]);
       seq++;
       continue;
     }
@@ -539,13 +581,18 @@ __global__ __launch_bounds__(FEW_THREADS, D == 128 ? 1 : 2) void attention_few_s
   const int per_tile = ROWS / a.group, lane = lane_id();
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
   if (blockIdx.x == 0)
-    for (int64_t i = threadIdx.x; i < a.m; i += FEW_THREADS) few_seq(a, per_tile, i, true);
+    for (int64_t i = threadIdx.x; i < a.m; i += FEW_THREADS) {
+      const FewSegment g(a, i);
+      g.seq(a, per_tile, g.ok, true);
+    }
   // The sequence of this unit; every wave looks.
   FewSeq s;
   int64_t seq = -1, before = 0;
+  SegChain chain;
   for (int64_t base = 0; base < a.m && seq < 0; base += WAVE) {
-    const int64_t i = base + lane;
-    const FewSeq mine = i < a.m ? few_seq(a, per_tile, i, false) : FewSeq{0, 0, 0, 0};
+    const FewSegment g(a, base + lane < a.m ? base + lane : a.m - 1);
+    const bool kept = chain.keep(g.ok & (base + lane < a.m), g.first, g.len, a.q_offsets, a.q_lens, a.m, a.q_rows, base);
+    const FewSeq mine = g.seq(a, per_tile, kept, false);
     const int64_t units = mine.units(a.kv_heads);
     const int64_t upto = before + wave_incl_scan<int64_t, OpAdd<int64_t>>(units);
     const uint64_t past = __ballot(upto > (int64_t)blockIdx.x);

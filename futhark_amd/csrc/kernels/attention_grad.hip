@@ -68,7 +68,9 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, 2) void atten
     const int64_t i = lane_id() < a.m ? lane_id() : a.m - 1;
     int64_t first, len, first2, len2;
     bool ok = segment_ok(a.q_offsets, a.q_lens, i, a.q_rows, first, len) & (lane_id() < a.m), found;
-    ok = ok & segment_ok(a.k_offsets, a.k_lens, i, a.k_rows, first2, len2);
+    const bool ok2 = segment_ok(a.k_offsets, a.k_lens, i, a.k_rows, first2, len2);
+    ok = SegChain().keep(ok, first, len, a.q_offsets, a.q_lens, a.m, a.q_rows, 0) &
+         SegChain().keep(ok2, first2, len2, a.k_offsets, a.k_lens, a.m, a.k_rows, 0);
     find_tile_by_keys(ok, first, len, first2, len2, len2, per_tile, a.causal, blockIdx.x / a.kv_heads, t, found);
     if (!found) return;
   } else if (!find_tile(a.q_offsets, a.q_lens, a.q_rows, a.k_offsets, a.k_lens, a.k_rows, a.m, per_tile,
@@ -252,7 +254,9 @@ __device__ __forceinline__ bool find_key_tile(const GradArgs &a, SegTile &t) {
   const int64_t i = lane_id() < a.m ? lane_id() : a.m - 1;
   int64_t first, len, first2, len2;
   bool ok = segment_ok(a.k_offsets, a.k_lens, i, a.k_rows, first, len) & (lane_id() < a.m), found;
-  ok = ok & segment_ok(a.q_offsets, a.q_lens, i, a.q_rows, first2, len2);
+  const bool ok2 = segment_ok(a.q_offsets, a.q_lens, i, a.q_rows, first2, len2);
+  ok = SegChain().keep(ok, first, len, a.k_offsets, a.k_lens, a.m, a.k_rows, 0) &
+       SegChain().keep(ok2, first2, len2, a.q_offsets, a.q_lens, a.m, a.q_rows, 0);
   find_tile_by_keys(ok, first, len, first2, len2, a.causal ? len : len2, AG_KEYS, a.causal, number, t, found);
   return found;
 }
@@ -313,7 +317,7 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 
   const uint32_t lds_base = lds_address(lds);
   clear_unloaded<D>(lds, L::TOKENS, a.dim);
   int *tokens_of = reinterpret_cast<int *>(lds + L::TOKENS);
-  if (threadIdx.x < AG_STEP) tokens_of[threadIdx.x] = threadIdx.x / steps.heads;
+  if (wave < 2) tokens_of[lane] = lane / steps.heads;  // (both, for their own loads below)
   // Row r of a step is token r / heads, head r % heads of the step's.  The usual
   // case: all rows of a step used, and within 32-bit offsets of its first.
   const bool near = steps.tokens * steps.heads == AG_STEP &&
@@ -328,7 +332,6 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 
   }
   // Loads of a step: FETCHES of every wave, and one more of the first two.
   constexpr int FETCHES = 2 * TileLoads<D, AG_THREADS>::COUNT;
-  const int my_token = lane / steps.heads, my_head = lane % steps.heads;
   const auto fetch = [&](const StepAt &s, int stage) __attribute__((always_inline)) {
     const uint32_t q_tile = lds_base + stage * L::BYTES, g_tile = q_tile + TILE;
     const int head = kv_head * a.group + s.head;
@@ -353,6 +356,7 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 
       }
     }
     if (wave < 2) {
+      const int my_token = tokens_of[lane], my_head = lane - my_token * steps.heads;
       const bool there = my_token < steps.tokens && s.token + my_token < q_len && s.head + my_head < a.group;
       const float *src = (wave == 0 ? a.shift : a.delta) + (t.first2 + s.token + my_token) * a.heads + head + my_head;
       const void *none = wave == 0 ? (const void *)&g_infinity : (const void *)&g_zeros;

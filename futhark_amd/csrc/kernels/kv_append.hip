@@ -34,10 +34,12 @@ template <int N> struct Look {
     }
   }
   // The number of the row's segment from `base` on, or -1.
-  __device__ __forceinline__ int find(int64_t row, int64_t &f, int64_t &l, int64_t &p) const {
+  __device__ __forceinline__ int find(int64_t row, const int64_t *offsets, const int64_t *lens, int64_t m, int64_t n, int64_t base,
+                                      SegChain &chain, int64_t &f, int64_t &l, int64_t &p) const {
 #pragma unroll
     for (int j = 0; j < N; j++) {
-      const uint64_t found = __ballot(ok[j] && row >= first[j] && row < first[j] + len[j]);
+      const bool kept = chain.keep(ok[j], first[j], len[j], offsets, lens, m, n, base + j * WAVE);
+      const uint64_t found = __ballot(kept && row >= first[j] && row < first[j] + len[j]);
       if (found != 0) {
         const int at = __builtin_ctzll(found);
         f = read_lane(first[j], at);
@@ -95,11 +97,12 @@ template <class E> __global__ __launch_bounds__(KA_THREADS) void kv_append_kerne
     mine[j] = bit_cast<uint4>(__builtin_nontemporal_load(reinterpret_cast<const i32x4 *>(src + i % per_row * 8)));
   }
   int64_t first, len, past;
-  int64_t seg = nearest.find(row, first, len, past);
+  SegChain chain;
+  int64_t seg = nearest.find(row, a.offsets, a.lens, a.m, a.n, 0, chain, first, len, past);
   for (int64_t base = WAVE; seg < 0 && base < a.m; base += WAVE * KA_SEGMENTS) {
     Look<KA_SEGMENTS> more;
     more.load(a.offsets, a.lens, a.pages.past_lens, a.m, a.n, base);
-    const int at = more.find(row, first, len, past);
+    const int at = more.find(row, a.offsets, a.lens, a.m, a.n, base, chain, first, len, past);
     if (at >= 0) seg = base + at;
   }
   if (blockIdx.x == 0 && blockIdx.y == 0) report_segments(a.offsets, a.lens, a.m, a.n, a.failure, a.code);

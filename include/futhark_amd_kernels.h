@@ -358,7 +358,9 @@ int fa_matmul_ws(fa_stream_t stream, fa_dtype in_t,
  * A segment that breaks the rules (or has a length or page number out of range,
  * below) is detected on the device: `code` is stored into *failure
  * (device-visible memory; NULL: not reported), the segment is left out, and
- * nothing outside the arrays is touched.
+ * nothing outside the arrays is touched.  Left out with it are a segment right
+ * behind one that does not lie inside the rows, and every later one that does not
+ * start behind all earlier ones: of segments that overlap, the first counts.
  *
  * Nothing is allocated and no state is kept between calls: launches may be
  * captured into a graph, and calls on several streams (captured ones too) may

@@ -881,3 +881,121 @@ def test_first_rows_of_sequences_have_no_gradient(K, t, h, hk, dim):
     for (f, n), (_, kn) in zip(p.segs_q, p.segs_k):
         assert not bool(p.dq[f:f + n - kn + 1].any())
         assert n == 1 or bool(p.dq[f + n - kn + 1:f + n].any(-1).all())
+
+
+# --------------------------------------------------------- segments that break the rules
+def kept_segments(offsets, lens, n):
+    """The numbers of the segments that are not left out, by the header's rules."""
+    kept, reach = [], 0
+    for i, (f, l) in enumerate(zip(offsets, lens)):
+        inside = 0 <= f <= n and 0 <= l <= n - f
+        ok = inside and f >= reach
+        if i > 0:
+            pf, pl = offsets[i - 1], lens[i - 1]
+            ok = ok and 0 <= pf <= n and 0 <= pl <= n - pf
+        if ok:
+            kept.append(i)
+        if inside:
+            reach = max(reach, f + l)
+    return kept
+
+
+# A broken segment and what comes behind it, in units of rows from the first one on.
+BROKEN = {
+    "overlap behind an overlap": [(0, 10), (5, 1), (6, 10), (16, 2)],
+    "far behind it": [(0, 20), (2, 1), (3, 1), (4, 0), (4, 9), (13, 4), (17, 8), (25, 3)],
+    "outside": [(0, 10), (4, 1 << 40), (6, 10), (16, 2)],
+    "negative": [(0, 10), (4, -1), (6, 10), (16, 2), (18, 1)],
+    "backwards": [(4, 10), (0, 4), (4, 10), (14, 2)],
+}
+
+
+def broken_segments(what, m, unit, at=None):
+    """m segments of `unit` rows, some of none, with the broken ones from number `at` on; offsets and
+    lengths, and the rows they need."""
+    at = m // 2 if at is None else at
+    offsets, lens, first = [], [], 0
+    for i in range(at):
+        offsets.append(first)
+        lens.append(0 if i % 7 == 3 else unit)
+        first += lens[-1]
+    for f, l in BROKEN[what]:
+        offsets.append(first + f * unit)
+        lens.append(l * unit if abs(l) < 1 << 30 else l)
+    first = offsets[-1] + lens[-1]
+    while len(offsets) < m:
+        offsets.append(first)
+        lens.append(unit)
+        first += unit
+    return offsets, lens, first
+
+
+@pytest.mark.parametrize("what", BROKEN)
+@pytest.mark.parametrize("m,unit,at", [(8, 7, 0), (40, 3, None), (200, 2, 62), (200, 2, 63), (300, 1, 127)])
+def test_segments_that_overlap_are_left_out(K, what, m, unit, at):
+    """Of segments that overlap the first counts, however many broken ones lie between."""
+    offsets, lens, rows = broken_segments(what, m, unit, at)
+    rows += 3
+    kept = kept_segments(offsets, lens, rows)
+    assert 0 < len(kept) < len(offsets)
+    t, h, hk, dim = "bf16", 4, 2, 64
+    p = Problem(t, h, hk, dim, [rows], seed=110)
+    rows = p.nq
+    for x in (p.qo, p.ko):
+        x.resize_(len(offsets)).copy_(torch.tensor(offsets))
+    for x in (p.ql, p.kl):
+        x.resize_(len(lens)).copy_(torch.tensor(lens))
+    p.segs_q = p.segs_k = list(zip(offsets, lens))
+    p.forward(K)
+    p.backward(K)
+    assert p.failure.item() == 5
+    p.failure.zero_()
+    p.segs_q = p.segs_k = [(offsets[i], lens[i]) for i in kept_segments(offsets, lens, rows)]
+    p.check_forward()
+    p.check_backward()
+
+
+def broken_cache(t, h, hk, dim, page, what, m, unit, at, past_of, extra_cols, seed):
+    offsets, lens, rows = broken_segments(what, m, unit, at)
+    new = [l if 0 <= l < 1 << 30 else unit for l in lens]
+    c = Cache(t, h, hk, dim, page, new, [past_of(i) for i in range(len(new))], seed=seed, extra_cols=extra_cols)
+    assert c.n >= rows
+    c.offsets.copy_(torch.tensor(offsets))
+    c.lens.copy_(torch.tensor(lens))
+    return c, kept_segments(offsets, lens, c.n), list(zip(offsets, lens))
+
+
+def only_kept(c, kept, segs):
+    assert c.failure.item() == 6
+    c.failure.zero_()
+    c.segs, c.past, c.table = [segs[i] for i in kept], [c.past[i] for i in kept], c.table[kept]
+
+
+@pytest.mark.parametrize("what", BROKEN)
+@pytest.mark.parametrize("h,hk,dim,m,unit,at,most_past,extra_cols", [
+    (4, 2, 64, 12, 1, 0, 300, 0),        # a block a unit
+    (4, 2, 128, 80, 1, 61, 90, 0),       # the same, several batches of segments
+    (4, 2, 64, 12, 1, 3, 1900, 99),      # a short line
+    (8, 8, 64, 200, 1, 100, 1700, 0),    # a line, a sequence a thread
+    (2, 1, 64, 700, 1, 254, 90, 99),     # a line, several sequences a thread
+    (8, 8, 64, 700, 1, 440, 120, 99),
+    (4, 2, 64, 12, 40, 3, 90, 0),        # many rows
+    (4, 2, 128, 80, 33, 62, 300, 0),     # the same, tiles in the order of the segments
+])
+def test_cached_segments_that_overlap_are_left_out(K, what, h, hk, dim, m, unit, at, most_past, extra_cols):
+    c, kept, segs = broken_cache("f16", h, hk, dim, 16, what, m, unit, at, lambda i: (37 * i) % most_past, extra_cols, 111)
+    assert 0 < len(kept) < len(segs)
+    c.attend(K)
+    only_kept(c, kept, segs)
+    c.check()
+
+
+@pytest.mark.parametrize("what", BROKEN)
+@pytest.mark.parametrize("m,unit,at", [(12, 5, 0), (80, 3, 62), (700, 1, 318), (700, 2, 400)])
+def test_appended_segments_that_overlap_are_left_out(K, what, m, unit, at):
+    c, kept, segs = broken_cache("f16", 2, 1, 64, 16, what, m, unit, at, lambda i: (11 * i) % 50, 0, 112)
+    freqs = torch.tensor([10000.0 ** (-j / 32) for j in range(32)], dtype=torch.float32, device=DEV)
+    kp, vp = c.kp.clone(), c.vp.clone()
+    c.append(K, freqs, 64, False)
+    only_kept(c, kept, segs)
+    check_append(c, kp, vp, freqs, 64, False)
