@@ -290,6 +290,10 @@ template <class E, int D> __global__ __launch_bounds__(AG_THREADS, D == 128 ? 1 
   extern __shared__ __align__(16) unsigned char lds[];
   const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), half = lane >> 5;
   const int kv_head = blockIdx.x % a.kv_heads;
+  if (a.q_rows == 0 && blockIdx.x == 0 && blockIdx.y == 0) {  // (without query rows the dq kernel is not launched)
+    report_segments(a.q_offsets, a.q_lens, a.m, a.q_rows, a.failure, a.code);
+    report_segments(a.k_offsets, a.k_lens, a.m, a.k_rows, a.failure, a.code);
+  }
   const int part = gridDim.y - 1 - blockIdx.y;  // tiles of many parts, the long ones, start first
   SegTile t;
   if (!find_key_tile(a, t)) return;

@@ -361,6 +361,8 @@ int fa_matmul_ws(fa_stream_t stream, fa_dtype in_t,
  * nothing outside the arrays is touched.  Left out with it are a segment right
  * behind one that does not lie inside the rows, and every later one that does not
  * start behind all earlier ones: of segments that overlap, the first counts.
+ * A call that has no rows to write (no query rows, and for the gradient no rows at
+ * all; no new tokens) returns at once and looks at no segment.
  *
  * Nothing is allocated and no state is kept between calls: launches may be
  * captured into a graph, and calls on several streams (captured ones too) may

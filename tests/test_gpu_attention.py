@@ -999,3 +999,23 @@ def test_appended_segments_that_overlap_are_left_out(K, what, m, unit, at):
     c.append(K, freqs, 64, False)
     only_kept(c, kept, segs)
     check_append(c, kp, vp, freqs, 64, False)
+
+
+@pytest.mark.parametrize("which,what", [("kl", 1 << 40), ("ko", -1), ("ql", 1), ("qo", 2)])
+def test_gradient_without_query_rows_reports_broken_segments(K, which, what):
+    """Keys nobody asks have gradients of zero, written by the second kernel alone."""
+    for broken in (False, True):
+        p = Problem("bf16", 4, 2, 64, [0, 0, 0], [40, 50, 60], seed=113)
+        p.nq = 0
+        if broken:
+            getattr(p, which)[1] = what
+        p.backward(K)
+        assert p.failure.item() == (5 if broken else 0)
+        kept = [0] if broken else [0, 1, 2]  # the one behind a segment outside the rows is left out too
+        for x in (p.dk, p.dv):
+            for f, n in [p.segs_k[i] for i in kept]:
+                assert bool((x[f:f + n] == 0).all())
+            if broken:
+                f, n = p.segs_k[1]
+                assert bool((x[f:f + n] == MARK).all())
+        assert bool((p.dq == MARK).all())
