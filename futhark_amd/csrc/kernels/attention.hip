@@ -369,7 +369,7 @@ template <class E, int D> __global__ __launch_bounds__(AT_THREADS) void attentio
   const int keys = u.t0 + u.tokens + u.k_len - u.q_len, dt = blockIdx.y;
   if (keys <= a.chunk || dt * 32 >= a.dim) return;
   const int row = threadIdx.x / WAVE * 32 + (lane_id() & 31), rows = u.tokens * a.group;
-  const int splits = (keys + a.chunk - 1) / a.chunk;
+  const int splits = (keys - 1) / a.chunk + 1;  // (the sum of the two may pass 2^31)
   float top = -INFINITY;
   for (int s = 0; s < splits; s++) top = fmaxf(top, part_ml(a, blockIdx.x, s, row)[0]);
   const float shift = top == -INFINITY ? 0.0f : top;

@@ -1019,3 +1019,35 @@ def test_gradient_without_query_rows_reports_broken_segments(K, which, what):
                 f, n = p.segs_k[1]
                 assert bool((x[f:f + n] == MARK).all())
         assert bool((p.dq == MARK).all())
+
+
+@pytest.mark.parametrize("n", [1, 100])  # few rows; many rows, whose keys are split
+def test_the_longest_table(K, n):
+    """2^31 - 2^20 positions, the same page over and over: a page's slot counts as often as it is seen.
+    (f32 sums of a part, of chunk = 2^31 / 512 keys here: weights chunk / 2 additions in a row, outputs
+    at most 17 / 16 chunk, each off by 2^-24 of what it adds to.)"""
+    t, dim, page, cols = "bf16", 8, 1 << 20, 2047
+    k, v = randn(generator(120), t, page, dim), (randn(generator(121), t, page, dim, scale=0.1).float() + 1).to(ref.DTYPE[t])
+    q = randn(generator(122), t, n, 1, dim)
+    out, lse = torch.full_like(q, MARK), torch.full((n, 1), MARK, dtype=torch.float32, device=DEV)
+    table = torch.zeros(1, cols, dtype=torch.int32, device=DEV)
+    off, lens = device_segments([(0, n)])
+    past = torch.tensor([cols * page - n], dtype=torch.int64, device=DEV)
+    fail = torch.zeros(1, dtype=torch.int32, device=DEV)
+    scale = 1 / math.sqrt(dim)
+    size = K.attention_paged_workspace_bytes(n, 1, 1, dim, 1, page, cols)
+    ws = torch.empty(max(size, 1), dtype=torch.uint8, device=DEV)
+    K.attention_paged(stream(), t, view(q), n, 1, 1, dim, off.data_ptr(), lens.data_ptr(), 1, past.data_ptr(), scale,
+                      k.data_ptr(), v.data_ptr(), 1, page, table.data_ptr(), cols, view(out), lse.data_ptr(),
+                      ws.data_ptr(), size, fail.data_ptr(), 1)
+    kd, vd = k.double(), v.double()
+    chunk = 2 ** 31 / 512
+    for i in sorted({0, n // 2, n - 1}):
+        s = kd @ q[i, 0].double() * scale
+        times = cols - (torch.arange(page, device=DEV) >= page - n + i + 1).double()
+        w = times * torch.exp(s - s.max())
+        o, l = (w @ vd) / w.sum(), s.max() + torch.log(w.sum())
+        rel = chunk / 2 * 2.0 ** -24 + chunk * 17 / 16 * 2.0 ** -24 + 4 * ref.U[t]
+        assert bool(((out[i, 0].double() - o).abs() <= rel * o.abs()).all()), (i, out[i, 0], o)
+        assert abs(lse[i, 0].item() - l.item()) <= -math.log(1 - chunk / 2 * 2.0 ** -24) + 0.01, (i, lse[i, 0], l)
+    assert fail.item() == 0
