@@ -444,7 +444,7 @@ extern "C" int fa_attention(fa_stream_t stream, fa_dtype t, const fa_heads *q, i
   if (rc == 0) rc = check_segments(q_offsets, q_lens, m, q_rows);
   if (rc == 0) rc = check_segments(k_offsets, k_lens, m, k_rows);
   if (rc != 0) return rc;
-  if (!(scale > 0.0f) || !(scale <= FLT_MAX)) return FA_EINVAL;
+  if ((rc = check_scale(scale)) != 0) return rc;
   if (q_rows == 0 || m == 0) return 0;
   rc = check_heads(q, q_rows, heads, head_dim, false);
   if (rc == 0) rc = check_heads(k, k_rows, kv_heads, head_dim, false);
@@ -491,7 +491,7 @@ extern "C" int fa_attention_paged(fa_stream_t stream, fa_dtype t, const fa_heads
   int rc = check_shape(t, heads, kv_heads, head_dim);
   if (rc == 0) rc = check_segments(offsets, lens, m, n);
   if (rc != 0) return rc;
-  if (!(scale > 0.0f) || !(scale <= FLT_MAX)) return FA_EINVAL;
+  if ((rc = check_scale(scale)) != 0) return rc;
   if (n == 0 || m == 0) return 0;
   rc = check_heads(q, n, heads, head_dim, false);
   if (rc == 0) rc = check_heads(out, n, heads, head_dim, true);

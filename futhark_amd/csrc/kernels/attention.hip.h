@@ -512,6 +512,9 @@ constexpr int64_t AT_MOST_BLOCKS = ((int64_t)1 << 24) - 1;
 // Most rows and positions: 32-bit numbers that may run a few tiles past them.
 constexpr int64_t AT_MOST_ROWS = INT32_MAX - 4095;
 
+// Scores are scaled by scale * log2(e), in f32.
+inline int check_scale(float scale) { return scale > 0.0f && scale * LOG2E <= FLT_MAX ? 0 : FA_EINVAL; }
+
 inline int check_segments(const int64_t *offsets, const int64_t *lens, int64_t m, int64_t n) {
   if (m < 0 || n < 0) return FA_EINVAL;
   if (m > AT_MOST_ROWS || n > AT_MOST_ROWS) return FA_ENOTSUP;

@@ -614,7 +614,7 @@ extern "C" int fa_attention_grad(fa_stream_t stream, fa_dtype t, const fa_heads 
   if (rc == 0) rc = check_segments(q_offsets, q_lens, m, q_rows);
   if (rc == 0) rc = check_segments(k_offsets, k_lens, m, k_rows);
   if (rc != 0) return rc;
-  if (!(scale > 0.0f) || !(scale <= FLT_MAX)) return FA_EINVAL;
+  if ((rc = check_scale(scale)) != 0) return rc;
   if (m == 0 || (q_rows == 0 && k_rows == 0)) return 0;
   rc = check_heads(q, q_rows, heads, head_dim, false);
   if (rc == 0) rc = check_heads(k, k_rows, kv_heads, head_dim, false);

@@ -384,8 +384,9 @@ typedef struct fa_heads {
  * key).  A row that sees no key, or only keys of score -inf, gives out = 0 and
  * lse = -inf.  Keys that a row does not see have no effect on it, whatever
  * values they hold; a NaN among the scores it sees makes its out and lse NaN.
- * scale is positive and finite.  lse: [q_rows][heads] f32, or NULL.  A pair of q
- * and k segments where either is invalid is left out. */
+ * scale is positive and at most FLT_MAX / log2(e), 2.358e38 (FA_EINVAL).  lse:
+ * [q_rows][heads] f32, or NULL.  A pair of q and k segments where either is
+ * invalid is left out. */
 int fa_attention(fa_stream_t stream, fa_dtype t, const fa_heads *q, int64_t q_rows,
                  const fa_heads *k, const fa_heads *v, int64_t k_rows,
                  int64_t heads, int64_t kv_heads, int64_t head_dim,

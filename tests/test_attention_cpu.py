@@ -106,6 +106,19 @@ def test_written_arrays_do_not_overlap_themselves(K, w, code):
         refused(K.attention_grad, grad_args(hk=4, grads=grads), code)
 
 
+@pytest.mark.parametrize("scale,ok", [(2.358e38, True), (2.36e38, False), (3.4028234e38, False), (1e-45, True)])
+def test_scales_whose_product_with_log2_e_is_not_finite(K, scale, ok):
+    """A score of zero times an infinite factor would be NaN.  (What is taken is refused for its
+    missing workspace, or has nothing to do.)"""
+    if not ok:
+        refused(K.attention, attention_args(scale=scale)[1] + [None, 0], FA_EINVAL)
+        refused(K.attention, attention_args(n=0, kn=0, scale=scale)[1] + [None, 0], FA_EINVAL)
+    else:
+        K.attention(*attention_args(n=0, kn=0, scale=scale)[1], None, 0)
+    refused(K.attention_grad, grad_args(ws=None, scale=scale), FA_ESCRATCH if ok else FA_EINVAL)
+    refused(K.attention_paged, paged_args(n=1000, h=8, hk=8, m=1000, ws=None, scale=scale), FA_ESCRATCH if ok else FA_EINVAL)
+
+
 def test_gradient_refuses_what_it_needs(K):
     refused(K.attention_grad, grad_args(lse=None), FA_EINVAL)
     refused(K.attention_grad, grad_args(dout=H(4, 64, data=None)), FA_EINVAL)
