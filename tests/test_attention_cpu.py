@@ -205,3 +205,7 @@ def test_limits_of_strides_and_launches(K):
     refused(K.attention_paged, paged_args(wb=1 << 62, **many), FA_ENOTSUP)       # many rows a sequence
     refused(K.attention_paged, paged_args(wb=1 << 62, m=most, **many), FA_ENOTSUP)  # one row a sequence
     refused(K.kv_append, append_args(n=1 << 24), FA_ENOTSUP)
+
+
+def test_version_tells_of_these_launchers(K):
+    assert K.lib.fa_version() >= 1003
