@@ -474,7 +474,7 @@ extern "C" size_t fa_attention_paged_workspace_bytes(int64_t n, int64_t heads, i
       (__int128)page_size * table_cols > AT_MOST_ROWS || check_shape(FA_F16, heads, kv_heads, head_dim) != 0)
     return 0;
   const int few = few_rows(n, heads, kv_heads, m);
-  if (few > 0) return few_workspace(few, n, heads, kv_heads, head_dim, m);
+  if (few > 0) return few_workspace(few, n, heads, kv_heads, head_dim, m, page_size * table_cols);
   const SplitPlan p = split_plan(n, heads, kv_heads, m, page_size * table_cols);
   if (p.splits == 1 || p.units > AT_MOST_BLOCKS) return 0;  // (more is refused)
   return (size_t)p.units * p.splits * AT_ROWS * ((head_dim <= 64 ? 64 : 128) + 2) * sizeof(float);

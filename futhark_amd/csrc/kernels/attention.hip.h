@@ -116,7 +116,8 @@ constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.693147180559945309f;
 // attention_few.hip: attention over the cache for few query rows a sequence.
 // Rows a unit of work holds for such a call, or 0 if the other kernel should take it.
 int few_rows(int64_t n, int64_t heads, int64_t kv_heads, int64_t m);
-size_t few_workspace(int rows, int64_t n, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t m);
+// Its workspace, 0 where one launch does it (`keys`: what a row of the table holds).
+size_t few_workspace(int rows, int64_t n, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t m, int64_t keys);
 int launch_few(hipStream_t stream, fa_dtype t, int rows, const AttentionArgs &a, void *workspace);
 
 // ------------------------------------------------------------------ segments

@@ -747,11 +747,12 @@ template <int D> static bool few_in_one_launch(int64_t units, int64_t keys) {
   return units * FEW_WAVES <= few_waves<D>() && keys <= (D == 128 ? 1024 : 1536);
 }
 
-size_t few_workspace(int rows, int64_t n, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t m) {
+size_t few_workspace(int rows, int64_t n, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t m, int64_t keys) {
+  const int64_t units = few_most_units(rows, n, heads / kv_heads, kv_heads, m);
+  if (head_dim <= 64 ? few_in_one_launch<64>(units, keys) : few_in_one_launch<128>(units, keys)) return 0;
   const int64_t floats = head_dim <= 64 ? few_part_floats(few_waves<64>(), rows, 64)
                                         : few_part_floats(few_waves<128>(), rows, 128);
-  return (size_t)floats * sizeof(float) + 16 +
-         (size_t)few_most_units(rows, n, heads / kv_heads, kv_heads, m) * sizeof(FewUnit);
+  return (size_t)floats * sizeof(float) + 16 + (size_t)units * sizeof(FewUnit);
 }
 
 template <class E, int D, int ROWS>

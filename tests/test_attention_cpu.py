@@ -209,3 +209,18 @@ def test_limits_of_strides_and_launches(K):
 
 def test_version_tells_of_these_launchers(K):
     assert K.lib.fa_version() >= 1003
+
+
+@pytest.mark.parametrize("h,hk,dim,keys", [(16, 4, 64, 1536), (32, 8, 128, 1024), (128, 2, 128, 16)])
+def test_what_takes_one_launch_needs_no_workspace(K, h, hk, dim, keys):
+    """Four short sequences of a token each: a block a unit, whose parts meet in LDS.  With one more
+    column the keys are cut over all waves, and parts go through the workspace."""
+    assert K.attention_paged_workspace_bytes(4, h, hk, dim, 4, 16, keys // 16) == 0
+    need = K.attention_paged_workspace_bytes(4, h, hk, dim, 4, 16, 1537 // 16 + 1)
+    assert need > 0
+    refused(K.attention_paged, paged_args(n=4, h=h, hk=hk, dim=dim, m=4, cols=97, wb=need - 1), FA_ESCRATCH)
+    refused(K.attention_paged, paged_args(n=4, h=h, hk=hk, dim=dim, m=4, cols=97, ws=None, wb=0), FA_ESCRATCH)
+
+
+def test_long_table_needs_a_workspace(K):
+    assert K.attention_paged_workspace_bytes(1, 8, 1, 128, 1, 16, 1 << 16) > 0

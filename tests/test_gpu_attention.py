@@ -1051,3 +1051,16 @@ def test_the_longest_table(K, n):
         assert bool(((out[i, 0].double() - o).abs() <= rel * o.abs()).all()), (i, out[i, 0], o)
         assert abs(lse[i, 0].item() - l.item()) <= -math.log(1 - chunk / 2 * 2.0 ** -24) + 0.01, (i, lse[i, 0], l)
     assert fail.item() == 0
+
+
+@pytest.mark.parametrize("t,h,hk,dim,page,new,past", [
+    ("f16", 16, 4, 64, 16, [1, 1, 1, 1], [500, 3, 1535, 90]),
+    ("bf16", 32, 8, 128, 16, [1, 2, 0, 1], [1000, 3, 500, 1023]),
+])
+def test_one_launch_without_a_workspace(K, t, h, hk, dim, page, new, past):
+    c = Cache(t, h, hk, dim, page, new, past, seed=130)
+    assert c.size == 0
+    K.attention_paged(stream(), t, view(c.q), c.n, h, hk, dim, c.offsets.data_ptr(), c.lens.data_ptr(), len(c.segs),
+                      c.past_lens.data_ptr(), c.scale, *c.cache(), view(c.out), c.lse.data_ptr(), None, 0,
+                      c.failure.data_ptr(), 6)
+    c.check()
