@@ -1064,3 +1064,165 @@ def test_one_launch_without_a_workspace(K, t, h, hk, dim, page, new, past):
                       c.past_lens.data_ptr(), c.scale, *c.cache(), view(c.out), c.lse.data_ptr(), None, 0,
                       c.failure.data_ptr(), 6)
     c.check()
+
+
+# ------------------------------------------------------- ways that calls above do not take
+@pytest.mark.parametrize("t,h,hk,dim,m,most_past", [
+    ("f16", 2, 1, 64, 300, 200),     # more sequences than threads of a block, a short line
+    ("bf16", 16, 8, 64, 300, 200),   # the same with more units than waves
+    ("bf16", 4, 2, 128, 600, 330),
+    ("f16", 6, 2, 96, 1025, 90),
+])
+def test_few_rows_of_many_sequences(K, t, h, hk, dim, m, most_past):
+    """A thread of a block counts several sequences; some are empty, one does not fit its table."""
+    new = [[1, 0, 1, 2, 1, 1, 3][i % 7] for i in range(m)]
+    c = Cache(t, h, hk, dim, 16, new, [(53 * i) % most_past for i in range(m)], gaps=(0, 1, 0), seed=140, extra_cols=99)
+    c.attend(K)
+    c.check()
+    bad = 2 * m // 3 - (2 * m // 3) % 7  # of one new token
+    c.past_lens[bad] = c.cols * 16
+    c.out.fill_(MARK)
+    c.lse.fill_(MARK)
+    c.attend(K)
+    assert c.failure.item() == 6
+    c.failure.zero_()
+    f, n = c.segs[bad]
+    assert n == 1 and bool((c.out[f:f + n] == MARK).all()) and bool((c.lse[f:f + n] == MARK).all())
+    keep = [i for i in range(m) if i != bad]
+    c.segs, c.past, c.table = [c.segs[i] for i in keep], [c.past[i] for i in keep], c.table[keep]
+    c.check()
+
+
+@pytest.mark.parametrize("t,h,hk,dim,new,past", [
+    ("bf16", 8, 2, 64, [(17 * i) % 80 for i in range(70)], [(211 * i) % 2000 for i in range(70)]),  # keys split
+    ("f16", 4, 1, 128, [40 + i % 9 for i in range(90)], [(97 * i) % 1500 for i in range(90)]),
+    ("f16", 64, 64, 128, [700, 3, 690], [100, 0, 310]),  # tiles of few sequences fill the chip
+])
+def test_many_rows_in_the_order_of_the_segments(K, t, h, hk, dim, new, past):
+    c = Cache(t, h, hk, dim, 16, new, past, gaps=(0, 2), seed=141)
+    c.attend(K)
+    c.check()
+
+
+@pytest.mark.parametrize("t,h,hk,dim,lens,causal", [
+    ("bf16", 4, 1, 128, [i % 6 for i in range(79)] + [2000], True),   # parts, more segments than lanes
+    ("f16", 8, 2, 64, [2300] + [(5 * i) % 9 for i in range(99)], False),
+    ("f16", 32, 32, 128, [2100, 20], True),                           # parts, many key heads
+])
+def test_split_key_tiles_in_the_order_of_the_segments(K, t, h, hk, dim, lens, causal):
+    p = Problem(t, h, hk, dim, lens, causal=causal, seed=142)
+    p.forward(K)
+    p.check_forward()
+    p.backward(K)
+    p.check_backward()
+
+
+# ------------------------------------------------------------------- ways against each other
+@pytest.mark.parametrize("i", range(len(PROMPTS)))
+def test_without_lse_the_same_bits(K, i):
+    p = Problem(*PROMPTS[i], seed=i)
+    p.forward(K)
+    out = p.out.clone()
+    p.out.fill_(MARK)
+    p.forward(K, lse=False)
+    assert torch.equal(out, p.out)
+
+
+@pytest.mark.parametrize("i", range(len(PAGED)))
+def test_paged_without_lse_the_same_bits(K, i):
+    *p, gaps, extra = PAGED[i]
+    c = Cache(*p, gaps=gaps, seed=200 + i, extra_cols=extra)
+    c.attend(K)
+    out = c.out.clone()
+    c.out.fill_(MARK)
+    c.attend(K, lse=False)
+    assert torch.equal(out, c.out)
+
+
+@pytest.mark.parametrize("t,h,hk,dim,page,new,past", [
+    ("bf16", 8, 2, 128, 16, [50, 1, 129], [0, 0, 0]),
+    ("f16", 4, 4, 64, 32, [1, 1, 1], [300, 0, 2000]),
+    ("bf16", 6, 2, 96, 8, [5, 200], [90, 700]),
+])
+def test_paged_and_packed_agree(K, t, h, hk, dim, page, new, past):
+    """The same attention over the cache and over its keys packed: within the sum of both bounds."""
+    c = Cache(t, h, hk, dim, page, new, past, seed=143)
+    c.attend(K)
+    c.check()
+    k, v, segs = c.gathered()
+    p = Problem(t, h, hk, dim, new, [n + s for n, s in zip(new, past)], seed=144)
+    assert p.segs_q == c.segs and p.segs_k == segs
+    p.q, p.k, p.v, p.nk = c.q, k, v, k.shape[0]
+    p.forward(K)
+    p.check_forward()
+    want, lse, tol_o, tol_l = ref.forward(t, p.q, k, v, c.segs, segs, c.scale, True)
+    live = ~lse.isnan()
+    ref.within(c.out[live], p.out[live].double(), 2 * tol_o[live])
+    ref.within(c.lse[live], p.lse[live].double(), 2 * tol_l[live])
+
+
+def test_a_serving_and_a_training_step_with_the_arrays_of_a_context(ctx, K):
+    """Cache append, attention over the cache and the gradient on a Futhark context's arrays and
+    stream; the context reads the results with its own calls."""
+    from futhark_amd import datagen as dg
+    h, hk, dim, page, lens = 4, 2, 64, 16, [40, 23]
+    n, offsets = sum(lens), [0, 40]
+    cols = max(-(-x // page) for x in lens)
+    pages = cols * len(lens) + 1
+    sizes = {"q": h, "k": hk, "v": hk, "dout": h}
+    bits = {x: dg.to_f16_bits(dg.normal_f32(90 + i, n * c * dim).reshape(1, n, c * dim))
+            for i, (x, c) in enumerate(sizes.items())}
+    arr = {x: ctx.new("f16_3d", b) for x, b in bits.items()}
+    for x, like in (("rotated", "q"), ("out", "q"), ("dq", "q"), ("dk", "k"), ("dv", "v")):
+        arr[x] = ctx.new("f16_3d", np.zeros_like(bits[like]))
+    for x in ("kp", "vp"):
+        arr[x] = ctx.new("f16_3d", np.zeros((pages * hk, page, dim), np.uint16))
+    table = np.arange(pages - 1, dtype=np.int32)[::-1].copy()
+    freqs = np.array([10000.0 ** (-j / 32) for j in range(32)], np.float32)
+    off, ln, zero = (ctx.new("i64_1d", np.array(x, np.int64)) for x in (offsets, lens, [0, 0]))
+    tab, fr, lse = ctx.new("i32_1d", table), ctx.new("f32_1d", freqs), ctx.new("f32_1d", np.zeros(n * h, np.float32))
+    fail = ctx.new("i32_1d", np.zeros(1, np.int32))
+    m, scale, width = 2, 1 / math.sqrt(dim), {**sizes, "rotated": h, "out": h, "dq": h, "dk": hk, "dv": hk}
+
+    def V(x):
+        return heads(arr[x].device_ptr, width[x] * dim, dim)
+
+    seg = (off.device_ptr, ln.device_ptr)
+    cache = (arr["kp"].device_ptr, arr["vp"].device_ptr, pages, page, tab.device_ptr, cols)
+    size = K.attention_paged_workspace_bytes(n, h, hk, dim, m, page, cols)
+    ws = ctx.new("u8_1d", np.zeros(max(size, 1), np.uint8))
+    K.kv_append(ctx.stream, "f16", V("q"), V("rotated"), V("k"), V("v"), n, h, hk, dim, *seg, m, zero.device_ptr,
+                fr.device_ptr, dim, 0, *cache, fail.device_ptr, 7)
+    K.attention_paged(ctx.stream, "f16", V("rotated"), n, h, hk, dim, *seg, m, zero.device_ptr, scale, *cache, V("out"),
+                      lse.device_ptr, ws.device_ptr, size, fail.device_ptr, 7)
+
+    def host(x):
+        return torch.from_numpy(arr[x].values().view(np.float16).reshape(n, -1, dim).copy())
+
+    pos = torch.cat([torch.arange(x) for x in lens])
+    f = torch.from_numpy(freqs)
+    q, k, v = (torch.from_numpy(bits[x].view(np.float16).reshape(n, -1, dim).copy()) for x in "qkv")
+    for x, want in (("rotated", ref.rotate(q, pos, f, dim, False)),):
+        ref.within(host(x), want, ref.U["f16"] * want.abs() + 4 * 2.0 ** -24 * 16 + ref.tiny("f16"))
+    stored = torch.from_numpy(arr["kp"].values().view(np.float16).reshape(pages, hk, page, dim).copy())
+    kd = torch.cat([stored[table[s * cols:(s + 1) * cols]].transpose(1, 2).reshape(-1, hk, dim)[:x]
+                    for s, x in enumerate(lens)])
+    want = ref.rotate(k, pos, f, dim, False)
+    ref.within(kd, want, ref.U["f16"] * want.abs() + 4 * 2.0 ** -24 * 16 + ref.tiny("f16"))
+    segs = list(zip(offsets, lens))
+    want, _, tol, _ = ref.forward("f16", host("rotated"), kd, v, segs, segs, scale, True)
+    ref.within(host("out"), want, tol)
+    # a training step on the prompts as they are
+    size = K.attention_grad_workspace_bytes(n, n, h, hk, dim, m)
+    ws2 = ctx.new("u8_1d", np.zeros(size, np.uint8))
+    args = ("f16", V("q"), n, V("k"), V("v"), n, h, hk, dim, *seg, *seg, m, scale, 1, V("out"))
+    K.attention(ctx.stream, *args, lse.device_ptr, fail.device_ptr, 7)
+    K.attention_grad(ctx.stream, *args, lse.device_ptr, V("dout"), V("dq"), V("dk"), V("dv"), ws2.device_ptr, size,
+                     fail.device_ptr, 7)
+    dout = torch.from_numpy(bits["dout"].view(np.float16).reshape(n, h, dim).copy())
+    grads, tols = ref.gradient("f16", q, k, v, dout, segs, segs, scale, True)
+    for x, want, tol in zip(("dq", "dk", "dv"), grads, tols):
+        ref.within(host(x), want, tol)
+    assert fail.values()[0] == 0
+    for x in (*arr.values(), off, ln, zero, tab, fr, lse, fail, ws, ws2):
+        x.free()
