@@ -17,7 +17,7 @@
 // product (the matrix units take nothing wider at this rate); sums stay f32.
 //
 // Bound by the matrix units at the clock that the card's power allows: nine prompts
-// of up to 8192 tokens, 32 + 8 heads of 128, 1.57 ms or 1.0 PFLOP/s, the units busy
+// of up to 8192 tokens, 32 + 8 heads of 128, 1.6 ms or 0.98 PFLOP/s, the units busy
 // half of the time at 1.9 GHz (a product of two 8192 x 8192 matrices: 1.38).  Two
 // blocks a CU hide each other's softmax; one with 64 rows a wave, half the LDS reads
 // and products and weights issued in turn by hand ran at 2.3 GHz and took 1.84 ms.
@@ -401,7 +401,9 @@ template <class E, int D> __global__ __launch_bounds__(AT_THREADS) void attentio
 // time (two a CU).  Several are ragged: twice as many, at least 256 keys to a block.
 // (Twenty chunks of up to 300 tokens behind up to 4096 105 -> 74 us, two of 32 heads
 // without groups 184 -> 117; six of up to 1024 behind up to 8192, which fill the chip
-// unsplit, 266 -> 280.  Three times as many: 93, 127, 279.)
+// unsplit, 266 -> 280.  Three times as many: 93, 127, 279.)  A table much wider than
+// its sequences are long is split too coarsely: 100 tokens behind 8092 take 42 us with
+// a table of their length and 203 with one of 131072 positions.
 struct SplitPlan {
   int64_t units;
   int chunk, splits;

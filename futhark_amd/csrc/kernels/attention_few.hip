@@ -14,11 +14,12 @@
 //
 // The products are 16 x 16 x 32: S^T = K Q^T with 16 query rows as columns, and
 // O^T += V^T P^T with the weights as right operand in the registers they are
-// computed in.
+// computed in.  They are rounded to the element type once, for that product, which
+// takes nothing wider; sums and statistics are f32.
 //
 // 64 sequences of up to 8192 keys, 8 key heads of 128: 518 MB in 88 us, 5.9 TB/s
 // (reading alone reaches 6.1 to 6.9), and 5 us for the second kernel; one of 131072:
-// 85 + 9 us.  Tens of microseconds and less are the chain lengths, page numbers,
+// 89 + 9 us.  Tens of microseconds and less are the chain lengths, page numbers,
 // keys, weights: four of up to 500 keys 7.8 us.
 #include "attention.hip.h"
 
@@ -742,7 +743,9 @@ static int64_t few_most_units(int rows, int64_t n, int64_t group, int64_t kv_hea
 // of the line and the second launch.  (Heads of 128, 4 to 32 sequences of up to 512
 // keys 12.7 us against 16 to 19 on the line, of 1040 19 against 17, of 2048 31
 // against 21; heads of 64, 500 keys 9.7 against 13.9, 1040 11.4 against 14.5, 2048
-// 20 against 22 where units fill the chip, 4000 30 against 15.5.)
+// 20 against 22 where units fill the chip, 4000 30 against 15.5.)  Only the table's
+// width is known here: four sequences of up to 500 keys take 15 us behind a table of
+// 16384 positions.
 template <int D> static bool few_in_one_launch(int64_t units, int64_t keys) {
   return units * FEW_WAVES <= few_waves<D>() && keys <= (D == 128 ? 1024 : 1536);
 }

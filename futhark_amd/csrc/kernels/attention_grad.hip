@@ -3,8 +3,10 @@
 // Both are bound by the matrix units at the clock that power allows, on long
 // sequences 1.2 and 1.08 PFLOP/s of the products they compute (one of 8192 tokens,
 // not causal, 32 + 8 heads of 128: 1.36 and 2.04 ms).  On ragged ones (five of up
-// to 4096: 255 and 390 us, the units busy 55 and 43 % of the time) about 13 us of a
-// key tile are its beginning and end.
+// to 4096: 271 and 430 us on average under the profiler, 261 and 394 at best, the
+// units busy 55 and 43 % of the time) about 13 us of a key tile are its beginning and
+// end.  Weights and derivatives of scores are rounded to the element type once, for
+// the products that they enter; sums, shifts and D are f32.
 #include "attention.hip.h"
 
 namespace fa {

@@ -421,6 +421,8 @@ int fa_attention_grad(fa_stream_t stream, fa_dtype t, const fa_heads *q, int64_t
  * (FA_ENOTSUP otherwise), 16-byte aligned; page_table is [m][table_cols] i32,
  * and position p of sequence i lives in slot p % page_size of page
  * page_table[i][p / page_size].  table_cols * page_size is at most 2^31 - 4096.
+ * How attention splits its work follows from the table's width, not from lengths:
+ * a table little wider than the longest sequence is the fastest.
  * Sequence i holds past_lens[i] tokens before the new ones, lens[i] tokens at
  * rows offsets[i]...; past + new must fit its table row.
  *
