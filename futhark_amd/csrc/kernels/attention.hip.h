@@ -246,8 +246,8 @@ __device__ __forceinline__ void find_tile_by_keys(bool ok, int64_t first, int64_
 // keys: where the chip holds half of them or more at a time (two blocks a CU, three
 // for D = 64).  With more the long ones even out, and tiles of one segment next to
 // each other share their keys in L2.  (600 units of six sequences with up to 8192
-// cached tokens, not split over keys, 288 -> 267 us, 1100 of forty prompts of up to 333 15.4 -> 13.5; but
-// 1400 of twenty sequences, forward and gradient, 290 -> 306.)
+// cached tokens, not split over keys, 288 -> 267 us, 1100 of forty prompts of up to
+// 333 15.4 -> 13.5; but 1400 of twenty sequences, forward and gradient, 290 -> 306.)
 inline bool takes_by_keys(int64_t units, int64_t m, int64_t dim) {
   return m <= WAVE && units <= 2 * NUM_CUS_HINT * (dim <= 64 ? 3 : 2);
 }

@@ -8,8 +8,8 @@
 // in the order they were asked for: the segments come first, the rows behind them,
 // and the page number past both by the scalar cache, so that looking up the place
 // and computing the angles hide behind the rows (14555 tokens of 32 + 8 heads of
-// 128: 79 -> 58 us a call, 6.1 TB/s).  Loads and stores are non-temporal: nothing is used
-// twice (88 -> 78 us before that).  32 tokens: 4.5 us, launch and the chain.
+// 128: 79 -> 58 us a call, 6.1 TB/s).  Loads and stores are non-temporal: nothing is
+// used twice (88 -> 78 us before that).  32 tokens: 4.5 us, launch and the chain.
 #include "attention.hip.h"
 
 namespace fa {
